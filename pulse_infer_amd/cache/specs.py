@@ -28,8 +28,8 @@ another, say) answers with a ``CombinedSpec`` of their specs; each of them is
 then served as if it were a run's own, and the run is handed the tuple of
 their views.
 
-Two specs are provided: keys and values of attention heads in pages, and a plain
-array per request.  A mixer that pages something else per token (one row of some
+Three specs are provided: keys and values of attention heads in pages, as they are
+or in 8 bits with scales, and a plain array per request.  A mixer that pages something else per token (one row of some
 width, keys and values of different widths, the tail of a convolution) brings a
 spec class of its own with these members; nothing in the cache manager or the
 step function changes.
@@ -47,6 +47,20 @@ class PagedCacheView:
     group: int
     keys: Any              # [pages, kv_heads, page_size, head_dim]
     values: Any            # [pages, kv_heads, head_dim, page_size]
+    page_size: int
+    writable: bool = True  # False: the run reads a cache that another run writes
+
+
+@dataclass
+class Paged8CacheView:
+    """The pages of one run of a group of attention layers whose keys and values are held in 8 bits (e4m3 bytes; a scale
+    for the keys and one for the values of every block and head, powers of two, a value scale negative where the block
+    holds a value that is not finite)."""
+
+    group: int
+    keys: Any              # float8_e4m3fn [pages, kv_heads, page_size, head_dim]
+    values: Any            # float8_e4m3fn [pages, kv_heads, page_size / block, head_dim, block]
+    scales: Any            # float32 [pages, kv_heads, page_size / block, 2]: of the keys, of the values
     page_size: int
     writable: bool = True  # False: the run reads a cache that another run writes
 
@@ -89,6 +103,44 @@ class PagedKVSpec:
                               writable=writable)
 
     def tensors(self, storage: Tuple[Any, Any]) -> List[Any]:
+        return list(storage)
+
+
+def block_tokens(page_size: int) -> int:
+    """Tokens that share a scale in a cache of 8 bits: 16, or a whole page whose size 16 does not divide."""
+    return 16 if page_size % 16 == 0 else page_size
+
+
+@dataclass(frozen=True)
+class Paged8KVSpec:
+    """``PagedKVSpec`` in 8 bits, whatever the run's storage type.  Storage: K ``[runs, pages, kv_heads, page, head_dim]``, V ``[runs,
+    pages, kv_heads, page / block, head_dim, block]`` (a channel's tokens of a block together: 16 bytes, a matrix-core operand's
+    load), scales ``[runs, pages, kv_heads, page / block, 2]``."""
+
+    num_kv_heads: int
+    head_dim: int
+    window: Optional[int] = None
+    chunk: Optional[int] = None
+
+    per_token = True
+
+    def bytes_per_token(self, element_size: int) -> int:
+        return 2 * self.num_kv_heads * self.head_dim + (8 * self.num_kv_heads + 15) // 16
+
+    def allocate(self, runs: int, units: int, page_size: int, device: Any, dtype: Any) -> Tuple[Any, Any, Any]:
+        import torch
+
+        block, heads, d = block_tokens(page_size), self.num_kv_heads, self.head_dim
+        shapes = ((runs, units, heads, page_size, d), (runs, units, heads, page_size // block, d, block))
+        keys, values = (torch.zeros(s, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for s in shapes)
+        return keys, values, torch.zeros((runs, units, heads, page_size // block, 2), dtype=torch.float32, device=device)
+
+    def view(self, storage: Tuple[Any, Any, Any], index: int, group: int, page_size: int, writable: bool) -> Paged8CacheView:
+        keys, values, scales = storage
+        return Paged8CacheView(group=group, keys=keys[index], values=values[index], scales=scales[index], page_size=page_size,
+                               writable=writable)
+
+    def tensors(self, storage: Tuple[Any, Any, Any]) -> List[Any]:
         return list(storage)
 
 

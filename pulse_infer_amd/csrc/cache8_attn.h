@@ -1,0 +1,42 @@
+// What the kernels of attention over a cache in 8 bits take.
+#pragma once
+
+#include "cache8.h"
+
+// The C entry points' arguments (ops/cache8.py fills it; the same fields in the same order).
+struct PulseAttn8 {
+    const void* q;               // [tokens, >= nq * d], rows q_stride elements apart
+    int64_t q_stride;
+    void* out;                   // [tokens, >= nq * d]
+    int64_t o_stride;
+    const uint8_t *keys, *values;
+    const float* scales;
+    const int *positions, *token_entry, *table;
+    const void* gate;            // logits of an output gate, [tokens, nq] or [tokens, nq * gate_width]; null: none
+    int64_t gate_stride;
+    const float* sink;           // [nq]: exp(sink) is one more term of the head's denominator; null: none
+    const int* items;            // the matrix-core kernels' work: (first row, rows, entry, 0) a piece, and how it is cut (attn8_cut)
+    const int* cut;
+    float *part_o, *part_ml;
+    int dtype, tokens, entries, table_width, nq, nkv, d, page_size, num_pages, window, chunk, gate_width, n_items, max_work;
+    float scale, softcap;
+};
+
+namespace cache8 {
+
+constexpr int TILE = 64;         // keys of a step of the matrix-core kernels
+
+// The lowest key that a token at `pos` sees.
+__device__ __forceinline__ int low_key(int window, int chunk, int pos) {
+    if (chunk > 0) return pos > 0 ? pos / chunk * chunk : 0;
+    return window > 0 ? max(0, pos - window + 1) : 0;
+}
+__device__ __forceinline__ float tanh_of(float x) { return 1.f - 2.f / (__expf(2.f * x) + 1.f); }
+__device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + __expf(-x)); }
+
+// Where a cut says what it found: the number of pieces, then the pieces (item, first tile, end, the item's first piece), then for every
+// item its first piece and how many it has.
+constexpr int CUT_HEAD = 4;
+__host__ __device__ inline int64_t cut_ints(int n_items, int max_work) { return CUT_HEAD + 4 * static_cast<int64_t>(max_work) + 2 * static_cast<int64_t>(n_items); }
+
+}  // namespace cache8

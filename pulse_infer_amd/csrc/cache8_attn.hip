@@ -1,0 +1,742 @@
+// Attention over a cache in 8 bits (cache8.h) on the matrix cores: bfloat16 rows, heads of a multiple of 32 channels up to 256, pages of a
+// multiple of 16 tokens.  Bytes become bfloat16 on their way into the matrix cores' operands (three bits of fraction: exactly), with the
+// block's scale applied by the same instruction; products, maxima, sums and accumulators are float32.  Weights are rounded to bfloat16
+// for the second product (a relative 2^-8 at most, as q was), the sum that divides them is of the unrounded ones.
+//
+// A piece of work is an item (some rows of one request that share a kv head: "columns", a head of a row each) and a stretch of tiles of
+// 64 keys.  Everything is kept transposed, so that a column stays in its lanes:
+//   S^T[key, col] = K[key, :] . q[col, :]      P^T = exp2(S^T c - m[col])      O^T[ch, col] += V^T[ch, key] P^T[key, col]
+//
+// attn8_cut      shares the tiles of all items out over a number of pieces: T = the least length for which sum ceil(tiles / T) fits, an
+//                item in equal pieces of at most T.  Made on the device from the positions, once a step for all layers, so that a
+//                recorded step's replays bring their own lengths.
+// attn8_few      up to 16 columns an item (a decoded token's heads; a few tokens).  Its four wavefronts take every fourth tile and
+//                meet at the end.  Bound by reading the cache.
+// attn8_many     128 columns an item (portions of prompts).  A tile is converted once for all and lies in LDS as bfloat16.
+// attn8_join     joins the pieces of items that were cut.
+#include "cache8_attn.h"
+
+#include <algorithm>
+
+int pulse_attn8_check(const PulseAttn8* a, const char* what);
+
+namespace {
+
+using cache8::TILE;
+
+constexpr int THREADS = 256, WAVES = THREADS / PULSE_WAVE;
+constexpr int FEW = 16, MANY = 128;
+constexpr float LOG2E = 1.44269504088896340736f;
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Eight bytes times a power of two, as a matrix-core operand.
+__device__ __forceinline__ bf16x8 operand(uint32_t lo, uint32_t hi, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// The same with nothing in the place of what is not a number, and ones (else zeros) in those places.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {    // 0xff in every byte that is NaN (0x7f, 0xff)
+    const uint32_t m = w & 0x7f7f7f7fu, t = (m + 0x01010101u) & 0x80808080u;
+    return (t >> 7) * 0xffu;
+}
+__device__ __forceinline__ bf16x8 ones_at(uint32_t lo, uint32_t hi) {     // 0x38: one
+    return operand(nan_bytes(lo) & 0x38383838u, nan_bytes(hi) & 0x38383838u, 1.f);
+}
+
+// A score in the units of exp2: the cap, if there is one, takes the place of the factor.
+struct Score {
+    float factor, cap_in, cap_out;
+    __device__ __forceinline__ float operator()(float s) const { return cap_out * cache8::tanh_of(s * cap_in); }
+};
+__device__ __forceinline__ Score score_of(const PulseAttn8& a) {
+    if (a.softcap > 0.f) return {1.f, a.scale / a.softcap, a.softcap * LOG2E};
+    return {a.scale * LOG2E, 0.f, 0.f};
+}
+
+// What a column's sums are multiplied by at the end: its denominator with the sink in it, and its head's gate.
+__device__ __forceinline__ float finish(const PulseAttn8& a, float m, float l, int row, int head) {
+    if (a.sink) l += __builtin_amdgcn_exp2f(a.sink[head] * LOG2E - (m == -INFINITY ? 0.f : m));
+    float inv = l == 0.f ? 0.f : 1.f / l;
+    if (a.gate && a.gate_width == 0) inv *= cache8::sigmoid_of(bf16_to_f32(static_cast<const bf16_t*>(a.gate)[row * a.gate_stride + head]));
+    return inv;
+}
+__device__ __forceinline__ float channel_gate(const PulseAttn8& a, int row, int head, int ch) {
+    if (!a.gate || ch >= a.gate_width) return 1.f;
+    return cache8::sigmoid_of(bf16_to_f32(static_cast<const bf16_t*>(a.gate)[row * a.gate_stride + static_cast<int64_t>(head) * a.gate_width + ch]));
+}
+
+// Four channels of a row, each times its factor.
+template <typename F>
+__device__ __forceinline__ void store4(bf16_t* to, f32x4 x, F factor) {
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = f32_to_bf16(x[e] * factor(e));
+    *reinterpret_cast<uint2*>(to) = make_uint2(y[0] | y[1] << 16, y[2] | y[3] << 16);
+}
+
+// ------------------------------------------------------------------------------------------------------------------ the cut
+__global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restrict__ items, int n, const int* __restrict__ positions,
+                                                            int window, int chunk, int slots, int least, int max_work, int* cut) {
+    __shared__ int s_wave[WAVES];
+    const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = tid / PULSE_WAVE;
+    auto tiles = [&](int i, int& first) {
+        const int4 it = items[i];
+        const int hi = positions[it.x + it.y - 1], lo = cache8::low_key(window, chunk, positions[it.x]);
+        first = lo / TILE;
+        return max(hi / TILE + 1 - first, 1);
+    };
+    int mine = 0, unused;
+    for (int i = tid; i < n; i += THREADS) mine += tiles(i, unused);
+    mine = wave_sum(mine);
+    if (lane == 0) s_wave[wave] = mine;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) total += s_wave[w];
+    const int length = max(least, (total + slots - 1) / slots);
+    int4* work = reinterpret_cast<int4*>(cut + cache8::CUT_HEAD);
+    int2* info = reinterpret_cast<int2*>(cut + cache8::CUT_HEAD + 4 * max_work);
+    int before = 0;
+    for (int base = 0; base < n; base += THREADS) {
+        const int i = base + tid;
+        int first = 0, count = 0, pieces = 0, each = 1;
+        if (i < n) {
+            count = tiles(i, first);
+            pieces = (count + length - 1) / length;
+            each = (count + pieces - 1) / pieces;
+            pieces = (count + each - 1) / each;
+        }
+        int sum = pieces;
+#pragma unroll
+        for (int step = 1; step < PULSE_WAVE; step *= 2) {
+            const int other = __shfl_up(sum, step);
+            sum += lane >= step ? other : 0;
+        }
+        __syncthreads();
+        if (lane == PULSE_WAVE - 1) s_wave[wave] = sum;
+        __syncthreads();
+        int at = before + sum - pieces, all = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            at += w < wave ? s_wave[w] : 0;
+            all += s_wave[w];
+        }
+        before += all;
+        if (i < n) {
+            info[i] = make_int2(at, pieces);
+            for (int z = 0; z < pieces && at + z < max_work; ++z)
+                work[at + z] = make_int4(i, first + z * each, min(first + count, first + (z + 1) * each), at);
+        }
+    }
+    if (tid == 0) cut[0] = min(before, max_work);
+}
+
+// --------------------------------------------------------------------------------------------------------- up to 16 columns
+// Lane l holds row l % 16 of an operand and its 8 numbers 8 (l / 16) .., and gets back rows 4 (l / 16) .. of column l % 16.  Which key or
+// channel a row or number stands for is free as long as both operands agree, so that every load is of 16 neighbouring bytes and no
+// weight changes its lane: row 4 b + i of score tile t is key 4 t + i of the tile's block b, so that lane group b holds the 16 keys of block
+// b; those are, eight by eight, the numbers of the second product, whose other operand is a channel's 16 bytes of the block.
+template <int D>
+struct Few {
+    static constexpr int K16 = D / 64, K8 = D % 64 / 32, STEPS = D / 32, MT = D / 16;
+    u32x4 k[4][K16 ? K16 : 1];
+    uint2 k8[4];
+    u32x4 v[MT];
+    float ks, vs;          // of the lane's row's block, of the lane's own block (negative: it holds values that are not finite)
+    bool there;            // the lane's own block
+};
+
+template <int D>
+__global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(PulseAttn8 a, cache8::Div blocks, int head_groups) {
+    using F = Few<D>;
+    __shared__ float s_o[WAVES][FEW][D + 4];
+    __shared__ float s_m[WAVES][FEW], s_l[WAVES][FEW];
+    const int w = blockIdx.y;
+    if (w >= uniform(a.cut[0])) return;
+    const int4 job = reinterpret_cast<const int4*>(a.cut + cache8::CUT_HEAD)[w];
+    const int item = uniform(job.x), tile_end = uniform(job.z), first_piece = uniform(job.w);
+    const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::CUT_HEAD + 4 * a.max_work)[item];
+    const bool whole = uniform(info.y) == 1;
+    const int4 it = reinterpret_cast<const int4*>(a.items)[item];
+    const int row0 = uniform(it.x), ntok = uniform(it.y), entry = uniform(it.z);
+    const int g = blockIdx.x / head_groups, part = blockIdx.x % head_groups;
+    const int group = a.nq / a.nkv, heads = min(group - part * FEW, FEW);
+    const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = uniform(tid / PULSE_WAVE);
+    const int r = lane % 16, b = lane / 16;
+    const int hi = uniform(a.positions[row0 + ntok - 1]), pos0 = uniform(a.positions[row0]);
+    const int lo = cache8::low_key(a.window, a.chunk, pos0), lo_last = cache8::low_key(a.window, a.chunk, hi);
+
+    // this lane's column: token r / heads, head r % heads
+    const int tok = r / heads;
+    const bool col_ok = tok < ntok;
+    const int col_row = row0 + (col_ok ? tok : 0), head = g * group + part * FEW + r % heads;
+    const int pos = col_ok ? a.positions[col_row] : -1, low = cache8::low_key(a.window, a.chunk, pos);
+    bf16x8 q[F::STEPS];
+    {
+        const bf16_t* from = static_cast<const bf16_t*>(a.q) + col_row * a.q_stride + static_cast<int64_t>(head) * D;
+        const bf16x8 none = {};
+#pragma unroll
+        for (int j = 0; j < F::K16; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) q[2 * j + s] = col_ok ? *reinterpret_cast<const bf16x8*>(from + 64 * j + 16 * b + 8 * s) : none;
+        if constexpr (F::K8) q[F::STEPS - 1] = col_ok ? *reinterpret_cast<const bf16x8*>(from + 64 * F::K16 + 8 * b) : none;
+    }
+    const Score score = score_of(a);
+    const int* bt = a.table + static_cast<int64_t>(entry) * a.table_width;
+
+    // where a tile's blocks lie: of the lane's row (block r / 4) and its own (block b)
+    struct Place { int pk, pv; };
+    auto find = [&](int tile) {
+        const int ik = blocks.over(4 * tile + r / 4), iv = blocks.over(4 * tile + b);
+        return Place{bt[min(ik, a.table_width - 1)], bt[min(iv, a.table_width - 1)]};
+    };
+    auto load = [&](int tile, Place at, F& x) {
+        const int nk = 4 * tile + r / 4, nv = 4 * tile + b;
+        auto there = [&](int n, int page) {
+            return page >= 0 && page < a.num_pages && blocks.over(n) < a.table_width && 16 * n <= hi && 16 * n + 15 >= lo;
+        };
+        const bool on_k = there(nk, at.pk);
+        x.there = there(nv, at.pv);
+        const int64_t hk = static_cast<int64_t>(on_k ? at.pk : 0) * a.nkv + g, hv = static_cast<int64_t>(x.there ? at.pv : 0) * a.nkv + g;
+        const int ik = on_k ? blocks.rest(nk) : 0, iv = x.there ? blocks.rest(nv) : 0;
+        const int64_t bk = hk * blocks.b + ik, bv = hv * blocks.b + iv;
+        const uint8_t* kp = a.keys + bk * (16 * D) + (r % 4) * D;
+        const uint8_t* vp = a.values + bv * (16 * D) + r * 16;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int j = 0; j < F::K16; ++j) x.k[t][j] = *reinterpret_cast<const u32x4*>(kp + 4 * t * D + 64 * j + 16 * b);
+            if constexpr (F::K8) x.k8[t] = *reinterpret_cast<const uint2*>(kp + 4 * t * D + 64 * F::K16 + 8 * b);
+        }
+#pragma unroll
+        for (int m = 0; m < F::MT; ++m) x.v[m] = *reinterpret_cast<const u32x4*>(vp + m * 256);
+        x.ks = a.scales[2 * bk];
+        x.vs = a.scales[2 * bv + 1];
+    };
+
+    f32x4 o[F::MT];
+#pragma unroll
+    for (int m = 0; m < F::MT; ++m) o[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, l = 0.f;
+
+    auto compute = [&](int tile, F& x) {
+        const int j0 = tile * TILE;
+        f32x4 s[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < F::K16; ++j) {
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(x.k[t][j][0], x.k[t][j][1], x.ks), q[2 * j], s[t], 0, 0, 0);
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(x.k[t][j][2], x.k[t][j][3], x.ks), q[2 * j + 1], s[t], 0, 0, 0);
+            }
+            if constexpr (F::K8) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(x.k8[t].x, x.k8[t].y, x.ks), q[F::STEPS - 1], s[t], 0, 0, 0);
+        }
+        if (a.softcap > 0.f) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][i] = score(s[t][i]);
+        }
+        // key j0 + 16 b + 4 t + i
+        const int from = low - j0 - 16 * b, to = x.there ? pos - j0 - 16 * b : -1;
+        const bool masked = j0 + TILE - 1 > pos0 || j0 < lo_last || __any(!x.there);
+        if (masked) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][i] = 4 * t + i >= from && 4 * t + i <= to ? s[t][i] : -INFINITY;
+            // (what was read in the place of a block that is not there)
+#pragma unroll
+            for (int m = 0; m < F::MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x.v[m][i] = x.there ? x.v[m][i] : 0u;
+        }
+        float best = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) best = fmaxf(best, s[t][i]);
+        best = across_rows(best, LaneMax()) * score.factor;
+        const float now = fmaxf(top, best);
+        if (__any(now > top)) {
+            const float again = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
+            l *= again;
+#pragma unroll
+            for (int m = 0; m < F::MT; ++m) o[m] *= again;
+            top = now;
+        }
+        const float shift = top == -INFINITY ? 0.f : -top;
+        bf16x8 p[2];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i], score.factor, shift));
+                l += e;
+                p[t / 2][4 * (t % 2) + i] = static_cast<__bf16>(e);
+            }
+        const float vs = fabsf(x.vs);
+        if (__builtin_expect(__any(x.there && x.vs < 0.f), 0)) {
+            // Values that are not finite belong to those who see them alone: they are left out of the sums, and a column that sees one
+            // in a channel (a product of ones says so) gets NaN there.
+            bf16x8 see[2];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) see[t / 2][4 * (t % 2) + i] = static_cast<__bf16>(4 * t + i >= from && 4 * t + i <= to ? 1.f : 0.f);
+#pragma unroll
+            for (int m = 0; m < F::MT; ++m) {
+                f32x4 bad = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    bad = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones_at(x.v[m][2 * u], x.v[m][2 * u + 1]), see[u], bad, 0, 0, 0);
+                    x.v[m][2 * u] &= ~nan_bytes(x.v[m][2 * u]);
+                    x.v[m][2 * u + 1] &= ~nan_bytes(x.v[m][2 * u + 1]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[m][i] = bad[i] > 0.f ? __builtin_nanf("") : o[m][i];
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < F::MT; ++m) {
+            o[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(x.v[m][0], x.v[m][1], vs), p[0], o[m], 0, 0, 0);
+            o[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(x.v[m][2], x.v[m][3], vs), p[1], o[m], 0, 0, 0);
+        }
+    };
+
+    int tile = uniform(job.y) + wave;
+    if (tile < tile_end) {
+        F now, next;
+        load(tile, find(tile), now);
+        Place ahead = find(tile + WAVES);
+        for (; tile < tile_end; tile += WAVES) {
+            const bool more = tile + WAVES < tile_end;
+            if (more) {
+                load(tile + WAVES, ahead, next);
+                ahead = find(tile + 2 * WAVES);
+            }
+            compute(tile, now);
+            if (more) now = next;
+        }
+    }
+    l = across_rows(l, LaneSum());
+
+    // the four wavefronts' columns meet
+    if (b == 0) {
+        s_m[wave][r] = top;
+        s_l[wave][r] = l;
+    }
+#pragma unroll
+    for (int m = 0; m < F::MT; ++m) *reinterpret_cast<f32x4*>(&s_o[wave][r][16 * m + 4 * b]) = o[m];
+    __syncthreads();
+    const int64_t at = (static_cast<int64_t>(w) * gridDim.x + blockIdx.x) * FEW;
+    constexpr int QUADS = D / 4;
+    for (int i = tid; i < FEW * QUADS; i += THREADS) {
+        const int c = i / QUADS, ch = i % QUADS * 4;
+        if (c >= ntok * heads) break;
+        float m = s_m[0][c], sum = 0.f;
+#pragma unroll
+        for (int v = 1; v < WAVES; ++v) m = fmaxf(m, s_m[v][c]);
+        f32x4 all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) {
+            const float f = s_m[v][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[v][c] - m);
+            // (a wavefront that has seen no key has zeros, or NaN for a column that saw a value that is none: kept)
+            sum += s_l[v][c] * f;
+            all += *reinterpret_cast<const f32x4*>(&s_o[v][c][ch]) * f;
+        }
+        const int row = row0 + c / heads, hd = g * group + part * FEW + c % heads;
+        if (whole) {
+            const float inv = finish(a, m, sum, row, hd);
+            bf16_t* to = static_cast<bf16_t*>(a.out) + row * a.o_stride + static_cast<int64_t>(hd) * D + ch;
+            store4(to, all, [&](int e) { return inv * channel_gate(a, row, hd, ch + e); });
+        } else {
+            *reinterpret_cast<f32x4*>(a.part_o + (at + c) * D + ch) = all;
+            if (ch == 0) {
+                a.part_ml[2 * (at + c)] = m;
+                a.part_ml[2 * (at + c) + 1] = sum;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ 128 columns
+// A wavefront takes 32 columns: lane l supplies row l % 32 of an operand and its 8 numbers 8 (l / 32) .., and gets back rows
+// 8 (i / 4) + 4 (l / 32) + i % 4, i < 16, of column l % 32.  The values lie in LDS in the order in which the weights come out of the
+// first product: of 16 keys the lanes of half h hold 4 h .. and 8 + 4 h .., which are one piece of 16 bytes.  Rows are 16 bytes longer than
+// they have to be, so that the eight rows that are read in a cycle lie in different banks.
+template <int D>
+__global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(PulseAttn8 a, cache8::Div blocks) {
+    constexpr int KROW = D + 8, VROW = TILE + 8;                 // in bfloat16 numbers
+    constexpr int PIECES = 4 * D, TURNS = (PIECES + THREADS - 1) / THREADS, STEPS = D / 16, MT = D / 32;
+    __shared__ __attribute__((aligned(16))) bf16_t s_k[2][TILE * KROW];
+    __shared__ __attribute__((aligned(16))) bf16_t s_v[2][D * VROW];
+    const int w = blockIdx.y;
+    if (w >= uniform(a.cut[0])) return;
+    const int4 job = reinterpret_cast<const int4*>(a.cut + cache8::CUT_HEAD)[w];
+    const int item = uniform(job.x), tile_begin = uniform(job.y), tile_end = uniform(job.z);
+    const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::CUT_HEAD + 4 * a.max_work)[item];
+    const bool whole = uniform(info.y) == 1;
+    const int4 it = reinterpret_cast<const int4*>(a.items)[item];
+    const int row0 = uniform(it.x), ntok = uniform(it.y), entry = uniform(it.z);
+    const int g = blockIdx.x, group = a.nq / a.nkv;
+    const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = uniform(tid / PULSE_WAVE);
+    const int r = lane % 32, half = lane / 32;
+    const int hi = uniform(a.positions[row0 + ntok - 1]), pos0 = uniform(a.positions[row0]);
+    const int lo = cache8::low_key(a.window, a.chunk, pos0);
+
+    const int col = wave * 32 + r, tok = col / group;
+    const bool col_ok = tok < ntok;
+    const int col_row = row0 + (col_ok ? tok : 0), head = g * group + (col_ok ? col - tok * group : 0);
+    const int pos = col_ok ? a.positions[col_row] : -1, low = cache8::low_key(a.window, a.chunk, pos);
+    // the wavefront's first and last position (its columns' tokens follow each other), -1 where it has no column
+    const int w_tok0 = wave * 32 / group, w_tok1 = min((wave * 32 + 31) / group, ntok - 1);
+    const bool w_any = w_tok0 < ntok;
+    const int w_first = w_any ? uniform(a.positions[row0 + w_tok0]) : -1, w_last = w_any ? uniform(a.positions[row0 + w_tok1]) : -1;
+    const int w_low = cache8::low_key(a.window, a.chunk, w_first), w_low_last = cache8::low_key(a.window, a.chunk, w_last);
+
+    bf16x8 q[STEPS];
+    {
+        const bf16_t* from = static_cast<const bf16_t*>(a.q) + col_row * a.q_stride + static_cast<int64_t>(head) * D;
+        const bf16x8 none = {};
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) q[s] = col_ok ? *reinterpret_cast<const bf16x8*>(from + 16 * s + 8 * half) : none;
+    }
+    const Score score = score_of(a);
+    const int* bt = a.table + static_cast<int64_t>(entry) * a.table_width;
+
+    // A tile's bytes: keys in pieces of 16 channels, values in pieces of a channel's 16 tokens of a block.
+    struct Raw {
+        u32x4 k[TURNS], v[TURNS];
+        float ks[TURNS], vs[TURNS];
+        bool bad;              // a block of the tile holds values that are not finite
+    };
+    auto place = [&](int n, int page, bool& there) {
+        there = page >= 0 && page < a.num_pages && blocks.over(n) < a.table_width && 16 * n <= hi && 16 * n + 15 >= lo;
+        return ((static_cast<int64_t>(there ? page : 0) * a.nkv + g) * blocks.b + (there ? blocks.rest(n) : 0));
+    };
+    struct Pages { int p[4]; };
+    auto find = [&](int tile) {
+        Pages x;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x.p[b] = bt[min(blocks.over(4 * tile + b), a.table_width - 1)];
+        return x;
+    };
+    auto load = [&](int tile, const Pages& pages, Raw& x) {
+        int64_t at[4];
+        bool there[4];
+        x.bad = false;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            at[b] = place(4 * tile + b, uniform(pages.p[b]), there[b]);
+            x.bad |= there[b] && a.scales[2 * at[b] + 1] < 0.f;
+        }
+        auto pick = [&](int b) { return b == 0 ? at[0] : b == 1 ? at[1] : b == 2 ? at[2] : at[3]; };
+        auto on = [&](int b) { return b == 0 ? there[0] : b == 1 ? there[1] : b == 2 ? there[2] : there[3]; };
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            const int n = tid + i * THREADS;
+            x.k[i] = x.v[i] = u32x4{0u, 0u, 0u, 0u};
+            x.ks[i] = x.vs[i] = 1.f;
+            if (PIECES % THREADS == 0 || n < PIECES) {
+                const int kr = n / (D / 16), kc = n % (D / 16), vb = n / D, vc = n % D;
+                const int64_t ak = pick(kr / 16), av = pick(vb);
+                if (on(kr / 16)) {
+                    x.k[i] = *reinterpret_cast<const u32x4*>(a.keys + ak * (16 * D) + (kr % 16) * D + kc * 16);
+                    x.ks[i] = a.scales[2 * ak];
+                }
+                if (on(vb)) {
+                    x.v[i] = *reinterpret_cast<const u32x4*>(a.values + av * (16 * D) + vc * 16);
+                    x.vs[i] = fabsf(a.scales[2 * av + 1]);
+                }
+            }
+        }
+    };
+    auto put = [&](const Raw& x, int stage) {
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            const int n = tid + i * THREADS;
+            if (PIECES % THREADS == 0 || n < PIECES) {
+                const int kr = n / (D / 16), kc = n % (D / 16), vb = n / D, vc = n % D;
+                bf16_t* k = &s_k[stage][kr * KROW + kc * 16];
+                *reinterpret_cast<bf16x8*>(k) = operand(x.k[i][0], x.k[i][1], x.ks[i]);
+                *reinterpret_cast<bf16x8*>(k + 8) = operand(x.k[i][2], x.k[i][3], x.ks[i]);
+                bf16_t* v = &s_v[stage][vc * VROW + vb * 16];
+                *reinterpret_cast<bf16x8*>(v) = operand(x.v[i][0], x.v[i][2], x.vs[i]);
+                *reinterpret_cast<bf16x8*>(v + 8) = operand(x.v[i][1], x.v[i][3], x.vs[i]);
+            }
+        }
+    };
+
+    f32x16 o[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) o[m] = f32x16{};
+    float top = -INFINITY, l = 0.f;
+
+    auto compute = [&](int tile, int stage, bool bad, const Pages& pages) {
+        const int j0 = tile * TILE;
+        if (j0 > w_last || j0 + TILE - 1 < w_low) return;       // no column of this wavefront sees a key of the tile
+        const bf16_t* sk = s_k[stage];
+        const bf16_t* sv = s_v[stage];
+        f32x16 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = f32x16{};
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(&sk[(32 * t + r) * KROW + 16 * i + 8 * half]), q[i],
+                                                               s[t], 0, 0, 0);
+        }
+        if (a.softcap > 0.f) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] = score(s[t][i]);
+        }
+        // key j0 + 32 t + 8 (i / 4) + 4 half + i % 4, of block 2 t + i / 8
+        bool gone = false;
+        uint32_t here = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            bool there;
+            place(4 * tile + b, uniform(pages.p[b]), there);
+            here |= (there ? 1u : 0u) << b;
+        }
+        gone = here != 15u;
+        auto seen = [&](int t, int i) {
+            const int j = j0 + 32 * t + 8 * (i / 4) + i % 4 + 4 * half;
+            return j >= low && j <= pos && (here >> (2 * t + i / 8) & 1u);
+        };
+        if (j0 + TILE - 1 > w_first || j0 < w_low_last || !w_any || gone) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] = seen(t, i) ? s[t][i] : -INFINITY;
+        }
+        float best = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) best = fmaxf(best, s[t][i]);
+        const WaveTwo two = wave_two<32>(__float_as_uint(best));
+        best = fmaxf(__uint_as_float(two.a), __uint_as_float(two.b)) * score.factor;
+        // the sums move to a new maximum only when it is 2^8 above the old one: weights stay below 2^8 until then
+        if (__any(best > top + 8.f || (top == -INFINITY && best > -INFINITY))) {
+            const float now = fmaxf(top, best);
+            const float again = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
+            l *= again;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) o[m] *= again;
+            top = now;
+        }
+        const float shift = top == -INFINITY ? 0.f : -top;
+        bf16x8 p[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i], score.factor, shift));
+                l += e;
+                p[2 * t + i / 8][i % 8] = static_cast<__bf16>(e);
+            }
+        auto value = [&](int m, int u) { return *reinterpret_cast<const bf16x8*>(&sv[(32 * m + r) * VROW + 16 * u + 8 * half]); };
+        if (__builtin_expect(bad, 0)) {
+            // as in attn8_few
+            bf16x8 see[4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) see[2 * t + i / 8][i % 8] = static_cast<__bf16>(seen(t, i) ? 1.f : 0.f);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                f32x16 count = f32x16{};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    u32x4 v = __builtin_bit_cast(u32x4, value(m, u)), one;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t none = ((v[i] & 0x7fffu) > 0x7f80u ? 0xffffu : 0u) | ((v[i] & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u);
+                        one[i] = none & 0x3f803f80u;
+                        v[i] &= ~none;
+                    }
+                    count = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, one), see[u], count, 0, 0, 0);
+                    o[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), p[u], o[m], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[m][i] = count[i] > 0.f ? __builtin_nanf("") : o[m][i];
+            }
+            return;
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value(m, u), p[u], o[m], 0, 0, 0);
+    };
+
+    {
+        Raw raw;
+        Pages pages = find(tile_begin), ahead = find(tile_begin + 1);
+        load(tile_begin, pages, raw);
+        bool bad = raw.bad;
+        put(raw, 0);
+        __syncthreads();
+        int stage = 0;
+        for (int tile = tile_begin; tile < tile_end; ++tile, stage ^= 1) {
+            const bool more = tile + 1 < tile_end;
+            Pages beyond = ahead;
+            if (more) {
+                load(tile + 1, ahead, raw);
+                beyond = find(tile + 2);
+            }
+            compute(tile, stage, bad, pages);
+            if (more) {
+                put(raw, stage ^ 1);       // (that stage was read before the last barrier)
+                bad = raw.bad;
+                pages = ahead;
+                ahead = beyond;
+            }
+            __syncthreads();
+        }
+    }
+    const WaveTwo two = wave_two<32>(__float_as_uint(l));
+    l = __uint_as_float(two.a) + __uint_as_float(two.b);
+    if (!col_ok) return;
+    if (whole) {
+        const float inv = finish(a, top, l, col_row, head);
+        bf16_t* to = static_cast<bf16_t*>(a.out) + col_row * a.o_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int ch = 32 * m + 8 * c + 4 * half;
+                store4(to + ch, f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]},
+                       [&](int e) { return inv * channel_gate(a, col_row, head, ch + e); });
+            }
+    } else {
+        const int64_t at = (static_cast<int64_t>(w) * gridDim.x + blockIdx.x) * MANY + col;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *reinterpret_cast<f32x4*>(a.part_o + at * D + 32 * m + 8 * c + 4 * half) =
+                    f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]};
+        if (half == 0) {
+            a.part_ml[2 * at] = top;
+            a.part_ml[2 * at + 1] = l;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- the join
+// out = sum_z w_z o_z / sum_z w_z l_z, w_z = exp2(m_z - max m), over an item's pieces in their order.
+template <int COLS>
+__global__ __launch_bounds__(THREADS) void attn8_join_kernel(PulseAttn8 a, int head_groups) {
+    const int item = blockIdx.y;
+    const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::CUT_HEAD + 4 * a.max_work)[item];
+    const int first = uniform(info.x), pieces = uniform(info.y);
+    if (pieces <= 1) return;
+    const int4 it = reinterpret_cast<const int4*>(a.items)[item];
+    const int group = a.nq / a.nkv, g = blockIdx.x / head_groups, part = blockIdx.x % head_groups;
+    const int heads = min(group - part * FEW, COLS == FEW ? FEW : group), d = a.d, quads = d / 4;
+    const int cols = it.y * heads;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * COLS;
+    const int64_t at0 = static_cast<int64_t>(first) * step + static_cast<int64_t>(blockIdx.x) * COLS;
+    for (int i = blockIdx.z * THREADS + threadIdx.x; i < cols * quads; i += gridDim.z * THREADS) {
+        const int c = i / quads, ch = i % quads * 4;
+        const int64_t at = at0 + c;
+        float m = -INFINITY;
+        for (int z = 0; z < pieces; ++z) m = fmaxf(m, a.part_ml[2 * (at + z * step)]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        f32x4 all = {0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < pieces; ++z) {
+            const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + z * step)] - ref);
+            l += a.part_ml[2 * (at + z * step) + 1] * f;
+            all += *reinterpret_cast<const f32x4*>(a.part_o + (at + z * step) * d + ch) * f;
+        }
+        const int row = it.x + c / heads, hd = g * group + part * FEW + c % heads;
+        const float inv = finish(a, m, l, row, hd);
+        bf16_t* to = static_cast<bf16_t*>(a.out) + row * a.o_stride + static_cast<int64_t>(hd) * d + ch;
+        store4(to, all, [&](int e) { return inv * channel_gate(a, row, hd, ch + e); });
+    }
+}
+
+int check_matrix(const PulseAttn8* a, const char* what) {
+    if (int rc = pulse_attn8_check(a, what)) return rc;
+    PULSE_REQUIRE(a->dtype == PULSE_BF16 && a->d % 32 == 0 && a->d <= 256 && a->page_size % cache8::BLOCK == 0,
+                  "%s: bfloat16 rows, heads of a multiple of 32 channels up to 256 and pages of a multiple of 16 tokens are served", what);
+    PULSE_REQUIRE(a->items && a->cut && a->n_items > 0 && a->max_work > 0 && a->max_work <= 65535 && a->n_items <= 65535, "%s: bad work list", what);
+    PULSE_REQUIRE(a->q_stride % 8 == 0 && a->o_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a->q) & 15) == 0 &&
+                      (reinterpret_cast<uintptr_t>(a->out) & 7) == 0, "%s: rows must be aligned to 16 bytes", what);
+    PULSE_REQUIRE(a->max_work == a->n_items || (a->part_o && a->part_ml), "%s: the room for pieces is missing", what);
+    return 0;
+}
+
+template <typename F>
+int by_width(int d, F go) {
+    switch (d) {
+        case 32: go(std::integral_constant<int, 32>()); break;
+        case 64: go(std::integral_constant<int, 64>()); break;
+        case 96: go(std::integral_constant<int, 96>()); break;
+        case 128: go(std::integral_constant<int, 128>()); break;
+        case 160: go(std::integral_constant<int, 160>()); break;
+        case 192: go(std::integral_constant<int, 192>()); break;
+        case 224: go(std::integral_constant<int, 224>()); break;
+        default: go(std::integral_constant<int, 256>()); break;
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int64_t pulse_attn8_cut_ints(int n_items, int max_work) { return cache8::cut_ints(n_items, max_work); }
+
+extern "C" int pulse_attn8_cut(const int* items, int n_items, const int* positions, int window, int chunk, int slots, int least,
+                               int max_work, int* cut, hipStream_t stream) {
+    PULSE_REQUIRE(items && positions && cut && n_items > 0 && slots > 0 && least > 0, "attn8_cut: bad work list");
+    PULSE_REQUIRE(max_work >= n_items && (max_work == n_items || max_work >= n_items + slots), "attn8_cut: room for %d pieces, %d are possible", max_work,
+                  n_items + slots);
+    PULSE_REQUIRE((reinterpret_cast<uintptr_t>(items) & 15) == 0 && (reinterpret_cast<uintptr_t>(cut) & 15) == 0, "attn8_cut: lists must be aligned to 16 bytes");
+    // (no room for more pieces than items: one each)
+    attn8_cut_kernel<<<1, THREADS, 0, stream>>>(reinterpret_cast<const int4*>(items), n_items, positions, window, chunk, slots,
+                                                max_work == n_items ? 0x3fffffff : least, max_work, cut);
+    PULSE_LAUNCH_CHECK("attn8_cut");
+    return 0;
+}
+
+extern "C" int pulse_attn8_few(const PulseAttn8* a, hipStream_t stream) {
+    if (int rc = check_matrix(a, "attn8_few")) return rc;
+    const int head_groups = (a->nq / a->nkv + FEW - 1) / FEW;
+    const cache8::Div blocks = cache8::div_by(a->page_size / cache8::BLOCK);
+    const dim3 grid(a->nkv * head_groups, a->max_work);
+    by_width(a->d, [&](auto d) { attn8_few_kernel<decltype(d)::value><<<grid, THREADS, 0, stream>>>(*a, blocks, head_groups); });
+    PULSE_LAUNCH_CHECK("attn8_few");
+    if (a->max_work > a->n_items) {
+        attn8_join_kernel<FEW><<<dim3(a->nkv * head_groups, a->n_items), THREADS, 0, stream>>>(*a, head_groups);
+        PULSE_LAUNCH_CHECK("attn8_join");
+    }
+    return 0;
+}
+
+extern "C" int pulse_attn8_many(const PulseAttn8* a, hipStream_t stream) {
+    if (int rc = check_matrix(a, "attn8_many")) return rc;
+    PULSE_REQUIRE(a->nq / a->nkv <= MANY, "attn8_many: %d heads on one (up to %d)", a->nq / a->nkv, MANY);
+    const cache8::Div blocks = cache8::div_by(a->page_size / cache8::BLOCK);
+    const dim3 grid(a->nkv, a->max_work);
+    by_width(a->d, [&](auto d) { attn8_many_kernel<decltype(d)::value><<<grid, THREADS, 0, stream>>>(*a, blocks); });
+    PULSE_LAUNCH_CHECK("attn8_many");
+    if (a->max_work > a->n_items) {
+        attn8_join_kernel<MANY><<<dim3(a->nkv, a->n_items, 8), THREADS, 0, stream>>>(*a, 1);
+        PULSE_LAUNCH_CHECK("attn8_join");
+    }
+    return 0;
+}
