@@ -58,17 +58,18 @@ __device__ __forceinline__ uint32_t moved(uint32_t b, float down) {
     return to_e4m3x4(x[0] * down, x[1] * down, x[2] * down, x[3] * down);
 }
 
-// a / b and a % b where b's logarithm is `shift`, or -1 where b is no power of two (a >= 0)
+// a / b and a % b for 0 <= a < 2^31 by a multiplication, without a branch: with L the least number for which 2^L >= b and
+// m = floor(2^(31 + L) / b) + 1 (less than 2^32), a m / 2^(31 + L) exceeds a / b by less than 1 / b.
 struct Div {
-    int b, shift;
-    __device__ __forceinline__ int over(int a) const { return shift >= 0 ? a >> shift : a / b; }
-    __device__ __forceinline__ int rest(int a) const { return shift >= 0 ? a & (b - 1) : a % b; }
+    int b;
+    uint32_t m, shift;
+    __device__ __forceinline__ int over(int a) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(a)) * m) >> shift); }
+    __device__ __forceinline__ int rest(int a) const { return a - over(a) * b; }
 };
 inline Div div_by(int b) {
-    int shift = -1;
-    for (int s = 0; s < 31; ++s)
-        if (b == 1 << s) shift = s;
-    return {b, shift};
+    uint32_t bits = 0;
+    while ((1ll << bits) < b) ++bits;
+    return {b, static_cast<uint32_t>((1ull << (31 + bits)) / static_cast<uint32_t>(b) + 1), 31 + bits};
 }
 
 }  // namespace cache8

@@ -205,11 +205,10 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
         };
         const bool on_k = there(nk, at.pk);
         x.there = there(nv, at.pv);
-        const int64_t hk = static_cast<int64_t>(on_k ? at.pk : 0) * a.nkv + g, hv = static_cast<int64_t>(x.there ? at.pv : 0) * a.nkv + g;
-        const int ik = on_k ? blocks.rest(nk) : 0, iv = x.there ? blocks.rest(nv) : 0;
-        const int64_t bk = hk * blocks.b + ik, bv = hv * blocks.b + iv;
-        const uint8_t* kp = a.keys + bk * (16 * D) + (r % 4) * D;
-        const uint8_t* vp = a.values + bv * (16 * D) + r * 16;
+        const uint32_t bk = on_k ? (static_cast<uint32_t>(at.pk) * a.nkv + g) * blocks.b + blocks.rest(nk) : 0u;
+        const uint32_t bv = x.there ? (static_cast<uint32_t>(at.pv) * a.nkv + g) * blocks.b + blocks.rest(nv) : 0u;
+        const uint8_t* kp = a.keys + static_cast<uint64_t>(bk) * (16 * D) + (r % 4) * D;
+        const uint8_t* vp = a.values + static_cast<uint64_t>(bv) * (16 * D) + r * 16;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -218,8 +217,8 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
         }
 #pragma unroll
         for (int m = 0; m < F::MT; ++m) x.v[m] = *reinterpret_cast<const u32x4*>(vp + m * 256);
-        x.ks = a.scales[2 * bk];
-        x.vs = a.scales[2 * bv + 1];
+        x.ks = a.scales[2ull * bk];
+        x.vs = a.scales[2ull * bv + 1];
     };
 
     f32x4 o[F::MT];
@@ -374,12 +373,18 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
 // 8 (i / 4) + 4 (l / 32) + i % 4, i < 16, of column l % 32.  The values lie in LDS in the order in which the weights come out of the
 // first product: of 16 keys the lanes of half h hold 4 h .. and 8 + 4 h .., which are one piece of 16 bytes.  Rows are 16 bytes longer than
 // they have to be, so that the eight rows that are read in a cycle lie in different banks.
-template <int D>
+//
+// A thread brings piece n of a tile's keys and of its values: 16 bytes at the same place of the same block (a row's 16 channels, a
+// channel's 16 tokens), asked for while the tile before is computed, and converts them into the other of two stages.  What is rare (caps,
+// masks, blocks that are not there or hold what is not finite, a maximum that grew) stands behind real branches: left to itself the
+// compiler computes both sides.
+template <int D, bool CAP>
 __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(PulseAttn8 a, cache8::Div blocks) {
     constexpr int KROW = D + 8, VROW = TILE + 8;                 // in bfloat16 numbers
     constexpr int PIECES = 4 * D, TURNS = (PIECES + THREADS - 1) / THREADS, STEPS = D / 16, MT = D / 32;
     __shared__ __attribute__((aligned(16))) bf16_t s_k[2][TILE * KROW];
     __shared__ __attribute__((aligned(16))) bf16_t s_v[2][D * VROW];
+    __shared__ int s_odd[2], s_gone[2][4];      // the tile + 1 in which something is out of the ordinary; in which the block is not there
     const int w = blockIdx.y;
     if (w >= uniform(a.cut[0])) return;
     const int4 job = reinterpret_cast<const int4*>(a.cut + cache8::CUT_HEAD)[w];
@@ -414,65 +419,52 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     const Score score = score_of(a);
     const int* bt = a.table + static_cast<int64_t>(entry) * a.table_width;
 
-    // A tile's bytes: keys in pieces of 16 channels, values in pieces of a channel's 16 tokens of a block.
     struct Raw {
         u32x4 k[TURNS], v[TURNS];
-        float ks[TURNS], vs[TURNS];
-        bool bad;              // a block of the tile holds values that are not finite
+        float2 scale[TURNS];
+        int there[TURNS];      // -1: beyond what the item sees, 0: not there, 1: there
     };
-    auto place = [&](int n, int page, bool& there) {
-        there = page >= 0 && page < a.num_pages && blocks.over(n) < a.table_width && 16 * n <= hi && 16 * n + 15 >= lo;
-        return ((static_cast<int64_t>(there ? page : 0) * a.nkv + g) * blocks.b + (there ? blocks.rest(n) : 0));
-    };
-    struct Pages { int p[4]; };
-    auto find = [&](int tile) {
+    struct Pages { int p[TURNS]; };
+    // (piece n is of block n / D of the tile; a last turn that not all threads take brings the others a piece for nobody)
+    auto find = [&](int tile) __attribute__((always_inline)) {
         Pages x;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x.p[b] = bt[min(blocks.over(4 * tile + b), a.table_width - 1)];
+        for (int i = 0; i < TURNS; ++i) x.p[i] = bt[min(blocks.over(4 * tile + min((tid + i * THREADS) / D, 3)), a.table_width - 1)];
         return x;
     };
-    auto load = [&](int tile, const Pages& pages, Raw& x) {
-        int64_t at[4];
-        bool there[4];
-        x.bad = false;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            at[b] = place(4 * tile + b, uniform(pages.p[b]), there[b]);
-            x.bad |= there[b] && a.scales[2 * at[b] + 1] < 0.f;
-        }
-        auto pick = [&](int b) { return b == 0 ? at[0] : b == 1 ? at[1] : b == 2 ? at[2] : at[3]; };
-        auto on = [&](int b) { return b == 0 ? there[0] : b == 1 ? there[1] : b == 2 ? there[2] : there[3]; };
+    auto load = [&](int tile, const Pages& pages, Raw& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) {
-            const int n = tid + i * THREADS;
-            x.k[i] = x.v[i] = u32x4{0u, 0u, 0u, 0u};
-            x.ks[i] = x.vs[i] = 1.f;
-            if (PIECES % THREADS == 0 || n < PIECES) {
-                const int kr = n / (D / 16), kc = n % (D / 16), vb = n / D, vc = n % D;
-                const int64_t ak = pick(kr / 16), av = pick(vb);
-                if (on(kr / 16)) {
-                    x.k[i] = *reinterpret_cast<const u32x4*>(a.keys + ak * (16 * D) + (kr % 16) * D + kc * 16);
-                    x.ks[i] = a.scales[2 * ak];
-                }
-                if (on(vb)) {
-                    x.v[i] = *reinterpret_cast<const u32x4*>(a.values + av * (16 * D) + vc * 16);
-                    x.vs[i] = fabsf(a.scales[2 * av + 1]);
-                }
-            }
+            const int n = tid + i * THREADS, b = 4 * tile + min(n / D, 3), page = pages.p[i];
+            const bool ours = 16 * b <= hi && 16 * b + 15 >= lo;
+            const bool there = ours && page >= 0 && page < a.num_pages && blocks.over(b) < a.table_width;
+            x.there[i] = there ? 1 : ours ? 0 : -1;
+            const uint32_t at = there ? (static_cast<uint32_t>(page) * a.nkv + g) * blocks.b + blocks.rest(b) : 0u;
+            const uint64_t byte = static_cast<uint64_t>(at) * (16 * D) + n % D * 16;
+            x.k[i] = *reinterpret_cast<const u32x4*>(a.keys + byte);
+            x.v[i] = *reinterpret_cast<const u32x4*>(a.values + byte);
+            x.scale[i] = reinterpret_cast<const float2*>(a.scales)[at];
         }
     };
-    auto put = [&](const Raw& x, int stage) {
+    auto put = [&](Raw& x, int stage, int tile) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) {
             const int n = tid + i * THREADS;
             if (PIECES % THREADS == 0 || n < PIECES) {
                 const int kr = n / (D / 16), kc = n % (D / 16), vb = n / D, vc = n % D;
+                if (__builtin_expect(x.there[i] <= 0 || x.scale[i].y < 0.f, 0)) {
+                    asm volatile("");
+                    if (x.there[i] <= 0) x.k[i] = x.v[i] = u32x4{0u, 0u, 0u, 0u};
+                    if (x.there[i] >= 0) s_odd[stage] = tile + 1;       // (every thread that writes it writes the same)
+                    if (x.there[i] == 0) s_gone[stage][vb] = tile + 1;
+                }
+                const float ks = x.scale[i].x, vs = fabsf(x.scale[i].y);
                 bf16_t* k = &s_k[stage][kr * KROW + kc * 16];
-                *reinterpret_cast<bf16x8*>(k) = operand(x.k[i][0], x.k[i][1], x.ks[i]);
-                *reinterpret_cast<bf16x8*>(k + 8) = operand(x.k[i][2], x.k[i][3], x.ks[i]);
+                *reinterpret_cast<bf16x8*>(k) = operand(x.k[i][0], x.k[i][1], ks);
+                *reinterpret_cast<bf16x8*>(k + 8) = operand(x.k[i][2], x.k[i][3], ks);
                 bf16_t* v = &s_v[stage][vc * VROW + vb * 16];
-                *reinterpret_cast<bf16x8*>(v) = operand(x.v[i][0], x.v[i][2], x.vs[i]);
-                *reinterpret_cast<bf16x8*>(v + 8) = operand(x.v[i][1], x.v[i][3], x.vs[i]);
+                *reinterpret_cast<bf16x8*>(v) = operand(x.v[i][0], x.v[i][2], vs);
+                *reinterpret_cast<bf16x8*>(v + 8) = operand(x.v[i][1], x.v[i][3], vs);
             }
         }
     };
@@ -482,41 +474,45 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     for (int m = 0; m < MT; ++m) o[m] = f32x16{};
     float top = -INFINITY, l = 0.f;
 
-    auto compute = [&](int tile, int stage, bool bad, const Pages& pages) {
+    auto compute = [&](int tile, int stage) __attribute__((always_inline)) {
         const int j0 = tile * TILE;
         if (j0 > w_last || j0 + TILE - 1 < w_low) return;       // no column of this wavefront sees a key of the tile
-        const bf16_t* sk = s_k[stage];
-        const bf16_t* sv = s_v[stage];
-        f32x16 s[2];
+        const bf16_t* sk = s_k[stage] + r * KROW + 8 * half;
+        const bf16_t* sv = s_v[stage] + r * VROW + 8 * half;
+        const bool odd = uniform(s_odd[stage]) == tile + 1;
+        constexpr int AHEAD = 4;       // operand reads run that many products ahead
+        auto key = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<const bf16x8*>(sk + i / STEPS * (32 * KROW) + i % STEPS * 16); };
+        auto value = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<const bf16x8*>(sv + i / 4 * (32 * VROW) + i % 4 * 16); };
+        bf16x8 ak[2 * STEPS], av[4 * MT];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            s[t] = f32x16{};
+        for (int i = 0; i < AHEAD; ++i) ak[i] = key(i);
+        f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
-            for (int i = 0; i < STEPS; ++i)
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(&sk[(32 * t + r) * KROW + 16 * i + 8 * half]), q[i],
-                                                               s[t], 0, 0, 0);
+        for (int i = 0; i < 2 * STEPS; ++i) {
+            if (i + AHEAD < 2 * STEPS) ak[i + AHEAD] = key(i + AHEAD);
+            else if (i + AHEAD - 2 * STEPS < 4 * MT) av[i + AHEAD - 2 * STEPS] = value(i + AHEAD - 2 * STEPS);
+            s[i / STEPS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ak[i], q[i % STEPS], s[i / STEPS], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (a.softcap > 0.f) {
+        if constexpr (CAP) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[t][i] = score(s[t][i]);
         }
-        // key j0 + 32 t + 8 (i / 4) + 4 half + i % 4, of block 2 t + i / 8
-        bool gone = false;
-        uint32_t here = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            bool there;
-            place(4 * tile + b, uniform(pages.p[b]), there);
-            here |= (there ? 1u : 0u) << b;
-        }
-        gone = here != 15u;
-        auto seen = [&](int t, int i) {
-            const int j = j0 + 32 * t + 8 * (i / 4) + i % 4 + 4 * half;
-            return j >= low && j <= pos && (here >> (2 * t + i / 8) & 1u);
+        // s[t][i] is of key j0 + 32 t + 8 (i / 4) + 4 half + i % 4, of block 2 t + i / 8
+        const int from = low - j0 - 4 * half, to = pos - j0 - 4 * half;
+        uint32_t gone = 0;
+        auto seen = [&](int t, int i) __attribute__((always_inline)) {
+            const int j = 32 * t + 8 * (i / 4) + i % 4;
+            return j >= from && j <= to && !(gone >> (2 * t + i / 8) & 1u);
         };
-        if (j0 + TILE - 1 > w_first || j0 < w_low_last || !w_any || gone) {
+        if (j0 + TILE - 1 > w_first || j0 < w_low_last || !w_any || odd) {
+            asm volatile("");
+            if (odd) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) gone |= (uniform(s_gone[stage][b]) == tile + 1 ? 1u : 0u) << b;
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -531,6 +527,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
         best = fmaxf(__uint_as_float(two.a), __uint_as_float(two.b)) * score.factor;
         // the sums move to a new maximum only when it is 2^8 above the old one: weights stay below 2^8 until then
         if (__any(best > top + 8.f || (top == -INFINITY && best > -INFINITY))) {
+            asm volatile("");
             const float now = fmaxf(top, best);
             const float again = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
             l *= again;
@@ -548,8 +545,8 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
                 l += e;
                 p[2 * t + i / 8][i % 8] = static_cast<__bf16>(e);
             }
-        auto value = [&](int m, int u) { return *reinterpret_cast<const bf16x8*>(&sv[(32 * m + r) * VROW + 16 * u + 8 * half]); };
-        if (__builtin_expect(bad, 0)) {
+        if (__builtin_expect(odd, 0)) {
+            asm volatile("");
             // as in attn8_few
             bf16x8 see[4];
 #pragma unroll
@@ -561,7 +558,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
                 f32x16 count = f32x16{};
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    u32x4 v = __builtin_bit_cast(u32x4, value(m, u)), one;
+                    u32x4 v = __builtin_bit_cast(u32x4, value(4 * m + u)), one;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t none = ((v[i] & 0x7fffu) > 0x7f80u ? 0xffffu : 0u) | ((v[i] & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u);
@@ -576,34 +573,34 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
             }
             return;
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) o[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value(m, u), p[u], o[m], 0, 0, 0);
+        for (int i = 0; i < 4 * MT; ++i) {
+            if (i + AHEAD < 4 * MT) av[i + AHEAD] = value(i + AHEAD);
+            o[i / 4] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av[i], p[i % 4], o[i / 4], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
     {
         Raw raw;
-        Pages pages = find(tile_begin), ahead = find(tile_begin + 1);
+        Pages pages = find(tile_begin);
+        if (tid < 2) s_odd[tid] = 0;
+        if (tid < 8) s_gone[tid / 4][tid % 4] = 0;
+        __syncthreads();
         load(tile_begin, pages, raw);
-        bool bad = raw.bad;
-        put(raw, 0);
+        pages = find(tile_begin + 1);
+        put(raw, 0, tile_begin);
         __syncthreads();
         int stage = 0;
         for (int tile = tile_begin; tile < tile_end; ++tile, stage ^= 1) {
             const bool more = tile + 1 < tile_end;
-            Pages beyond = ahead;
             if (more) {
-                load(tile + 1, ahead, raw);
-                beyond = find(tile + 2);
+                load(tile + 1, pages, raw);
+                pages = find(tile + 2);
             }
-            compute(tile, stage, bad, pages);
-            if (more) {
-                put(raw, stage ^ 1);       // (that stage was read before the last barrier)
-                bad = raw.bad;
-                pages = ahead;
-                ahead = beyond;
-            }
+            compute(tile, stage);
+            if (more) put(raw, stage ^ 1, tile + 1);       // (that stage was read before the last barrier)
             __syncthreads();
         }
     }
@@ -613,14 +610,18 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     if (whole) {
         const float inv = finish(a, top, l, col_row, head);
         bf16_t* to = static_cast<bf16_t*>(a.out) + col_row * a.o_stride + static_cast<int64_t>(head) * D;
+        if (__builtin_expect(a.gate_width > 0, 0)) {
+            asm volatile("");
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[m][i] *= channel_gate(a, col_row, head, 32 * m + 8 * (i / 4) + 4 * half + i % 4);
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int ch = 32 * m + 8 * c + 4 * half;
-                store4(to + ch, f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]},
-                       [&](int e) { return inv * channel_gate(a, col_row, head, ch + e); });
-            }
+            for (int c = 0; c < 4; ++c)
+                store4(to + 32 * m + 8 * c + 4 * half, f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]}, [&](int) { return inv; });
     } else {
         const int64_t at = (static_cast<int64_t>(w) * gridDim.x + blockIdx.x) * MANY + col;
 #pragma unroll
@@ -674,6 +675,7 @@ int check_matrix(const PulseAttn8* a, const char* what) {
     if (int rc = pulse_attn8_check(a, what)) return rc;
     PULSE_REQUIRE(a->dtype == PULSE_BF16 && a->d % 32 == 0 && a->d <= 256 && a->page_size % cache8::BLOCK == 0,
                   "%s: bfloat16 rows, heads of a multiple of 32 channels up to 256 and pages of a multiple of 16 tokens are served", what);
+    PULSE_REQUIRE(static_cast<int64_t>(a->num_pages) * a->nkv * (a->page_size / cache8::BLOCK) <= 0x7fffffff, "%s: too many pages", what);
     PULSE_REQUIRE(a->items && a->cut && a->n_items > 0 && a->max_work > 0 && a->max_work <= 65535 && a->n_items <= 65535, "%s: bad work list", what);
     PULSE_REQUIRE(a->q_stride % 8 == 0 && a->o_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a->q) & 15) == 0 &&
                       (reinterpret_cast<uintptr_t>(a->out) & 7) == 0, "%s: rows must be aligned to 16 bytes", what);
@@ -732,7 +734,10 @@ extern "C" int pulse_attn8_many(const PulseAttn8* a, hipStream_t stream) {
     PULSE_REQUIRE(a->nq / a->nkv <= MANY, "attn8_many: %d heads on one (up to %d)", a->nq / a->nkv, MANY);
     const cache8::Div blocks = cache8::div_by(a->page_size / cache8::BLOCK);
     const dim3 grid(a->nkv, a->max_work);
-    by_width(a->d, [&](auto d) { attn8_many_kernel<decltype(d)::value><<<grid, THREADS, 0, stream>>>(*a, blocks); });
+    by_width(a->d, [&](auto d) {
+        if (a->softcap > 0.f) attn8_many_kernel<decltype(d)::value, true><<<grid, THREADS, 0, stream>>>(*a, blocks);
+        else attn8_many_kernel<decltype(d)::value, false><<<grid, THREADS, 0, stream>>>(*a, blocks);
+    });
     PULSE_LAUNCH_CHECK("attn8_many");
     if (a->max_work > a->n_items) {
         attn8_join_kernel<MANY><<<dim3(a->nkv, a->n_items, 8), THREADS, 0, stream>>>(*a, 1);
