@@ -384,7 +384,9 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     constexpr int PIECES = 4 * D, TURNS = (PIECES + THREADS - 1) / THREADS, STEPS = D / 16, MT = D / 32;
     __shared__ __attribute__((aligned(16))) bf16_t s_k[2][TILE * KROW];
     __shared__ __attribute__((aligned(16))) bf16_t s_v[2][D * VROW];
-    __shared__ int s_odd[2], s_gone[2][4];      // the tile + 1 in which something is out of the ordinary; in which the block is not there
+    // the tile + 1 in which something is out of the ordinary; in which a block is not there; in which it holds values that are none, and which
+    __shared__ int s_odd[2], s_gone[2][4], s_bad[2][4];
+    __shared__ __attribute__((aligned(8))) uint16_t s_none[2][D][4];
     const int w = blockIdx.y;
     if (w >= uniform(a.cut[0])) return;
     const int4 job = reinterpret_cast<const int4*>(a.cut + cache8::CUT_HEAD)[w];
@@ -457,6 +459,19 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
                     if (x.there[i] <= 0) x.k[i] = x.v[i] = u32x4{0u, 0u, 0u, 0u};
                     if (x.there[i] >= 0) s_odd[stage] = tile + 1;       // (every thread that writes it writes the same)
                     if (x.there[i] == 0) s_gone[stage][vb] = tile + 1;
+                    if (x.there[i] > 0) {
+                        // Values that are not finite belong to those who see them alone: they leave the sums here, and a column that sees
+                        // one gets NaN in its channel.
+                        s_bad[stage][vb] = tile + 1;
+                        uint32_t none = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t bytes = nan_bytes(x.v[i][e]);
+                            none |= ((bytes & 1u) | (bytes >> 7 & 2u) | (bytes >> 14 & 4u) | (bytes >> 21 & 8u)) << (4 * e);
+                            x.v[i][e] &= ~bytes;
+                        }
+                        s_none[stage][vc][vb] = static_cast<uint16_t>(none);
+                    }
                 }
                 const float ks = x.scale[i].x, vs = fabsf(x.scale[i].y);
                 bf16_t* k = &s_k[stage][kr * KROW + kc * 16];
@@ -545,34 +560,6 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
                 l += e;
                 p[2 * t + i / 8][i % 8] = static_cast<__bf16>(e);
             }
-        if (__builtin_expect(odd, 0)) {
-            asm volatile("");
-            // as in attn8_few
-            bf16x8 see[4];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) see[2 * t + i / 8][i % 8] = static_cast<__bf16>(seen(t, i) ? 1.f : 0.f);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                f32x16 count = f32x16{};
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    u32x4 v = __builtin_bit_cast(u32x4, value(4 * m + u)), one;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t none = ((v[i] & 0x7fffu) > 0x7f80u ? 0xffffu : 0u) | ((v[i] & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u);
-                        one[i] = none & 0x3f803f80u;
-                        v[i] &= ~none;
-                    }
-                    count = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, one), see[u], count, 0, 0, 0);
-                    o[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), p[u], o[m], 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[m][i] = count[i] > 0.f ? __builtin_nanf("") : o[m][i];
-            }
-            return;
-        }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 4 * MT; ++i) {
@@ -580,13 +567,29 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
             o[i / 4] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av[i], p[i % 4], o[i / 4], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (__builtin_expect(odd, 0)) {
+            asm volatile("");
+            // the keys of the tile that this column sees, and of those the ones whose value in a channel is none
+            const int begin = max(low - j0, 0), end = min(pos - j0 + 1, TILE);
+            uint64_t seen_keys = end > begin ? (~0ull >> (TILE - (end - begin))) << begin : 0ull;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                if (uniform(s_gone[stage][b]) == tile + 1 || uniform(s_bad[stage][b]) != tile + 1) seen_keys &= ~(0xffffull << (16 * b));
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint64_t none = *reinterpret_cast<const uint64_t*>(s_none[stage][32 * m + 8 * (i / 4) + 4 * half + i % 4]);
+                    if (none & seen_keys) o[m][i] = __builtin_nanf("");
+                }
+        }
     };
 
     {
         Raw raw;
         Pages pages = find(tile_begin);
         if (tid < 2) s_odd[tid] = 0;
-        if (tid < 8) s_gone[tid / 4][tid % 4] = 0;
+        if (tid < 8) s_gone[tid / 4][tid % 4] = s_bad[tid / 4][tid % 4] = 0;
         __syncthreads();
         load(tile_begin, pages, raw);
         pages = find(tile_begin + 1);
