@@ -51,13 +51,16 @@ __device__ __forceinline__ bf16x8 ones_at(uint32_t lo, uint32_t hi) {     // 0x3
     return operand(nan_bytes(lo) & 0x38383838u, nan_bytes(hi) & 0x38383838u, 1.f);
 }
 
-// A score in the units of exp2: the cap, if there is one, takes the place of the factor.
+// A score in the units of exp2; a cap takes the place of the factor: cap tanh(x / cap) log2 e = c - 2 c / (exp(2 x / cap) + 1) with
+// c = cap log2 e.  (The hardware's reciprocal: its error and the difference's are some 2^-22 of the cap.)
 struct Score {
-    float factor, cap_in, cap_out;
-    __device__ __forceinline__ float operator()(float s) const { return cap_out * cache8::tanh_of(s * cap_in); }
+    float factor, in, out;
+    __device__ __forceinline__ float operator()(float s) const {
+        return fmaf(-2.f * out, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * in) + 1.f), out);
+    }
 };
 __device__ __forceinline__ Score score_of(const PulseAttn8& a) {
-    if (a.softcap > 0.f) return {1.f, a.scale / a.softcap, a.softcap * LOG2E};
+    if (a.softcap > 0.f) return {1.f, 2.f * LOG2E * a.scale / a.softcap, a.softcap * LOG2E};
     return {a.scale * LOG2E, 0.f, 0.f};
 }
 
@@ -154,7 +157,7 @@ struct Few {
     bool there;            // the lane's own block
 };
 
-template <int D>
+template <int D, bool CAP>
 __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(PulseAttn8 a, cache8::Div blocks, int head_groups) {
     using F = Few<D>;
     __shared__ float s_o[WAVES][FEW][D + 4];
@@ -239,7 +242,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
             }
             if constexpr (F::K8) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(operand(x.k8[t].x, x.k8[t].y, x.ks), q[F::STEPS - 1], s[t], 0, 0, 0);
         }
-        if (a.softcap > 0.f) {
+        if constexpr (CAP) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -249,6 +252,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
         const int from = low - j0 - 16 * b, to = x.there ? pos - j0 - 16 * b : -1;
         const bool masked = j0 + TILE - 1 > pos0 || j0 < lo_last || __any(!x.there);
         if (masked) {
+            asm volatile("");
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -267,6 +271,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
         best = across_rows(best, LaneMax()) * score.factor;
         const float now = fmaxf(top, best);
         if (__any(now > top)) {
+            asm volatile("");
             const float again = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - now);
             l *= again;
 #pragma unroll
@@ -285,6 +290,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
             }
         const float vs = fabsf(x.vs);
         if (__builtin_expect(__any(x.there && x.vs < 0.f), 0)) {
+            asm volatile("");
             // Values that are not finite belong to those who see them alone: they are left out of the sums, and a column that sees one
             // in a channel (a product of ones says so) gets NaN there.
             bf16x8 see[2];
@@ -642,35 +648,57 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
 
 // ---------------------------------------------------------------------------------------------------------------- the join
 // out = sum_z w_z o_z / sum_z w_z l_z, w_z = exp2(m_z - max m), over an item's pieces in their order.
+// A workgroup takes `each` of an item's columns, a thread four channels of a column and every ZS-th piece; their sums meet in LDS.
 template <int COLS>
-__global__ __launch_bounds__(THREADS) void attn8_join_kernel(PulseAttn8 a, int head_groups) {
+__global__ __launch_bounds__(THREADS) void attn8_join_kernel(PulseAttn8 a, int head_groups, int each) {
     const int item = blockIdx.y;
     const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::CUT_HEAD + 4 * a.max_work)[item];
     const int first = uniform(info.x), pieces = uniform(info.y);
     if (pieces <= 1) return;
+    __shared__ f32x4 s_o[THREADS];
+    __shared__ float s_l[THREADS];
     const int4 it = reinterpret_cast<const int4*>(a.items)[item];
-    const int group = a.nq / a.nkv, g = blockIdx.x / head_groups, part = blockIdx.x % head_groups;
-    const int heads = min(group - part * FEW, COLS == FEW ? FEW : group), d = a.d, quads = d / 4;
-    const int cols = it.y * heads;
+    const int gp = blockIdx.x;                 // the kv head and sixteen of its heads
+    const int group = a.nq / a.nkv, g = gp / head_groups, part = gp % head_groups;
+    const int heads = COLS == FEW ? min(group - part * FEW, FEW) : group, d = a.d, quads = d / 4;
+    const int cols = it.y * heads, units = each * quads, zs = max(1, THREADS / units), tid = threadIdx.x;
     const int64_t step = static_cast<int64_t>(gridDim.x) * COLS;
-    const int64_t at0 = static_cast<int64_t>(first) * step + static_cast<int64_t>(blockIdx.x) * COLS;
-    for (int i = blockIdx.z * THREADS + threadIdx.x; i < cols * quads; i += gridDim.z * THREADS) {
-        const int c = i / quads, ch = i % quads * 4;
-        const int64_t at = at0 + c;
-        float m = -INFINITY;
+    const int64_t at0 = static_cast<int64_t>(first) * step + static_cast<int64_t>(gp) * COLS;
+    for (int u0 = 0; u0 < units; u0 += THREADS) {         // (one turn where the columns' channels are no more than the threads)
+        const int unit = zs > 1 ? tid % units : u0 + tid, z0 = zs > 1 ? tid / units : 0;
+        const int c = blockIdx.z * each + unit / quads, ch = unit % quads * 4;
+        const bool on = unit < units && z0 < zs && c < cols;
+        const int64_t at = at0 + (on ? c : 0);
+        float m = -INFINITY, l = 0.f;
+        f32x4 all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
         for (int z = 0; z < pieces; ++z) m = fmaxf(m, a.part_ml[2 * (at + z * step)]);
         const float ref = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
-        f32x4 all = {0.f, 0.f, 0.f, 0.f};
-        for (int z = 0; z < pieces; ++z) {
-            const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + z * step)] - ref);
-            l += a.part_ml[2 * (at + z * step) + 1] * f;
-            all += *reinterpret_cast<const f32x4*>(a.part_o + (at + z * step) * d + ch) * f;
+        if (on) {
+#pragma unroll 4
+            for (int z = z0; z < pieces; z += zs) {
+                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at + z * step));
+                const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_o + (at + z * step) * d + ch);
+                const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+                l += ml.y * f;
+                all += o * f;
+            }
         }
-        const int row = it.x + c / heads, hd = g * group + part * FEW + c % heads;
-        const float inv = finish(a, m, l, row, hd);
-        bf16_t* to = static_cast<bf16_t*>(a.out) + row * a.o_stride + static_cast<int64_t>(hd) * d + ch;
-        store4(to, all, [&](int e) { return inv * channel_gate(a, row, hd, ch + e); });
+        if (zs > 1) {
+            s_o[tid] = all;
+            s_l[tid] = l;
+            __syncthreads();
+            for (int z = 1; z < zs && z0 == 0 && unit < units; ++z) {
+                all += s_o[unit + z * units];
+                l += s_l[unit + z * units];
+            }
+        }
+        if (on && z0 == 0) {
+            const int row = it.x + c / heads, hd = g * group + part * FEW + c % heads;
+            const float inv = finish(a, m, l, row, hd);
+            bf16_t* to = static_cast<bf16_t*>(a.out) + row * a.o_stride + static_cast<int64_t>(hd) * d + ch;
+            store4(to, all, [&](int e) { return inv * channel_gate(a, row, hd, ch + e); });
+        }
     }
 }
 
@@ -723,10 +751,16 @@ extern "C" int pulse_attn8_few(const PulseAttn8* a, hipStream_t stream) {
     const int head_groups = (a->nq / a->nkv + FEW - 1) / FEW;
     const cache8::Div blocks = cache8::div_by(a->page_size / cache8::BLOCK);
     const dim3 grid(a->nkv * head_groups, a->max_work);
-    by_width(a->d, [&](auto d) { attn8_few_kernel<decltype(d)::value><<<grid, THREADS, 0, stream>>>(*a, blocks, head_groups); });
+    by_width(a->d, [&](auto d) {
+        if (a->softcap > 0.f) attn8_few_kernel<decltype(d)::value, true><<<grid, THREADS, 0, stream>>>(*a, blocks, head_groups);
+        else attn8_few_kernel<decltype(d)::value, false><<<grid, THREADS, 0, stream>>>(*a, blocks, head_groups);
+    });
     PULSE_LAUNCH_CHECK("attn8_few");
     if (a->max_work > a->n_items) {
-        attn8_join_kernel<FEW><<<dim3(a->nkv * head_groups, a->n_items), THREADS, 0, stream>>>(*a, head_groups);
+        // few items: a workgroup a column, so that many pieces are read by many; many: a workgroup for all of them
+        const int cols = a->nq / a->nkv > FEW ? FEW : FEW / (a->nq / a->nkv) * (a->nq / a->nkv);
+        const int each = static_cast<int64_t>(a->n_items) * a->nkv * head_groups * cols <= 4 * pulse_compute_units() ? 1 : cols;
+        attn8_join_kernel<FEW><<<dim3(a->nkv * head_groups, a->n_items, (cols + each - 1) / each), THREADS, 0, stream>>>(*a, head_groups, each);
         PULSE_LAUNCH_CHECK("attn8_join");
     }
     return 0;
@@ -743,7 +777,7 @@ extern "C" int pulse_attn8_many(const PulseAttn8* a, hipStream_t stream) {
     });
     PULSE_LAUNCH_CHECK("attn8_many");
     if (a->max_work > a->n_items) {
-        attn8_join_kernel<MANY><<<dim3(a->nkv, a->n_items, 8), THREADS, 0, stream>>>(*a, 1);
+        attn8_join_kernel<MANY><<<dim3(a->nkv, a->n_items, MANY / 16), THREADS, 0, stream>>>(*a, 1, 16);
         PULSE_LAUNCH_CHECK("attn8_join");
     }
     return 0;

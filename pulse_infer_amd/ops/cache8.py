@@ -23,6 +23,7 @@ from .library import KernelError, call
 
 MAX_REQUESTS = 4096          # of step_maps
 MAX_HEAD_DIM = 512           # of store and of attention
+TILE = 64                    # keys of a step of the matrix-core kernels
 FEW, MANY = 16, 128          # columns (rows times the heads that share a kv head) of an item of the two matrix-core kernels
 
 
@@ -206,8 +207,12 @@ class AttentionPlan:
     alone (how many tokens each request brings); the second is made on the GPU from the positions, by ``cut``, once a step for all
     layers that are alike in heads, window and chunk."""
 
-    FEW_LEAST = 4        # tiles of 64 keys of a piece of attn8_few: one a wavefront
-    MANY_LEAST = 8
+    # Workgroups a compute unit that a kernel's keys are shared out over, and the fewest tiles of 64 keys of a piece.
+    FEW_SLOTS, FEW_LEAST = 4, 8
+    MANY_SLOTS, MANY_LEAST = 2, 8
+    # Nothing is cut (and nothing joined) where the items fill the GPU by themselves, two workgroups a unit, and the longest is at most
+    # that many times what a unit's share of them would be.
+    FEW_EVEN, MANY_EVEN = 1.15, 2.2
     FEW_COLUMNS = 32     # up to which a portion goes through attn8_few
 
     def __init__(self, entries: Sequence[Any], nq: int, nkv: int, d: int, *, page_size: int, dtype: torch.dtype, window: int = 0,
@@ -237,28 +242,35 @@ class AttentionPlan:
         units = compute_units()
         to_device = to_device or (lambda flat: torch.tensor(flat, dtype=torch.int32, device=self.device))
 
-        def add(name: str, columns: int, items: List[Tuple], groups: int, slots: int, least: int) -> None:
+        def add(name: str, columns: int, items: List[Tuple], groups: int, slots: float, least: int, even: float) -> None:
             n = len(items)
             if not n:
                 return
-            slots = max(1, slots)
-            room = n + slots
+            tiles = [(last + rows - 1) // TILE + 1 - self._low(last) // TILE for last, _, rows, _ in items]
+            whole = n * groups >= 2 * units and max(tiles) * 2 * units <= even * sum(tiles) * groups
+            slots = max(1, int(slots * units) // groups)
+            room = n if whole else n + slots
             _need(room <= 65535, f"plan: {n} items are too many")
             on_gpu = to_device([v for _, row, rows, entry in items for v in (row, rows, entry, 0)])
             cut = torch.empty(4 + 4 * room + 2 * n, dtype=torch.int32, device=self.device)
             self.works.append((on_gpu, n, slots, least, room, cut))
             args = _Attn8.from_buffer_copy(base)
             args.items, args.cut, args.n_items, args.max_work = on_gpu.data_ptr(), cut.data_ptr(), n, room
-            self.calls.append((name, args, room * groups * columns))
+            self.calls.append((name, args, 0 if whole else room * groups * columns))
 
-        groups = nkv * ((group + FEW - 1) // FEW)
-        add("pulse_attn8_few", FEW, few, groups, 2 * units // groups, self.FEW_LEAST)
+        add("pulse_attn8_few", FEW, few, nkv * ((group + FEW - 1) // FEW), self.FEW_SLOTS, self.FEW_LEAST, self.FEW_EVEN)
         # The longest walks first; where two workgroups share a unit, the second ones' from the other end, the shortest beside the longest.
         many.sort(key=lambda it: -it[0])
         first = max(1, units // nkv)
         if first < len(many) <= 2 * first:
             many[first:] = many[:first - 1:-1]
-        add("pulse_attn8_many", MANY, many, nkv, (2 if len(many) <= first else 1) * units // nkv, self.MANY_LEAST)
+        add("pulse_attn8_many", MANY, many, nkv, self.MANY_SLOTS, self.MANY_LEAST, self.MANY_EVEN)
+
+    def _low(self, position: int) -> int:
+        """The lowest key that a token at ``position`` sees."""
+        if self.chunk:
+            return position - position % self.chunk
+        return max(0, position - self.window + 1) if self.window else 0
 
     def cut(self, positions: torch.Tensor) -> "AttentionPlan":
         """Shares the keys out for the rows' ``positions``: for every step, before its first ``attention``."""
