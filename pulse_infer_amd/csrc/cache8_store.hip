@@ -105,162 +105,318 @@ __device__ __forceinline__ void prepare_pairs(const StoreArgs& a, const TW* w, c
     for (int i = 0; i < 4; ++i) {
         x[i] *= factor;
         y[i] *= factor;
-        const int p = 4 * c + i;
-        if (p < half) {
-            const float cs = cos_t[t * half + p], sn = sin_t[t * half + p];
-            const float u = x[i] * cs - y[i] * sn, v = x[i] * sn + y[i] * cs;
-            x[i] = u;
-            y[i] = v;
+    }
+    auto turn = [&](int i, float cs, float sn) {
+        const float u = x[i] * cs - y[i] * sn, v = x[i] * sn + y[i] * cs;
+        x[i] = u;
+        y[i] = v;
+    };
+    if constexpr (WHOLE) {       // (four pairs are rotated, or none of them)
+        if (4 * c < half) {
+            const float4 cs = *reinterpret_cast<const float4*>(cos_t + t * half + 4 * c), sn = *reinterpret_cast<const float4*>(sin_t + t * half + 4 * c);
+            turn(0, cs.x, sn.x), turn(1, cs.y, sn.y), turn(2, cs.z, sn.z), turn(3, cs.w, sn.w);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * c + i < half) turn(i, cos_t[t * half + 4 * c + i], sin_t[t * half + 4 * c + i]);
     }
 }
 
-template <typename T, typename TW, bool WHOLE>
-__global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out, const TW* __restrict__ q_w,
-                                                         const TW* __restrict__ k_w, const float* __restrict__ cos_t,
-                                                         const float* __restrict__ sin_t, uint8_t* __restrict__ keys,
-                                                         uint8_t* __restrict__ values, float* __restrict__ scales,
-                                                         const int* __restrict__ positions, const int4* __restrict__ work, StoreArgs a) {
-    const int tid = threadIdx.x;
-    const int c = tid % a.lanes;
-    const int heads_at_once = THREADS / a.lanes;
-    const bool on = 8 * c < a.d;
-    const int block_groups = a.n_blocks * a.nkv;
-    if (static_cast<int>(blockIdx.x) >= block_groups) {
-        // q: neighbouring groups of lanes take neighbouring heads of the rows in turn
-        const int64_t i = static_cast<int64_t>(blockIdx.x - block_groups) * heads_at_once + tid / a.lanes;
-        const bool live = i < static_cast<int64_t>(a.tokens) * a.nq;
-        const int64_t t = live ? i / a.nq : 0;
-        const int h = live ? static_cast<int>(i - t * a.nq) : 0;
-        const T* row = qkv + t * a.row_stride + static_cast<int64_t>(h) * a.d;
-        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-        if (on) read_pairs<T, WHOLE>(a, row, c, x, y);
-        float factor = 1.f;
-        if (a.temp_every > 0) factor = 1.f + a.temp_coef * logf(static_cast<float>((positions[t] + 1) / a.temp_every) + 1.f);
-        prepare_pairs<TW, WHOLE>(a, q_w, cos_t, sin_t, t, c, factor, x, y);
-        if (!on || !live) return;
-        T* to = q_out + t * a.q_stride + static_cast<int64_t>(h) * a.d;
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-            int ia, ib;
-            channels_of(a, 4 * c + i4, ia, ib);
-            if (2 * (4 * c + i4) < a.d) {
-                to[ia] = from_f32<T>(x[i4]);
-                to[ib] = from_f32<T>(y[i4]);
-            }
-        }
-        return;
-    }
-
-    __shared__ float s_max[2][THREADS / PULSE_WAVE];
-    __shared__ int s_bad;
-    const int4 job = work[blockIdx.x / a.nkv];
-    const int g = blockIdx.x % a.nkv;
-    const int first = job.x, rows = job.y, at = job.w;
-    // (a list that says anything else is not followed)
-    if (rows <= 0 || job.z < 0 || job.z >= a.all_blocks || at < 0 || at + rows > a.block || first < 0 || first + rows > a.tokens) return;
-    const int64_t page = job.z / a.blocks_per_page;
-    const int inner = job.z - static_cast<int>(page) * a.blocks_per_page;
-    const int64_t head = page * a.nkv + g;
-    uint8_t* kb = keys + (head * a.page_size + static_cast<int64_t>(inner) * a.block) * a.d;      // [token][channel]
-    uint8_t* vb = values + (head * a.page_size + static_cast<int64_t>(inner) * a.block) * a.d;    // [channel][token]
-    float* sc = scales + (head * a.blocks_per_page + inner) * 2;
-    const bool fresh = at == 0;
-    const float had_k = fresh ? 0.f : sc[0], had_v = fresh ? 0.f : sc[1];
-
-    auto key_pairs = [&](int j, float (&x)[4], float (&y)[4]) {
-        const int64_t t = first + min(j, rows - 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = y[i] = 0.f;
-        if (on) read_pairs<T, WHOLE>(a, qkv + t * a.row_stride + static_cast<int64_t>(a.nq + g) * a.d, c, x, y);
-        prepare_pairs<TW, WHOLE>(a, k_w, cos_t, sin_t, t, c, 1.f, x, y);
-    };
-    // values: a thread takes a pair of neighbouring channels and every `groups`-th token
-    const int pairs = a.d / 2, groups = max(1, THREADS / pairs);
-    const int vc = 2 * (tid % pairs), vg = tid / pairs;
-    const bool v_on = vg < groups;
-    const T* vrow = qkv + static_cast<int64_t>(a.v_head0 + g) * a.d + vc;
-
-    float kmax = 0.f, vmax = 0.f;
-    int bad = 0;
-    for (int j0 = 0; j0 < rows; j0 += heads_at_once) {
-        float x[4], y[4];
-        key_pairs(j0 + tid / a.lanes, x, y);
+// Those pairs of a row of q to their places.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void write_pairs(const StoreArgs& a, T* to, int c, const float (&x)[4], const float (&y)[4]) {
+    if constexpr (WHOLE) {
+        const bool apart = a.pairing == 1 && 8 * c < a.rotary_dim;
+        float one[4], two[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            kmax = fmaxf(kmax, cache8::finite(x[i]) ? fabsf(x[i]) : 0.f);
-            kmax = fmaxf(kmax, cache8::finite(y[i]) ? fabsf(y[i]) : 0.f);
+            one[i] = apart ? x[i] : (i % 2 ? y[i / 2] : x[i / 2]);
+            two[i] = apart ? y[i] : (i % 2 ? y[2 + i / 2] : x[2 + i / 2]);
         }
-    }
-    for (int j = vg; j < rows && v_on; j += groups) {
-        const T* v = vrow + (first + j) * a.row_stride;
-        const float x = to_f32<T>(v[0]), y = to_f32<T>(v[1]);
-        vmax = fmaxf(vmax, fmaxf(cache8::finite(x) ? fabsf(x) : 0.f, cache8::finite(y) ? fabsf(y) : 0.f));
-        bad |= !cache8::finite(x) | !cache8::finite(y);
-    }
-    kmax = wave_max(kmax);
-    vmax = wave_max(vmax);
-    if (tid == 0) s_bad = 0;
-    __syncthreads();
-    if (bad) s_bad = 1;
-    if (tid % PULSE_WAVE == 0) {
-        s_max[0][tid / PULSE_WAVE] = kmax;
-        s_max[1][tid / PULSE_WAVE] = vmax;
-    }
-    __syncthreads();
-    kmax = vmax = 0.f;
-#pragma unroll
-    for (int w = 0; w < THREADS / PULSE_WAVE; ++w) {
-        kmax = fmaxf(kmax, s_max[0][w]);
-        vmax = fmaxf(vmax, s_max[1][w]);
-    }
-    const int was_k = fresh ? cache8::LEAST : cache8::exponent_of(had_k), was_v = fresh ? cache8::LEAST : cache8::exponent_of(had_v);
-    const int ek = max(was_k, cache8::exponent_for(kmax)), ev = max(was_v, cache8::exponent_for(vmax));
-    const float by_k = cache8::pow2(-ek), by_v = cache8::pow2(-ev);
-
-    // what the block holds besides the new tokens: nothing (a block that is begun: zeros behind them), or earlier bytes at their scale
-    if (fresh || ek != was_k) {
-        const float down = cache8::pow2(max(was_k - ek, -126));
-        for (int i = tid; i < a.block * a.d; i += THREADS) {
-            const int token = i / a.d;
-            if (token < at || token >= at + rows) kb[i] = fresh ? 0 : static_cast<uint8_t>(cache8::moved(kb[i], down));
+        const int first = apart ? 4 * c : 8 * c, second = apart ? first + a.rotary_dim / 2 : first + 4;
+        if constexpr (sizeof(T) == 2) {
+            auto pack = [](const float* v) {
+                return make_uint2(f32_to_bf16(v[0]) | static_cast<uint32_t>(f32_to_bf16(v[1])) << 16, f32_to_bf16(v[2]) | static_cast<uint32_t>(f32_to_bf16(v[3])) << 16);
+            };
+            *reinterpret_cast<uint2*>(to + first) = pack(one);
+            *reinterpret_cast<uint2*>(to + second) = pack(two);
+        } else {
+            *reinterpret_cast<float4*>(to + first) = make_float4(one[0], one[1], one[2], one[3]);
+            *reinterpret_cast<float4*>(to + second) = make_float4(two[0], two[1], two[2], two[3]);
         }
-    }
-    if (fresh || ev != was_v) {
-        const float down = cache8::pow2(max(was_v - ev, -126));
-        for (int i = tid; i < a.block * a.d; i += THREADS) {
-            const int token = i % a.block;
-            if (token < at || token >= at + rows) vb[i] = fresh ? 0 : static_cast<uint8_t>(cache8::moved(vb[i], down));
-        }
-    }
-    for (int j0 = 0; j0 < rows; j0 += heads_at_once) {
-        float x[4], y[4];
-        const int j = j0 + tid / a.lanes;
-        key_pairs(j, x, y);
-        if (j >= rows || !on) continue;
-        uint8_t* to = kb + static_cast<int64_t>(at + j) * a.d;
+    } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             int ia, ib;
             channels_of(a, 4 * c + i, ia, ib);
             if (2 * (4 * c + i) < a.d) {
-                const uint32_t both = cache8::to_e4m3x2(x[i] * by_k, y[i] * by_k);
+                to[ia] = from_f32<T>(x[i]);
+                to[ib] = from_f32<T>(y[i]);
+            }
+        }
+    }
+}
+
+// A workgroup's share of q: neighbouring groups of lanes take neighbouring heads of the rows in turn.
+template <typename T, typename TW, bool WHOLE>
+__device__ __forceinline__ void rows_of_q(const StoreArgs& a, int64_t first, const T* qkv, T* q_out, const TW* q_w, const float* cos_t,
+                                          const float* sin_t, const int* positions) {
+    const int tid = threadIdx.x, c = tid % a.lanes;
+    const int64_t i = first * (THREADS / a.lanes) + tid / a.lanes;
+    const bool live = i < static_cast<int64_t>(a.tokens) * a.nq, on = 8 * c < a.d;
+    const int64_t t = live ? i / a.nq : 0;
+    const int h = live ? static_cast<int>(i - t * a.nq) : 0;
+    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+    if (on) read_pairs<T, WHOLE>(a, qkv + t * a.row_stride + static_cast<int64_t>(h) * a.d, c, x, y);
+    float factor = 1.f;
+    if (a.temp_every > 0) factor = 1.f + a.temp_coef * logf(static_cast<float>((positions[t] + 1) / a.temp_every) + 1.f);
+    prepare_pairs<TW, WHOLE>(a, q_w, cos_t, sin_t, t, c, factor, x, y);
+    if (on && live) write_pairs<T, WHOLE>(a, q_out + t * a.q_stride + static_cast<int64_t>(h) * a.d, c, x, y);
+}
+
+// The largest finite |x| of the keys and of the values that the workgroup's threads have, and whether a value is none.
+__device__ __forceinline__ void largest(float& kmax, float& vmax, bool& bad) {
+    __shared__ float s_max[2][THREADS / PULSE_WAVE];
+    __shared__ int s_bad[THREADS / PULSE_WAVE];
+    const int wave = threadIdx.x / PULSE_WAVE;
+    kmax = wave_max(kmax);
+    vmax = wave_max(vmax);
+    const bool any = __any(bad);
+    if (threadIdx.x % PULSE_WAVE == 0) {
+        s_max[0][wave] = kmax;
+        s_max[1][wave] = vmax;
+        s_bad[wave] = any;
+    }
+    __syncthreads();
+    kmax = vmax = 0.f;
+    bad = false;
+#pragma unroll
+    for (int w = 0; w < THREADS / PULSE_WAVE; ++w) {
+        kmax = fmaxf(kmax, s_max[0][w]);
+        vmax = fmaxf(vmax, s_max[1][w]);
+        bad |= s_bad[w] != 0;
+    }
+}
+__device__ __forceinline__ float size_of(float x) { return cache8::finite(x) ? fabsf(x) : 0.f; }
+
+// What a workgroup of a (block, kv head) has to do, or nothing (a list that says what cannot be is not followed).
+struct Job {
+    int first, rows, at, g;
+    uint8_t *keys, *values;      // the block's, of this head: [token][channel], [channel][token]
+    float* scale;
+};
+__device__ __forceinline__ bool job_of(const StoreArgs& a, const int4* work, uint8_t* keys, uint8_t* values, float* scales, Job& j) {
+    const int4 w = work[blockIdx.x / a.nkv];
+    j.g = blockIdx.x % a.nkv;
+    j.first = w.x, j.rows = w.y, j.at = w.w;
+    if (w.y <= 0 || w.z < 0 || w.z >= a.all_blocks || w.w < 0 || w.w + w.y > a.block || w.x < 0 || w.x + w.y > a.tokens) return false;
+    const int64_t page = w.z / a.blocks_per_page, head = page * a.nkv + j.g;
+    const int inner = w.z - static_cast<int>(page) * a.blocks_per_page;
+    j.keys = keys + (head * a.page_size + static_cast<int64_t>(inner) * a.block) * a.d;
+    j.values = values + (head * a.page_size + static_cast<int64_t>(inner) * a.block) * a.d;
+    j.scale = scales + (head * a.blocks_per_page + inner) * 2;
+    return true;
+}
+
+// Blocks of 16 tokens and heads of a multiple of 8 channels, NP * 128 at most, in whole pieces: what is read is kept in registers until
+// the scale is known.  Keys: a group of lanes takes a token's row.  Values: a thread takes a pair of channels and four of the block's
+// tokens, whose bytes are a word; a word that holds earlier tokens too is put together with them.
+template <typename T, typename TW, int NP>
+__global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T* q_out, const TW* __restrict__ q_w, const TW* __restrict__ k_w,
+                                                                const float* __restrict__ cos_t, const float* __restrict__ sin_t,
+                                                                uint8_t* keys, uint8_t* values, float* scales, const int* __restrict__ positions,
+                                                                const int4* __restrict__ work, StoreArgs a) {
+    const int tid = threadIdx.x, block_groups = a.n_blocks * a.nkv;
+    if (static_cast<int>(blockIdx.x) >= block_groups) {
+        rows_of_q<T, TW, true>(a, blockIdx.x - block_groups, qkv, q_out, q_w, cos_t, sin_t, positions);
+        return;
+    }
+    Job j;
+    if (!job_of(a, work, keys, values, scales, j)) return;
+    const int c = tid % a.lanes, at_once = THREADS / a.lanes, d = a.d;
+    const bool on = 8 * c < d, fresh = j.at == 0;
+    const float had_k = fresh ? 0.f : j.scale[0], had_v = fresh ? 0.f : j.scale[1];
+    const int pairs = d / 2, quad = tid / pairs, vc = 2 * (tid % pairs);      // (of the first NP; the others are THREADS / pairs quads further on)
+    const int quads_at_once = THREADS / pairs;
+
+    // everything that is read is asked for before anything waits
+    float kx[NP][4], ky[NP][4], vx[NP][4], vy[NP][4];
+    uint32_t old[NP][2];
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        const int i = n * at_once + tid / a.lanes;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kx[n][e] = ky[n][e] = vx[n][e] = vy[n][e] = 0.f;
+        if (on && i < j.rows) read_pairs<T, true>(a, qkv + static_cast<int64_t>(j.first + i) * a.row_stride + static_cast<int64_t>(a.nq + j.g) * d, c, kx[n], ky[n]);
+        const int qd = quad + n * quads_at_once;
+        old[n][0] = old[n][1] = 0;
+        if (quad < quads_at_once && qd < 4) {
+            if (!fresh) {
+                old[n][0] = *reinterpret_cast<const uint32_t*>(j.values + vc * 16 + qd * 4);
+                old[n][1] = *reinterpret_cast<const uint32_t*>(j.values + vc * 16 + 16 + qd * 4);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 4 * qd + e - j.at;
+                if (row >= 0 && row < j.rows) {
+                    const T* v = qkv + static_cast<int64_t>(j.first + row) * a.row_stride + static_cast<int64_t>(a.v_head0 + j.g) * d + vc;
+                    if constexpr (sizeof(T) == 2) {
+                        const uint32_t u = *reinterpret_cast<const uint32_t*>(v);
+                        vx[n][e] = __uint_as_float(u << 16), vy[n][e] = __uint_as_float(u & 0xffff0000u);
+                    } else {
+                        const float2 u = *reinterpret_cast<const float2*>(v);
+                        vx[n][e] = u.x, vy[n][e] = u.y;
+                    }
+                }
+            }
+        }
+    }
+    float kmax = 0.f, vmax = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        const int i = n * at_once + tid / a.lanes;
+        prepare_pairs<TW, true>(a, k_w, cos_t, sin_t, j.first + min(i, j.rows - 1), c, 1.f, kx[n], ky[n]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (i < j.rows) kmax = fmaxf(kmax, fmaxf(size_of(kx[n][e]), size_of(ky[n][e])));
+            vmax = fmaxf(vmax, fmaxf(size_of(vx[n][e]), size_of(vy[n][e])));
+            bad |= !cache8::finite(vx[n][e]) | !cache8::finite(vy[n][e]);
+        }
+    }
+    largest(kmax, vmax, bad);
+    const int was_k = fresh ? cache8::LEAST : cache8::exponent_of(had_k), was_v = fresh ? cache8::LEAST : cache8::exponent_of(had_v);
+    const int ek = max(was_k, cache8::exponent_for(kmax)), ev = max(was_v, cache8::exponent_for(vmax));
+    const float by_k = cache8::pow2(-ek), by_v = cache8::pow2(-ev);
+    const bool grew_k = !fresh && ek != was_k, grew_v = !fresh && ev != was_v;
+    const float down_k = cache8::pow2(max(was_k - ek, -126)), down_v = cache8::pow2(max(was_v - ev, -126));
+
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        const int i = n * at_once + tid / a.lanes;
+        if (on && i < j.rows) {
+            const bool apart = a.pairing == 1 && 8 * c < a.rotary_dim;
+            const int first = apart ? 4 * c : 8 * c, second = apart ? first + a.rotary_dim / 2 : first + 4;
+            uint32_t lo = 0, hi = 0;
+            if (apart) {
+                lo = cache8::to_e4m3x4(kx[n][0] * by_k, kx[n][1] * by_k, kx[n][2] * by_k, kx[n][3] * by_k);
+                hi = cache8::to_e4m3x4(ky[n][0] * by_k, ky[n][1] * by_k, ky[n][2] * by_k, ky[n][3] * by_k);
+            } else {
+                lo = cache8::to_e4m3x4(kx[n][0] * by_k, ky[n][0] * by_k, kx[n][1] * by_k, ky[n][1] * by_k);
+                hi = cache8::to_e4m3x4(kx[n][2] * by_k, ky[n][2] * by_k, kx[n][3] * by_k, ky[n][3] * by_k);
+            }
+            uint8_t* to = j.keys + (j.at + i) * d;
+            *reinterpret_cast<uint32_t*>(to + first) = lo;
+            *reinterpret_cast<uint32_t*>(to + second) = hi;
+        }
+        const int qd = quad + n * quads_at_once;
+        if (quad < quads_at_once && qd < 4) {
+            uint32_t fill = 0;       // the bytes of the new tokens
+#pragma unroll
+            for (int e = 0; e < 4; ++e) fill |= 4 * qd + e >= j.at && 4 * qd + e < j.at + j.rows ? 0xffu << (8 * e) : 0u;
+            if (fill || fresh || grew_v) {
+                uint32_t x = old[n][0], y = old[n][1];
+                if (grew_v) x = cache8::moved(x, down_v), y = cache8::moved(y, down_v);
+                x = (x & ~fill) | (cache8::to_e4m3x4(vx[n][0] * by_v, vx[n][1] * by_v, vx[n][2] * by_v, vx[n][3] * by_v) & fill);
+                y = (y & ~fill) | (cache8::to_e4m3x4(vy[n][0] * by_v, vy[n][1] * by_v, vy[n][2] * by_v, vy[n][3] * by_v) & fill);
+                *reinterpret_cast<uint32_t*>(j.values + vc * 16 + qd * 4) = x;
+                *reinterpret_cast<uint32_t*>(j.values + vc * 16 + 16 + qd * 4) = y;
+            }
+        }
+    }
+    if ((fresh && j.rows < 16) || grew_k) {
+        // the keys around the new ones: zeros in a block that is begun, else at their new scale
+        uint32_t* all = reinterpret_cast<uint32_t*>(j.keys);
+        const int begin = j.at * d / 4, end = (j.at + j.rows) * d / 4;
+        for (int i = tid; i < 4 * d; i += THREADS)
+            if (i < begin || i >= end) all[i] = fresh ? 0u : cache8::moved(all[i], down_k);
+    }
+    if (tid == 0) {
+        j.scale[0] = cache8::pow2(ek);
+        j.scale[1] = bad || (!fresh && had_v < 0.f) ? -cache8::pow2(ev) : cache8::pow2(ev);
+    }
+}
+
+// Every size: two readings, the first for the scale.
+template <typename T, typename TW>
+__global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out, const TW* __restrict__ q_w, const TW* __restrict__ k_w,
+                                                         const float* __restrict__ cos_t, const float* __restrict__ sin_t, uint8_t* keys,
+                                                         uint8_t* values, float* scales, const int* __restrict__ positions,
+                                                         const int4* __restrict__ work, StoreArgs a) {
+    const int tid = threadIdx.x, block_groups = a.n_blocks * a.nkv;
+    if (static_cast<int>(blockIdx.x) >= block_groups) {
+        rows_of_q<T, TW, false>(a, blockIdx.x - block_groups, qkv, q_out, q_w, cos_t, sin_t, positions);
+        return;
+    }
+    Job j;
+    if (!job_of(a, work, keys, values, scales, j)) return;
+    const int c = tid % a.lanes, at_once = THREADS / a.lanes, d = a.d;
+    const bool on = 8 * c < d, fresh = j.at == 0;
+    const float had_k = fresh ? 0.f : j.scale[0], had_v = fresh ? 0.f : j.scale[1];
+    auto key_pairs = [&](int i, float (&x)[4], float (&y)[4]) {
+        const int64_t t = j.first + min(i, j.rows - 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = y[e] = 0.f;
+        if (on) read_pairs<T, false>(a, qkv + t * a.row_stride + static_cast<int64_t>(a.nq + j.g) * d, c, x, y);
+        prepare_pairs<TW, false>(a, k_w, cos_t, sin_t, t, c, 1.f, x, y);
+    };
+    // values: a thread takes a pair of neighbouring channels and every `groups`-th token
+    const int pairs = d / 2, groups = THREADS / pairs, vc = 2 * (tid % pairs), vg = tid / pairs;
+    const T* vrow = qkv + static_cast<int64_t>(j.first) * a.row_stride + static_cast<int64_t>(a.v_head0 + j.g) * d + vc;
+    float kmax = 0.f, vmax = 0.f;
+    bool bad = false;
+    for (int i0 = 0; i0 < j.rows; i0 += at_once) {
+        float x[4], y[4];
+        key_pairs(i0 + tid / a.lanes, x, y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kmax = fmaxf(kmax, fmaxf(size_of(x[e]), size_of(y[e])));
+    }
+    for (int i = vg; i < j.rows && vg < groups; i += groups) {
+        const float x = to_f32<T>(vrow[i * a.row_stride]), y = to_f32<T>(vrow[i * a.row_stride + 1]);
+        vmax = fmaxf(vmax, fmaxf(size_of(x), size_of(y)));
+        bad |= !cache8::finite(x) | !cache8::finite(y);
+    }
+    largest(kmax, vmax, bad);
+    const int was_k = fresh ? cache8::LEAST : cache8::exponent_of(had_k), was_v = fresh ? cache8::LEAST : cache8::exponent_of(had_v);
+    const int ek = max(was_k, cache8::exponent_for(kmax)), ev = max(was_v, cache8::exponent_for(vmax));
+    const float by_k = cache8::pow2(-ek), by_v = cache8::pow2(-ev);
+
+    // what the block holds besides the new tokens: nothing (a block that is begun: zeros behind them), or earlier bytes at their scale
+    auto around = [&](uint8_t* bytes, bool by_channel, float down) {
+        for (int i = tid; i < a.block * d; i += THREADS) {
+            const int token = by_channel ? i % a.block : i / d;
+            if (token < j.at || token >= j.at + j.rows) bytes[i] = fresh ? 0 : static_cast<uint8_t>(cache8::moved(bytes[i], down));
+        }
+    };
+    if (fresh || ek != was_k) around(j.keys, false, cache8::pow2(max(was_k - ek, -126)));
+    if (fresh || ev != was_v) around(j.values, true, cache8::pow2(max(was_v - ev, -126)));
+    for (int i0 = 0; i0 < j.rows; i0 += at_once) {
+        float x[4], y[4];
+        const int i = i0 + tid / a.lanes;
+        key_pairs(i, x, y);
+        if (i >= j.rows || !on) continue;
+        uint8_t* to = j.keys + static_cast<int64_t>(j.at + i) * d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            int ia, ib;
+            channels_of(a, 4 * c + e, ia, ib);
+            if (2 * (4 * c + e) < d) {
+                const uint32_t both = cache8::to_e4m3x2(x[e] * by_k, y[e] * by_k);
                 to[ia] = static_cast<uint8_t>(both);
                 to[ib] = static_cast<uint8_t>(both >> 8);
             }
         }
     }
-    for (int j = vg; j < rows && v_on; j += groups) {
-        const T* v = vrow + (first + j) * a.row_stride;
-        const uint32_t both = cache8::to_e4m3x2(to_f32<T>(v[0]) * by_v, to_f32<T>(v[1]) * by_v);
-        uint8_t* to = vb + static_cast<int64_t>(vc) * a.block + at + j;
+    for (int i = vg; i < j.rows && vg < groups; i += groups) {
+        const uint32_t both = cache8::to_e4m3x2(to_f32<T>(vrow[i * a.row_stride]) * by_v, to_f32<T>(vrow[i * a.row_stride + 1]) * by_v);
+        uint8_t* to = j.values + static_cast<int64_t>(vc) * a.block + j.at + i;
         to[0] = static_cast<uint8_t>(both);
         to[a.block] = static_cast<uint8_t>(both >> 8);
     }
     if (tid == 0) {
-        const bool marked = s_bad || (!fresh && had_v < 0.f);
-        sc[0] = cache8::pow2(ek);
-        sc[1] = marked ? -cache8::pow2(ev) : cache8::pow2(ev);
+        j.scale[0] = cache8::pow2(ek);
+        j.scale[1] = bad || (!fresh && had_v < 0.f) ? -cache8::pow2(ev) : cache8::pow2(ev);
     }
 }
 
@@ -291,25 +447,28 @@ extern "C" int pulse_store8(const void* qkv, int x_dtype, int64_t row_stride, vo
     PULSE_REQUIRE(grid <= 0x7fffffff, "store8: too many rows");
     const int size = x_dtype == PULSE_F32 ? 4 : 2, w_size = w_dtype == PULSE_F32 ? 4 : 2;
     auto aligned = [](const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; };
-    const bool whole = d % 8 == 0 && rotary_dim % 8 == 0 && row_stride % 4 == 0 && aligned(qkv, 4 * size) && aligned(q_w, 4 * w_size) &&
-                       aligned(k_w, 4 * w_size);
-    auto go = [&](auto x, auto w, auto v) {
+    const bool whole = block == cache8::BLOCK && d % 8 == 0 && rotary_dim % 8 == 0 && row_stride % 4 == 0 && q_stride % 4 == 0 &&
+                       aligned(qkv, 4 * size) && aligned(q_out, 4 * size) && aligned(q_w, 4 * w_size) && aligned(k_w, 4 * w_size) &&
+                       aligned(cos_t, 16) && aligned(sin_t, 16) && aligned(keys, 4) && aligned(values, 4);
+    auto go = [&](auto x, auto w) {
         using T = decltype(x);
         using TW = decltype(w);
-        store8_kernel<T, TW, decltype(v)::value><<<static_cast<int>(grid), THREADS, 0, stream>>>(
-            static_cast<const T*>(qkv), static_cast<T*>(q_out), static_cast<const TW*>(q_w), static_cast<const TW*>(k_w), cos_t, sin_t,
-            static_cast<uint8_t*>(keys), static_cast<uint8_t*>(values), scales, positions, reinterpret_cast<const int4*>(work), a);
+        auto run = [&](auto kernel) {
+            kernel<<<static_cast<int>(grid), THREADS, 0, stream>>>(
+                static_cast<const T*>(qkv), static_cast<T*>(q_out), static_cast<const TW*>(q_w), static_cast<const TW*>(k_w), cos_t, sin_t,
+                static_cast<uint8_t*>(keys), static_cast<uint8_t*>(values), scales, positions, reinterpret_cast<const int4*>(work), a);
+        };
+        if (!whole) run(store8_kernel<T, TW>);
+        else if (d <= 128) run(store8_blocks_kernel<T, TW, 1>);
+        else if (d <= 256) run(store8_blocks_kernel<T, TW, 2>);
+        else run(store8_blocks_kernel<T, TW, 4>);
     };
-    auto by_weight = [&](auto x, auto v) {
-        if (w_dtype == PULSE_F32) go(x, float(), v);
-        else go(x, bf16_t(), v);
+    auto by_weight = [&](auto x) {
+        if (w_dtype == PULSE_F32) go(x, float());
+        else go(x, bf16_t());
     };
-    auto by_type = [&](auto v) {
-        if (x_dtype == PULSE_F32) by_weight(float(), v);
-        else by_weight(bf16_t(), v);
-    };
-    if (whole) by_type(std::true_type());
-    else by_type(std::false_type());
+    if (x_dtype == PULSE_F32) by_weight(float());
+    else by_weight(bf16_t());
     PULSE_LAUNCH_CHECK("store8");
     return 0;
 }
