@@ -148,9 +148,17 @@ __global__ __launch_bounds__(THREADS) void step_maps_kernel(MapArgs a) {
 
 }  // namespace
 
-extern "C" int pulse_step_maps(const int* start, const int* count, int requests, const int* pages, int n_pages, int page_size,
-                               int num_pages, int block, int* first_row, int* positions, int* token_entry, int* slots, int rows,
-                               int* table, int width, int* blocks, int n_blocks, hipStream_t stream) {
+// The entry point's arguments (ops/cache8.py fills it; the same fields in the same order).
+struct PulseStepMaps {
+    const int *start, *count, *pages;
+    int *first_row, *positions, *token_entry, *slots, *table, *blocks;
+    int requests, n_pages, page_size, num_pages, block, rows, width, n_blocks;
+};
+
+extern "C" int pulse_step_maps(const PulseStepMaps* args, hipStream_t stream) {
+    PULSE_REQUIRE(args != nullptr, "step_maps: no arguments");
+    const auto [start, count, pages, first_row, positions, token_entry, slots, table, blocks, requests, n_pages, page_size, num_pages, block,
+                rows, width, n_blocks] = *args;
     PULSE_REQUIRE(requests > 0 && requests <= MAX_REQUESTS, "step_maps: %d requests (1 to %d are served)", requests, MAX_REQUESTS);
     PULSE_REQUIRE(start && count && page_size > 0 && num_pages > 0 && rows >= 0 && width >= 0 && n_blocks >= 0, "step_maps: bad sizes");
     PULSE_REQUIRE(static_cast<int64_t>(num_pages) * page_size <= 0x7fffffff, "step_maps: %d pages of %d tokens have no slot numbers in 32 bits",

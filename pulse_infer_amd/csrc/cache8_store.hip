@@ -422,11 +422,34 @@ __global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out,
 
 }  // namespace
 
-extern "C" int pulse_store8(const void* qkv, int x_dtype, int64_t row_stride, void* q_out, int64_t q_stride, const void* q_w,
-                            const void* k_w, int w_dtype, float eps, const float* cos_t, const float* sin_t, int rotary_dim, int pairing,
-                            void* keys, void* values, float* scales, int num_pages, int page_size, const int* positions, const int* work,
-                            int n_blocks, int tokens, int nq, int nkv, int d, int plain_norm, int v_head0, float temp_coef,
-                            int temp_every, hipStream_t stream) {
+// The entry point's arguments (ops/cache8.py fills it; the same fields in the same order).
+struct PulseStore8 {
+    const void* qkv;
+    int64_t row_stride;
+    void* q_out;
+    int64_t q_stride;
+    const void *q_w, *k_w;
+    const float *cos_t, *sin_t;
+    void *keys, *values;
+    float* scales;
+    const int *positions, *work;
+    int x_dtype, w_dtype, rotary_dim, pairing, num_pages, page_size, n_blocks, tokens, nq, nkv, d, plain_norm, v_head0, temp_every;
+    float eps, temp_coef;
+};
+
+extern "C" int pulse_store8(const PulseStore8* args, hipStream_t stream) {
+    PULSE_REQUIRE(args != nullptr, "store8: no arguments");
+    const PulseStore8& in = *args;
+    const void *qkv = in.qkv, *q_w = in.q_w, *k_w = in.k_w;
+    void *q_out = in.q_out, *keys = in.keys, *values = in.values;
+    const float *cos_t = in.cos_t, *sin_t = in.sin_t;
+    float* scales = in.scales;
+    const int *positions = in.positions, *work = in.work;
+    const int64_t row_stride = in.row_stride, q_stride = in.q_stride;
+    const int x_dtype = in.x_dtype, w_dtype = in.w_dtype, rotary_dim = in.rotary_dim, pairing = in.pairing, num_pages = in.num_pages,
+              page_size = in.page_size, n_blocks = in.n_blocks, tokens = in.tokens, nq = in.nq, nkv = in.nkv, d = in.d,
+              plain_norm = in.plain_norm, v_head0 = in.v_head0, temp_every = in.temp_every;
+    const float eps = in.eps, temp_coef = in.temp_coef;
     PULSE_REQUIRE(pulse_dtype_ok(x_dtype) && pulse_dtype_ok(w_dtype), "store8: unknown storage type");
     PULSE_REQUIRE(tokens >= 0 && n_blocks >= 0 && nq > 0 && nkv > 0 && num_pages > 0 && page_size > 0 && v_head0 >= 0, "store8: bad sizes");
     PULSE_REQUIRE(d >= 2 && d % 2 == 0 && d <= MAX_DIM, "store8: heads of %d channels (even, up to %d)", d, MAX_DIM);

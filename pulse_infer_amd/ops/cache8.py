@@ -11,14 +11,14 @@ falls back to another implementation.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import Any, Callable, List, Optional, Sequence, Tuple
 
 import torch
 
 from ..cache.specs import Paged8CacheView, block_tokens
 from .device import compute_units
-from .kernels import _TAG, _f32, _gpu, _i32, _i64, _need, _ptr, _stream, _tag
+from .kernels import _TAG, _gpu, _i32, _need, _ptr, _stream, _tag
 from .library import KernelError, call
 
 MAX_REQUESTS = 4096          # of step_maps
@@ -60,6 +60,16 @@ def _pages(what: str, view: Paged8CacheView, nkv: int, d: int) -> Tuple[int, int
     if not (keys.is_contiguous() and values.is_contiguous() and scales.is_contiguous()) or (keys.data_ptr() | values.data_ptr() | scales.data_ptr()) % 16:
         _refuse(what, "the cache must be contiguous and aligned to 16 bytes")
     return pages, page
+
+
+# The arguments of the entry points as the structures of csrc/cache8_maps.hip, cache8_store.hip and cache8_attn.h, put together at once.
+_MAPS = struct.Struct("@9Q8i")
+_STORE = struct.Struct("@QqQq9Q14i2f")
+_ATTN = struct.Struct("@QqQq7Qq5Q14i2f")
+
+
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _block_list(what: str, blocks: torch.Tensor) -> int:
@@ -116,9 +126,9 @@ def step_maps(start: torch.Tensor, count: torch.Tensor, *, page_size: int, num_p
         _refuse(what, "slots and blocks need the pages or the table")
     if blocks is not None:
         places = _block_list(what, blocks)
-    call("pulse_step_maps", _ptr(start), _ptr(count), _i32(n), _ptr(pages), _i32(listed), _i32(page_size), _i32(num_pages), _i32(block),
-         _ptr(first_row), _ptr(positions), _ptr(token_entry), _ptr(slots), _i32(max(rows, 0)), _ptr(table), _i32(width), _ptr(blocks),
-         _i32(places), _stream())
+    call("pulse_step_maps", _MAPS.pack(start.data_ptr(), count.data_ptr(), _at(pages), _at(first_row), _at(positions), _at(token_entry),
+                                       _at(slots), _at(table), _at(blocks), n, listed, page_size, num_pages, block, max(rows, 0), width,
+                                       places), _stream())
 
 
 def blocks_touched(entries: Sequence[Any], page_size: int) -> int:
@@ -180,23 +190,13 @@ def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, vie
         coef, every = float(q_temperature[0]), int(q_temperature[1])
         if every <= 0:
             _refuse(what, "the query temperature's interval must be positive")
-    call("pulse_store8", _ptr(qkv), _i32(_tag(qkv, what)), _i64(stride), _ptr(q_out), _i64(q_stride), _ptr(q_weight),
-         _ptr(k_weight), _i32(w_tag), _f32(eps), _ptr(cos), _ptr(sin), _i32(rotated), _i32(pairing), _ptr(view.keys), _ptr(view.values),
-         _ptr(view.scales), _i32(pages), _i32(page), _ptr(positions), _ptr(blocks), _i32(places), _i32(tokens), _i32(nq), _i32(nkv),
-         _i32(d), _i32(plain_norm), _i32(v_head0), _f32(coef), _i32(every), _stream())
+    call("pulse_store8", _STORE.pack(
+        qkv.data_ptr(), stride, q_out.data_ptr(), q_stride, _at(q_weight), _at(k_weight), _at(cos), _at(sin), view.keys.data_ptr(),
+        view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(), blocks.data_ptr(), _tag(qkv, what), w_tag, rotated, pairing,
+        pages, page, places, tokens, nq, nkv, d, plain_norm, v_head0, every, eps, coef), _stream())
 
 
 # --------------------------------------------------------------------------------------------------------- the attention
-class _Attn8(ctypes.Structure):
-    # as PulseAttn8 of csrc/cache8_attn.h
-    _fields_ = ([("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("o_stride", ctypes.c_int64)]
-                + [(n, ctypes.c_void_p) for n in ("keys", "values", "scales", "positions", "token_entry", "table", "gate")]
-                + [("gate_stride", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("sink", "items", "cut", "part_o", "part_ml")]
-                + [(n, ctypes.c_int) for n in ("dtype", "tokens", "entries", "table_width", "nq", "nkv", "d", "page_size", "num_pages",
-                                               "window", "chunk", "gate_width", "n_items", "max_work")]
-                + [("scale", ctypes.c_float), ("softcap", ctypes.c_float)])
-
-
 def matrix_cores(d: int, page_size: int, dtype: torch.dtype) -> bool:
     """Whether attention runs on the matrix cores; anything else goes to the kernel that serves every size."""
     return dtype == torch.bfloat16 and d % 32 == 0 and d <= 256 and page_size % 16 == 0
@@ -223,15 +223,15 @@ class AttentionPlan:
         _need(dtype in (torch.bfloat16, torch.float32), f"plan: storage type {dtype} is not supported (float32 or bfloat16)")
         self.nq, self.nkv, self.d, self.page_size, self.dtype = nq, nkv, d, int(page_size), dtype
         self.window, self.chunk, self.workspace = int(window), int(chunk), workspace
+        self.tag = _TAG[dtype]
         self.rows = max((e.first_row + e.count for e in entries), default=0)
         self.entries = len(entries)
         self.matrix = matrix_cores(d, page_size, dtype)
         self.device = torch.device(device)
         self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, cut)
-        self.calls: List[Tuple] = []      # (entry point, arguments without the call's tensors, columns of the room for pieces)
-        base = _Attn8(dtype=_TAG[dtype], nq=nq, nkv=nkv, d=d, page_size=self.page_size, window=self.window, chunk=self.chunk)
+        self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces)
         if not self.matrix:
-            self.calls.append(("pulse_attn8_plain", base, 0))
+            self.calls.append(("pulse_attn8_plain", 0, 0, 0, 0, 0))
             return
         group = nq // nkv
         few, many = [], []
@@ -254,9 +254,7 @@ class AttentionPlan:
             on_gpu = to_device([v for _, row, rows, entry in items for v in (row, rows, entry, 0)])
             cut = torch.empty(4 + 4 * room + 2 * n, dtype=torch.int32, device=self.device)
             self.works.append((on_gpu, n, slots, least, room, cut))
-            args = _Attn8.from_buffer_copy(base)
-            args.items, args.cut, args.n_items, args.max_work = on_gpu.data_ptr(), cut.data_ptr(), n, room
-            self.calls.append((name, args, 0 if whole else room * groups * columns))
+            self.calls.append((name, on_gpu.data_ptr(), cut.data_ptr(), n, room, 0 if whole else room * groups * columns))
 
         add("pulse_attn8_few", FEW, few, nkv * ((group + FEW - 1) // FEW), self.FEW_SLOTS, self.FEW_LEAST, self.FEW_EVEN)
         # The longest walks first; where two workgroups share a unit, the second ones' from the other end, the shortest beside the longest.
@@ -339,17 +337,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     q_at, out_at = q.data_ptr(), out.data_ptr()
     if plan.matrix and (q_at % 16 or q_stride % 8 or out_at % 8 or o_stride % 4):
         _refuse(what, "rows must be aligned to 16 bytes")
-    for name, args, rows in plan.calls:
-        args = _Attn8.from_buffer_copy(args)      # (its own: a call may be kept and made again)
-        args.q, args.q_stride, args.out, args.o_stride = q_at, q_stride, out_at, o_stride
-        args.keys, args.values, args.scales = view.keys.data_ptr(), view.values.data_ptr(), view.scales.data_ptr()
-        args.positions, args.token_entry, args.table = positions.data_ptr(), token_entry.data_ptr(), table.data_ptr()
-        args.entries, args.table_width = table.shape
-        args.tokens, args.num_pages, args.scale, args.softcap = tokens, pages, scale, softcap
-        if gate is not None:
-            args.gate, args.gate_stride, args.gate_width = gate.data_ptr(), gate_stride, gate_width
-        if sink is not None:
-            args.sink = sink.data_ptr()
+    for name, items, cut, n_items, room, rows in plan.calls:
+        part_o = part_ml = 0
         if rows:
             if workspace is not None:
                 o = workspace.buffer("attention8.part_o", rows, d, torch.float32)
@@ -357,5 +346,9 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
             else:
                 o = torch.empty((rows, d), dtype=torch.float32, device=q.device)
                 ml = torch.empty((rows, 2), dtype=torch.float32, device=q.device)
-            args.part_o, args.part_ml = o.data_ptr(), ml.data_ptr()
-        call(name, ctypes.byref(args), _stream())
+            part_o, part_ml = o.data_ptr(), ml.data_ptr()
+        call(name, _ATTN.pack(
+            q_at, q_stride, out_at, o_stride, view.keys.data_ptr(), view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(),
+            token_entry.data_ptr(), table.data_ptr(), _at(gate), gate_stride, _at(sink), items, cut, part_o, part_ml, plan.tag, tokens,
+            table.shape[0], table.shape[1], nq, nkv, d, page, pages, plan.window, plan.chunk, gate_width, n_items, room, scale, softcap),
+            _stream())
