@@ -38,6 +38,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--init", default="fan_in", help="random weights: 'fan_in' or a standard deviation such as 0.02")
     p.add_argument("--dtype", choices=["bfloat16", "float32", "bf16", "f32"], default="bfloat16")
     p.add_argument("--device", default="cuda:0")
+    p.add_argument("--cache-dtype", choices=["auto", "float8_e4m3"], default="auto",
+                   help="how attention keeps keys and values: as the activations, or in 8 bits with a scale for every 16 tokens and head")
     p.add_argument("--prompt-ids", action="append", default=[], help="comma separated token ids; may be repeated")
     p.add_argument("--prompt-file", default=None, help="JSON file: a list of lists of token ids")
     p.add_argument("--prompt-len", type=int, action="append", default=[], help="a prompt of N seeded random ids; may be repeated")
@@ -138,10 +140,11 @@ def main(argv: Optional[List[str]] = None) -> int:
                    extend_portions=not args.fixed_chunk)
     if args.random_weights:
         init = args.init if args.init == "fan_in" else float(args.init)
-        llm = LLM.from_config_random(config, weights_seed=args.seed, init=init, dtype=dtype, device=args.device, **options)
+        llm = LLM.from_config_random(config, weights_seed=args.seed, init=init, dtype=dtype, device=args.device,
+                                     cache_dtype=args.cache_dtype, **options)
     else:
         llm = LLM.from_pretrained(model_dir, dtype=dtype, device=args.device, config_overrides=overrides,
-                                  strict=args.strict, **options)
+                                  strict=args.strict, cache_dtype=args.cache_dtype, **options)
 
     prompts: List[List[int]] = [[int(t) for t in s.split(",") if t.strip()] for s in args.prompt_ids]
     if args.prompt_file:

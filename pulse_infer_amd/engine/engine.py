@@ -285,6 +285,11 @@ class ContinuousBatchEngine:
         return self.scheduler.get_stats()
 
 
+def _options(cache_dtype: str) -> Optional[Dict[str, Any]]:
+    """What a model's builder is told beyond its configuration (nothing, where that is all as usual)."""
+    return None if cache_dtype == "auto" else {"cache_dtype": cache_dtype}
+
+
 class LLM:
     """Python entry point: a model folder in, generated token ids out."""
 
@@ -305,21 +310,24 @@ class LLM:
 
     @classmethod
     def from_pretrained(cls, model_dir: str, dtype: str = "bfloat16", device: str = "cuda:0",
-                        config_overrides: Optional[Dict[str, Any]] = None, strict: bool = False, **engine_options):
-        """``strict``: a tensor in the folder that no part of the model asks for is an error (else a warning)."""
+                        config_overrides: Optional[Dict[str, Any]] = None, strict: bool = False, cache_dtype: str = "auto",
+                        **engine_options):
+        """``strict``: a tensor in the folder that no part of the model asks for is an error (else a warning).
+        ``cache_dtype``: "auto" (keys and values as the activations) or "float8_e4m3" (in 8 bits with a scale for every 16 tokens and
+        head: half the memory, and half of what a decoding step reads of it)."""
         config, model = load_model(model_dir, mode=dtype, device=device, config_overrides=config_overrides,
-                                   strict=strict)
+                                   strict=strict, options=_options(cache_dtype))
         return cls(model, config, **engine_options)
 
     @classmethod
     def from_config_random(cls, config: Any, weights_seed: int = 0, init: Any = "fan_in", dtype: str = "bfloat16",
-                           device: str = "cuda:0", **engine_options):
+                           device: str = "cuda:0", cache_dtype: str = "auto", **engine_options):
         """Random weights made on the GPU, without a file (for sizes not worth writing to disk)."""
         from ..models.causal_lm import expected_tensors
         from ..weights.random_init import RandomSource
 
         source = RandomSource(expected_tensors(config.model_spec()), weights_seed, init, torch.bfloat16, device=device)
-        model = build_model(config, source, mode=dtype, device=device)
+        model = build_model(config, source, mode=dtype, device=device, options=_options(cache_dtype))
         return cls(model, config, **engine_options)
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 32, temperature: float = 0.0,

@@ -23,6 +23,7 @@ import torch
 from .. import log
 from ..cache.manager import CacheManager
 from ..models.causal_lm import CausalLM
+from ..ops import cache8
 from ..parts.base import EntryMeta, StepContext, contexts_uneven
 
 
@@ -191,6 +192,54 @@ class ModelRunner:
             flat[offsets[8 + gi]:offsets[9 + gi]] = table.reshape(-1)
         flat[offsets[8 + len(widths)]] = max(m.start + m.count for m in metas)
 
+    def _made_on_device(self, entries: Sequence[StepEntry], metas: List[EntryMeta], want_rows: List[int], max_context: int, uneven: bool,
+                        feed=None) -> StepContext:
+        """The context of a step that is run once: the host sends the ids, three numbers a request and the requests' pages, one after
+        the other; rows, positions and block tables are made of them on the device (``cache8.step_maps``)."""
+        cache, groups = self.cache, self.cache.groups
+        total, batch = metas[-1].first_row + metas[-1].count, len(metas)
+        widths = [max(1, max(g.pages_for(m.start + m.count) for m in metas)) for g in groups]
+        if self.device.type != "cuda" or batch > cache8.MAX_REQUESTS:      # (no GPU, or more than its maps are made for at once: on the host)
+            offsets = self._layout(total, batch, len(want_rows), widths)
+            flat = np.zeros(int(offsets[-1]), dtype=np.int32)
+            self._fill(flat, offsets, entries, metas, want_rows, widths)
+            dev = self._staging.upload(flat)
+            self._feed(dev[offsets[0]:offsets[1]], feed)
+            return self._context(dev, offsets, metas, len(want_rows), widths, self.model.workspace, max_context, uneven)
+        ints: List[int] = []
+        for e in entries:
+            ints.extend(e.tokens)
+        ints.extend(m.start for m in metas)
+        ints.extend(m.count for m in metas)
+        ints.extend(m.slot for m in metas)
+        ints.extend(want_rows)
+        ints.append(max_context)
+        cuts = [0, total, total + batch, total + 2 * batch, total + 3 * batch, len(ints) - 1, len(ints)]
+        for gi, g in enumerate(groups):
+            for m in metas:
+                ints.extend(cache.table(gi, m.request)[:g.pages_for(m.start + m.count)])
+            cuts.append(len(ints))
+        sent = self._staging.upload_values(ints)
+        ids, start, count, slot, want, live = (sent[a:b] for a, b in zip(cuts, cuts[1:7]))
+        self._feed(ids, feed)
+        made = torch.empty(2 * total + batch + 1 + batch * sum(widths), dtype=torch.int32, device=self.device)
+        positions, token_entry, first_row = made[:total], made[total:2 * total], made[2 * total:2 * total + batch + 1]
+        tables, at = {}, 2 * total + batch + 1
+        rows: dict = dict(positions=positions, token_entry=token_entry, first_row=first_row)
+        for gi, (g, width) in enumerate(zip(groups, widths)):
+            tables[gi] = made[at:at + batch * width].view(batch, width)
+            at += batch * width
+            cache8.step_maps(start, count, page_size=g.page_size, num_pages=g.pool.num_pages, pages=sent[cuts[6 + gi]:cuts[7 + gi]],
+                             table=tables[gi], **rows)
+            rows = {}
+        if rows:                             # (a model that pages nothing)
+            cache8.step_maps(start, count, page_size=cache.page_size, num_pages=1, **rows)
+        return StepContext(
+            num_tokens=total, entries=metas, token_ids=ids, positions=positions, token_entry=token_entry, entry_start=start,
+            entry_count=count, entry_first_row=first_row, entry_slot=slot, block_tables=tables, want_rows=want, num_wanted=len(want_rows),
+            workspace=self.model.workspace, max_count=max(m.count for m in metas), max_context=max_context, live_context=live, uneven=uneven,
+            upload=self._staging.upload_values)
+
     def _refill(self, rec: "_Captured", entries: Sequence[StepEntry], metas: List[EntryMeta]) -> None:
         """The integers of a step of single tokens in a recording's buffer: only what changes from one such step to
         the next (ids, positions, slots, the longest context) and the block-table rows of requests whose tables have
@@ -257,14 +306,7 @@ class ModelRunner:
         if self._graph_ok(entries, metas) and self._graph_ready(len(metas), max_context, uneven):
             logits = self._step_captured(entries, metas, want_rows, max_context, uneven, feed)
         else:
-            widths = [max(1, max(g.pages_for(m.start + m.count) for m in metas)) for g in cache.groups]
-            offsets = self._layout(total, len(metas), len(want_rows), widths)
-            flat = np.zeros(int(offsets[-1]), dtype=np.int32)
-            self._fill(flat, offsets, entries, metas, want_rows, widths)
-            dev = self._staging.upload(flat)
-            self._feed(dev[offsets[0]:offsets[1]], feed)
-            ctx = self._context(dev, offsets, metas, len(want_rows), widths, self.model.workspace, max_context, uneven)
-            logits = self.model.forward(ctx, self.views)
+            logits = self.model.forward(self._made_on_device(entries, metas, want_rows, max_context, uneven, feed), self.views)
         for m in metas:
             cache.advance(m.request, m.start + m.count)
         self.steps += 1

@@ -13,6 +13,7 @@ from typing import Any, Dict, List, Optional
 
 import torch
 
+from ..cache.specs import Paged8KVSpec, members
 from ..parts.base import (BLOCKS, EMBEDDINGS, HEADS, NORMS, POSITIONS, BuildContext, EntryMeta, ResidualStream,
                           StepContext, Workspace, joined, says)
 from ..parts.rejoin import OriginRejoin
@@ -21,6 +22,7 @@ from .alike import AlikeRuns
 from .spec import ModelSpec
 
 ACT_DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
+CACHE_DTYPES = ("auto", "float8_e4m3")      # "auto": as the activations; else what attention keeps of keys and values
 
 
 def expected_tensors(spec: ModelSpec) -> Dict[str, TensorSpec]:
@@ -54,6 +56,8 @@ class CausalLM:
         self.act_dtype = ACT_DTYPES[mode]
         self.workspace = Workspace(self.device)
         self.options = dict(options or {})
+        if self.options.get("cache_dtype", "auto") not in CACHE_DTYPES:
+            raise ValueError(f"unknown cache dtype '{self.options['cache_dtype']}', choose from {sorted(CACHE_DTYPES)}")
         loader = WeightLoader(source, expected_tensors(spec), mode, self.device, strict=strict)
         build = BuildContext(loader=loader, mode=mode, device=self.device, act_dtype=self.act_dtype,
                              workspace=self.workspace, options=dict(options or {}))
@@ -78,7 +82,19 @@ class CausalLM:
         out = []
         for run in self.spec.order:
             out.append(None if run.cache_of is not None else self.blocks[run.layer].cache_spec())
+        if self.options.get("cache_dtype", "auto") != "auto":
+            self._check_eight_bits(out)
         return out
+
+    def _check_eight_bits(self, specs: List[Any]) -> None:
+        """Some run must keep its keys and values in 8 bits, and who reads another run's cache must take it as it is."""
+        eight = [any(isinstance(part, Paged8KVSpec) for part in members(spec) or (spec,)) for spec in specs]
+        if not any(eight):
+            raise ValueError(f"no layer of '{self.spec.architecture}' keeps keys and values in 8 bits (cache_dtype "
+                             f"'{self.options['cache_dtype']}'): that is for mixers of kind 'attention'")
+        for index, run in enumerate(self.spec.order):
+            if run.cache_of is not None and isinstance(self.blocks[run.layer].cache_spec(), Paged8KVSpec) != eight[run.cache_of]:
+                raise ValueError(f"order[{index}] reads the cache of order[{run.cache_of}], and only one of the two is for 8 bits")
 
     # ---------------------------------------------------------------- recording
     MAX_RECORDED_ROWS = 64      # up to here every product of a step of single tokens can be this package's own kernel;

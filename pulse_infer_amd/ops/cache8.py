@@ -205,7 +205,7 @@ def matrix_cores(d: int, page_size: int, dtype: torch.dtype) -> bool:
 class AttentionPlan:
     """A step's attention: which rows go together, and how the keys are shared out over the GPU.  The first depends on the step's shape
     alone (how many tokens each request brings); the second is made on the GPU from the positions, by ``cut``, once a step for all
-    layers that are alike in heads, window and chunk."""
+    layers that are alike in heads, window and chunk.  ``plain``: everything goes to the kernel that serves every size."""
 
     # Workgroups a compute unit that a kernel's keys are shared out over, and the fewest tiles of 64 keys of a piece.
     FEW_SLOTS, FEW_LEAST = 4, 8
@@ -216,7 +216,7 @@ class AttentionPlan:
     FEW_COLUMNS = 32     # up to which a portion goes through attn8_few
 
     def __init__(self, entries: Sequence[Any], nq: int, nkv: int, d: int, *, page_size: int, dtype: torch.dtype, window: int = 0,
-                 chunk: int = 0, device: Any = "cuda", workspace: Any = None, to_device: Optional[Callable] = None):
+                 chunk: int = 0, device: Any = "cuda", workspace: Any = None, to_device: Optional[Callable] = None, plain: bool = False):
         _need(nq > 0 and nkv > 0 and nq % nkv == 0, f"plan: {nq} query heads are not a multiple of {nkv} key/value heads")
         _need(0 < d <= MAX_HEAD_DIM, f"plan: heads of {d} channels (up to {MAX_HEAD_DIM})")
         _need(window >= 0 and chunk >= 0 and not (window and chunk), "plan: a window and chunks at once, or a negative one")
@@ -226,7 +226,7 @@ class AttentionPlan:
         self.tag = _TAG[dtype]
         self.rows = max((e.first_row + e.count for e in entries), default=0)
         self.entries = len(entries)
-        self.matrix = matrix_cores(d, page_size, dtype)
+        self.matrix = not plain and matrix_cores(d, page_size, dtype)
         self.device = torch.device(device)
         self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, cut)
         self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces)

@@ -29,6 +29,10 @@ Variations, all parameters of the part:
 * ``chunk = n`` (in place of a window): positions fall into chunks of n, counted from 0, and a token sees the earlier tokens
   of its own chunk only: lo = position - position mod n;
 * ``names``: the tensors' names below the part's prefix.
+
+With the build option ``cache_dtype = "float8_e4m3"`` keys and values are held in 8 bits (``Paged8KVSpec``; ``ops/cache8.py``): norm, rotation
+and the rounding into the pages are one kernel, the attention reads the bytes, and the step's list of blocks and its plan are made once for
+all layers that are alike.  Parts derived from this one keep their caches as they are.
 """
 from __future__ import annotations
 
@@ -36,8 +40,8 @@ from typing import Any, Dict, Optional
 
 import torch
 
-from ..cache.manager import PagedKVSpec
-from ..ops import attention_mfma, kernels
+from ..cache.specs import Paged8CacheView, Paged8KVSpec, PagedKVSpec
+from ..ops import attention_mfma, cache8, kernels
 from ..weights.store import TensorSpec
 from .base import MIXERS, BuildContext, LazyNorm, PagedCacheView, Part, StepContext, StepCost, joined
 from .linear import Linear
@@ -150,7 +154,12 @@ class PagedAttention(Part):
         self.sink = self._load_sink(load, names["sink"]) if params.get("sink", False) else self._fixed_sink(params, build)
         self.act_dtype = build.act_dtype
         self.options = build.options
+        self.eight_bits = type(self) is PagedAttention and build.options.get("cache_dtype") == "float8_e4m3"
+        if self.eight_bits and (self.d % 2 or self.d > cache8.MAX_HEAD_DIM or not self.scale > 0.0):
+            raise ValueError(f"a cache in 8 bits takes heads of an even number of channels up to {cache8.MAX_HEAD_DIM} and a positive "
+                             f"scale, got {self.d} and {self.scale}")
 
+    eight_bits = False
     gate_width = 0     # > 0: the output gate has a logit for each of that many channels of a head (a subclass's)
     score_cap = 0.0
     sink = None
@@ -179,7 +188,9 @@ class PagedAttention(Part):
             raise ValueError("attention has a window or chunks, not both")
         return int(chunk or 0)
 
-    def cache_spec(self) -> PagedKVSpec:
+    def cache_spec(self) -> Any:
+        if self.eight_bits:
+            return Paged8KVSpec(self.nkv, self.d, int(self.window) if self.window is not None else None, self.chunk or None)
         return PagedKVSpec(self.nkv, self.d, int(self.window) if self.window is not None else None,
                            chunk=self.chunk or None)
 
@@ -203,16 +214,19 @@ class PagedAttention(Part):
         tables = ctx.position_product(self.position, self.encodings) if self.position is not None else None
         table = ctx.block_tables[cache.group]
         attn = ws.buffer("attention.out", tokens, q_cols, self.act_dtype)
-        from_raw = self.decodes_from_raw(ctx, cache, qkv, tables)
+        eight = isinstance(cache, Paged8CacheView)
+        from_raw = not eight and self.decodes_from_raw(ctx, cache, qkv, tables)
         # (of the projection only q, k and v are read behind the rotation, which may take them as shares; a gate lies beside them)
         parts = None
-        if self.qkv.may_part(tokens) and not from_raw and rows is None and not self.output_gate and not isinstance(x, LazyNorm) \
+        if self.qkv.may_part(tokens) and not from_raw and not eight and rows is None and not self.output_gate and not isinstance(x, LazyNorm) \
                 and kernels.qk_rope_takes_parts(qkv, self.d, tables.rotary_dim if tables is not None else 0, cache.keys, self.q_w, self.k_w,
                                                 *((tables.cos, tables.sin) if tables is not None else ())):
             parts = self.qkv.forward_parts(x, ws)
         if parts is None:
             self.qkv.forward(x, qkv, rows=rows)
-        if from_raw:
+        if eight:
+            self.attend8(qkv, attn, ctx, cache, table, tables, gate)
+        elif from_raw:
             # decoded tokens only: the attention kernel prepares q and each token's own key itself
             self.attend(qkv, attn, ctx, cache, table, raw=(tables, write), gate=gate)
         else:
@@ -252,6 +266,37 @@ class PagedAttention(Part):
             return True
         return (tables.cos.dtype == torch.float32 and tables.cos.is_contiguous() and tables.sin.is_contiguous()
                 and attention_mfma.decode_takes(self.d, tables.rotary_dim, tables.pairing))
+
+    def attend8(self, qkv: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: Paged8CacheView, table: torch.Tensor, tables: Any,
+                gate: Optional[torch.Tensor]) -> None:
+        """q, k and v of the projection's rows prepared, k and v stored in 8 bits, and ``out`` = attention over the cache."""
+        rotation = dict(cos=tables.cos, sin=tables.sin, rotary_dim=tables.rotary_dim, pairing=tables.pairing) if tables is not None else {}
+        if cache.writable:
+            key = f"attention8.blocks:{cache.group}"
+            if key not in ctx.extras:      # the blocks that the step writes to: once a step, for all layers of the group
+                blocks = ctx.workspace.buffer(f"attention8.blocks:{cache.group}", cache8.blocks_touched(ctx.entries, cache.page_size), 4,
+                                              torch.int32)
+                cache8.step_maps(ctx.entry_start, ctx.entry_count, page_size=cache.page_size, num_pages=cache.keys.shape[0], table=table,
+                                 blocks=blocks)
+                ctx.extras[key] = blocks
+            cache8.store(qkv, qkv, self.nq, self.nkv, self.d, cache, ctx.positions, ctx.extras[key], q_weight=self.q_w, k_weight=self.k_w,
+                         eps=self.eps, plain_norm=self.plain_norm, v_head0=self.v_head0, q_temperature=self.q_temperature, **rotation)
+        else:
+            kernels.qk_rope_kv(qkv, self.nq, self.nkv, self.d, self.q_w, self.k_w, self.eps, rotation.get("cos"), rotation.get("sin"),
+                               rotation.get("rotary_dim", 0), rotation.get("pairing", 0), None, None, ctx.positions, ctx.token_entry, None,
+                               write_kv=False, plain_norm=self.plain_norm, v_head0=self.v_head0, q_temperature=self.q_temperature)
+        window = int(self.window) if self.window is not None else 0
+        plain = self.options.get("attention", "auto") == "generic"
+        key = f"attention8.plan:{self.nq}:{self.nkv}:{self.d}:{window}:{self.chunk}:{cache.page_size}:{plain}"
+        if f"static:{key}" not in ctx.extras:      # which rows go together depends on the step's shape alone
+            ctx.extras[f"static:{key}"] = cache8.AttentionPlan(
+                ctx.entries, self.nq, self.nkv, self.d, page_size=cache.page_size, dtype=qkv.dtype, window=window, chunk=self.chunk,
+                device=qkv.device, workspace=ctx.workspace, to_device=ctx.to_device, plain=plain)
+        plan = ctx.extras[f"static:{key}"]
+        if key not in ctx.extras:                  # how the keys are shared out, on the step's positions
+            ctx.extras[key] = plan.cut(ctx.positions)
+        cache8.attention(qkv, out, plan, cache, ctx.positions, ctx.token_entry, table, self.scale, gate=gate, sink=self.sink,
+                         softcap=self.score_cap)
 
     def attend(self, q: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: PagedCacheView,
                table: torch.Tensor, raw: Optional[tuple] = None, gate: Optional[torch.Tensor] = None) -> None:
