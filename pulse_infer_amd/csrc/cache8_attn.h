@@ -35,8 +35,7 @@ __device__ __forceinline__ float tanh_of(float x) { return 1.f - 2.f / (__expf(2
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + __expf(-x)); }
 
 // Where a cut says what it found: the number of pieces, then the pieces (item, first tile, end, the item's first piece), then for every
-// item its first piece and how many it has.
+// item its first piece and how many it has, then attn8_few's counters of arrived pieces.
 constexpr int CUT_HEAD = 4;
-__host__ __device__ inline int64_t cut_ints(int n_items, int max_work) { return CUT_HEAD + 4 * static_cast<int64_t>(max_work) + 2 * static_cast<int64_t>(n_items); }
 
 }  // namespace cache8

@@ -87,7 +87,7 @@ __device__ __forceinline__ void store4(bf16_t* to, f32x4 x, F factor) {
 
 // ------------------------------------------------------------------------------------------------------------------ the cut
 __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restrict__ items, int n, const int* __restrict__ positions,
-                                                            int window, int chunk, int slots, int least, int max_work, int* cut) {
+                                                            int window, int chunk, int slots, int least, int max_work, int groups, int* cut) {
     __shared__ int s_wave[WAVES];
     const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = tid / PULSE_WAVE;
     auto tiles = [&](int i, int& first) {
@@ -107,6 +107,8 @@ __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restri
     const int length = max(least, (total + slots - 1) / slots);
     int4* work = reinterpret_cast<int4*>(cut + cache8::CUT_HEAD);
     int2* info = reinterpret_cast<int2*>(cut + cache8::CUT_HEAD + 4 * max_work);
+    int* arrived = cut + cache8::CUT_HEAD + 4 * max_work + 2 * n;
+    for (int i = tid; i < n * groups; i += THREADS) arrived[i] = 0;
     int before = 0;
     for (int base = 0; base < n; base += THREADS) {
         const int i = base + tid;
@@ -140,6 +142,69 @@ __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restri
         }
     }
     if (tid == 0) cut[0] = min(before, max_work);
+}
+
+// Two numbers to and from memory that workgroups of one launch share: past the caches that belong to one die (relaxed atomics of the
+// device's scope), so that neither side has to write a cache back or to empty it.
+__device__ __forceinline__ void share2(float* to, float x, float y) {
+    const uint64_t both = static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool SHARED>
+__device__ __forceinline__ float2 shared2(const float* from) {
+    if constexpr (!SHARED) return *reinterpret_cast<const float2*>(from);
+    const uint64_t both = __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float(static_cast<uint32_t>(both)), __uint_as_float(static_cast<uint32_t>(both >> 32)));
+}
+
+// The join: out = sum_z w_z o_z / sum_z w_z l_z, w_z = exp2(m_z - max m), over an item's pieces in their order (pieces of one column are
+// COLS columns and the launch's `heads_x` apart).  A thread takes four channels of one of the columns c0 .. c0 + each - 1 and, where the
+// threads are more than that, every ZS-th piece; their sums meet in LDS.  SHARED: the pieces are this launch's.
+template <int COLS, bool SHARED>
+__device__ __forceinline__ void join_columns(const PulseAttn8& a, int first, int pieces, int heads_x, int x, int c0, int each, int row0, int cols,
+                                             int head0, int heads) {
+    __shared__ f32x4 s_sum[THREADS];
+    __shared__ float s_den[THREADS];
+    const int tid = threadIdx.x, d = a.d, quads = d / 4, units = each * quads, zs = max(1, THREADS / units);
+    const int64_t step = static_cast<int64_t>(heads_x) * COLS, at0 = static_cast<int64_t>(first) * step + static_cast<int64_t>(x) * COLS;
+    for (int u0 = 0; u0 < units; u0 += THREADS) {
+        const int unit = zs > 1 ? tid % units : u0 + tid, z0 = zs > 1 ? tid / units : 0;
+        const int c = c0 + unit / quads, ch = unit % quads * 4;
+        const bool on = unit < units && z0 < zs && c < cols;
+        const int64_t at = at0 + (on ? c : c0);
+        float m = -INFINITY, l = 0.f;
+        f32x4 all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int z = 0; z < pieces; ++z) m = fmaxf(m, shared2<SHARED>(a.part_ml + 2 * (at + z * step)).x);
+        const float ref = m == -INFINITY ? 0.f : m;
+        if (on) {
+#pragma unroll 8
+            for (int z = z0; z < pieces; z += zs) {
+                const float2 ml = shared2<SHARED>(a.part_ml + 2 * (at + z * step));
+                const float* from = a.part_o + (at + z * step) * d + ch;
+                const float2 lo = shared2<SHARED>(from), hi = shared2<SHARED>(from + 2);
+                const f32x4 o = {lo.x, lo.y, hi.x, hi.y};
+                const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+                l += ml.y * f;
+                all += o * f;
+            }
+        }
+        if (zs > 1) {
+            s_sum[tid] = all;
+            s_den[tid] = l;
+            __syncthreads();
+            for (int z = 1; z < zs && z0 == 0 && unit < units; ++z) {
+                all += s_sum[unit + z * units];
+                l += s_den[unit + z * units];
+            }
+        }
+        if (on && z0 == 0) {
+            const int row = row0 + c / heads, hd = head0 + c % heads;
+            const float inv = finish(a, m, l, row, hd);
+            bf16_t* to = static_cast<bf16_t*>(a.out) + row * a.o_stride + static_cast<int64_t>(hd) * d + ch;
+            store4(to, all, [&](int e) { return inv * channel_gate(a, row, hd, ch + e); });
+        }
+    }
 }
 
 // --------------------------------------------------------------------------------------------------------- up to 16 columns
@@ -365,13 +430,26 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
             bf16_t* to = static_cast<bf16_t*>(a.out) + row * a.o_stride + static_cast<int64_t>(hd) * D + ch;
             store4(to, all, [&](int e) { return inv * channel_gate(a, row, hd, ch + e); });
         } else {
-            *reinterpret_cast<f32x4*>(a.part_o + (at + c) * D + ch) = all;
-            if (ch == 0) {
-                a.part_ml[2 * (at + c)] = m;
-                a.part_ml[2 * (at + c) + 1] = sum;
-            }
+            share2(a.part_o + (at + c) * D + ch, all[0], all[1]);
+            share2(a.part_o + (at + c) * D + ch + 2, all[2], all[3]);
+            if (ch == 0) share2(a.part_ml + 2 * (at + c), m, sum);
         }
     }
+    if (whole) return;
+    // The piece that comes last joins them all.  (Its sums go by the pieces' order: who comes last changes nothing.)  A wavefront has
+    // its sums where all dies see them before it meets the others, and only then is the piece counted; the counter is left at zero for the
+    // next launch.  (By a release and an acquire, which write a die's cache back for every piece, 24 requests took 82 us for 42.)
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    __shared__ int s_last;
+    int* arrived = const_cast<int*>(a.cut) + cache8::CUT_HEAD + 4 * a.max_work + 2 * a.n_items + item * gridDim.x + blockIdx.x;
+    __syncthreads();
+    if (tid == 0) {
+        const int before = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = before == info.y - 1;
+        if (s_last) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (s_last) join_columns<FEW, true>(a, first_piece, uniform(info.y), gridDim.x, blockIdx.x, 0, ntok * heads, row0, ntok * heads, g * group + part * FEW, heads);
 }
 
 // ------------------------------------------------------------------------------------------------------------ 128 columns
@@ -646,60 +724,16 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     }
 }
 
-// ---------------------------------------------------------------------------------------------------------------- the join
-// out = sum_z w_z o_z / sum_z w_z l_z, w_z = exp2(m_z - max m), over an item's pieces in their order.
-// A workgroup takes `each` of an item's columns, a thread four channels of a column and every ZS-th piece; their sums meet in LDS.
-template <int COLS>
-__global__ __launch_bounds__(THREADS) void attn8_join_kernel(PulseAttn8 a, int head_groups, int each) {
+// The portions' pieces, 16 columns a workgroup (two thirds of a launch's time is that it is one: the few's last piece joins them itself,
+// but 128 columns of a head take longer than that for one workgroup).
+__global__ __launch_bounds__(THREADS) void attn8_join_kernel(PulseAttn8 a) {
     const int item = blockIdx.y;
     const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::CUT_HEAD + 4 * a.max_work)[item];
     const int first = uniform(info.x), pieces = uniform(info.y);
     if (pieces <= 1) return;
-    __shared__ f32x4 s_o[THREADS];
-    __shared__ float s_l[THREADS];
     const int4 it = reinterpret_cast<const int4*>(a.items)[item];
-    const int gp = blockIdx.x;                 // the kv head and sixteen of its heads
-    const int group = a.nq / a.nkv, g = gp / head_groups, part = gp % head_groups;
-    const int heads = COLS == FEW ? min(group - part * FEW, FEW) : group, d = a.d, quads = d / 4;
-    const int cols = it.y * heads, units = each * quads, zs = max(1, THREADS / units), tid = threadIdx.x;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * COLS;
-    const int64_t at0 = static_cast<int64_t>(first) * step + static_cast<int64_t>(gp) * COLS;
-    for (int u0 = 0; u0 < units; u0 += THREADS) {         // (one turn where the columns' channels are no more than the threads)
-        const int unit = zs > 1 ? tid % units : u0 + tid, z0 = zs > 1 ? tid / units : 0;
-        const int c = blockIdx.z * each + unit / quads, ch = unit % quads * 4;
-        const bool on = unit < units && z0 < zs && c < cols;
-        const int64_t at = at0 + (on ? c : 0);
-        float m = -INFINITY, l = 0.f;
-        f32x4 all = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int z = 0; z < pieces; ++z) m = fmaxf(m, a.part_ml[2 * (at + z * step)]);
-        const float ref = m == -INFINITY ? 0.f : m;
-        if (on) {
-#pragma unroll 4
-            for (int z = z0; z < pieces; z += zs) {
-                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (at + z * step));
-                const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_o + (at + z * step) * d + ch);
-                const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-                l += ml.y * f;
-                all += o * f;
-            }
-        }
-        if (zs > 1) {
-            s_o[tid] = all;
-            s_l[tid] = l;
-            __syncthreads();
-            for (int z = 1; z < zs && z0 == 0 && unit < units; ++z) {
-                all += s_o[unit + z * units];
-                l += s_l[unit + z * units];
-            }
-        }
-        if (on && z0 == 0) {
-            const int row = it.x + c / heads, hd = g * group + part * FEW + c % heads;
-            const float inv = finish(a, m, l, row, hd);
-            bf16_t* to = static_cast<bf16_t*>(a.out) + row * a.o_stride + static_cast<int64_t>(hd) * d + ch;
-            store4(to, all, [&](int e) { return inv * channel_gate(a, row, hd, ch + e); });
-        }
-    }
+    const int group = a.nq / a.nkv;
+    join_columns<MANY, false>(a, first, pieces, gridDim.x, blockIdx.x, blockIdx.z * 16, 16, it.x, it.y * group, blockIdx.x * group, group);
 }
 
 int check_matrix(const PulseAttn8* a, const char* what) {
@@ -731,17 +765,15 @@ int by_width(int d, F go) {
 
 }  // namespace
 
-extern "C" int64_t pulse_attn8_cut_ints(int n_items, int max_work) { return cache8::cut_ints(n_items, max_work); }
-
+// `groups`: the kv heads (and sixteens of their heads) that attn8_few has a counter of arrived pieces for; 0 for attn8_many.
 extern "C" int pulse_attn8_cut(const int* items, int n_items, const int* positions, int window, int chunk, int slots, int least,
-                               int max_work, int* cut, hipStream_t stream) {
-    PULSE_REQUIRE(items && positions && cut && n_items > 0 && slots > 0 && least > 0, "attn8_cut: bad work list");
-    PULSE_REQUIRE(max_work >= n_items && (max_work == n_items || max_work >= n_items + slots), "attn8_cut: room for %d pieces, %d are possible", max_work,
-                  n_items + slots);
+                               int max_work, int groups, int* cut, hipStream_t stream) {
+    PULSE_REQUIRE(items && positions && cut && n_items > 0 && slots > 0 && least > 0 && groups >= 0, "attn8_cut: bad work list");
+    PULSE_REQUIRE(max_work == n_items || max_work >= n_items + slots, "attn8_cut: room for %d pieces, %d are possible", max_work, n_items + slots);
     PULSE_REQUIRE((reinterpret_cast<uintptr_t>(items) & 15) == 0 && (reinterpret_cast<uintptr_t>(cut) & 15) == 0, "attn8_cut: lists must be aligned to 16 bytes");
     // (no room for more pieces than items: one each)
     attn8_cut_kernel<<<1, THREADS, 0, stream>>>(reinterpret_cast<const int4*>(items), n_items, positions, window, chunk, slots,
-                                                max_work == n_items ? 0x3fffffff : least, max_work, cut);
+                                                max_work == n_items ? 0x3fffffff : least, max_work, groups, cut);
     PULSE_LAUNCH_CHECK("attn8_cut");
     return 0;
 }
@@ -756,13 +788,6 @@ extern "C" int pulse_attn8_few(const PulseAttn8* a, hipStream_t stream) {
         else attn8_few_kernel<decltype(d)::value, false><<<grid, THREADS, 0, stream>>>(*a, blocks, head_groups);
     });
     PULSE_LAUNCH_CHECK("attn8_few");
-    if (a->max_work > a->n_items) {
-        // few items: a workgroup a column, so that many pieces are read by many; many: a workgroup for all of them
-        const int cols = a->nq / a->nkv > FEW ? FEW : FEW / (a->nq / a->nkv) * (a->nq / a->nkv);
-        const int each = static_cast<int64_t>(a->n_items) * a->nkv * head_groups * cols <= 4 * pulse_compute_units() ? 1 : cols;
-        attn8_join_kernel<FEW><<<dim3(a->nkv * head_groups, a->n_items, (cols + each - 1) / each), THREADS, 0, stream>>>(*a, head_groups, each);
-        PULSE_LAUNCH_CHECK("attn8_join");
-    }
     return 0;
 }
 
@@ -777,7 +802,7 @@ extern "C" int pulse_attn8_many(const PulseAttn8* a, hipStream_t stream) {
     });
     PULSE_LAUNCH_CHECK("attn8_many");
     if (a->max_work > a->n_items) {
-        attn8_join_kernel<MANY><<<dim3(a->nkv, a->n_items, MANY / 16), THREADS, 0, stream>>>(*a, 1, 16);
+        attn8_join_kernel<<<dim3(a->nkv, a->n_items, MANY / 16), THREADS, 0, stream>>>(*a);
         PULSE_LAUNCH_CHECK("attn8_join");
     }
     return 0;

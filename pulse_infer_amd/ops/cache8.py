@@ -228,7 +228,7 @@ class AttentionPlan:
         self.entries = len(entries)
         self.matrix = not plain and matrix_cores(d, page_size, dtype)
         self.device = torch.device(device)
-        self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, cut)
+        self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, counters an item, cut)
         self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces)
         if not self.matrix:
             self.calls.append(("pulse_attn8_plain", 0, 0, 0, 0, 0))
@@ -252,8 +252,9 @@ class AttentionPlan:
             room = n if whole else n + slots
             _need(room <= 65535, f"plan: {n} items are too many")
             on_gpu = to_device([v for _, row, rows, entry in items for v in (row, rows, entry, 0)])
-            cut = torch.empty(4 + 4 * room + 2 * n, dtype=torch.int32, device=self.device)
-            self.works.append((on_gpu, n, slots, least, room, cut))
+            counters = n * groups if columns == FEW else 0
+            cut = torch.empty(4 + 4 * room + 2 * n + counters, dtype=torch.int32, device=self.device)
+            self.works.append((on_gpu, n, slots, least, room, counters // n, cut))
             self.calls.append((name, on_gpu.data_ptr(), cut.data_ptr(), n, room, 0 if whole else room * groups * columns))
 
         add("pulse_attn8_few", FEW, few, nkv * ((group + FEW - 1) // FEW), self.FEW_SLOTS, self.FEW_LEAST, self.FEW_EVEN)
@@ -274,9 +275,9 @@ class AttentionPlan:
         """Shares the keys out for the rows' ``positions``: for every step, before its first ``attention``."""
         _here("plan", (positions,))
         _ints("plan", "positions", positions, self.rows)
-        for items, n, slots, least, room, cut in self.works:
+        for items, n, slots, least, room, groups, cut in self.works:
             call("pulse_attn8_cut", _ptr(items), _i32(n), _ptr(positions), _i32(self.window), _i32(self.chunk), _i32(slots), _i32(least),
-                 _i32(room), _ptr(cut), _stream())
+                 _i32(room), _i32(groups), _ptr(cut), _stream())
         return self
 
 
