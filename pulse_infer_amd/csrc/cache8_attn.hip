@@ -36,6 +36,13 @@ typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// A number that nothing in the launch writes; ONE: the same for the wavefront, read by the scalar unit.
+template <bool ONE, typename T>
+__device__ __forceinline__ T read_only(const T* p) {
+    if constexpr (ONE) return *reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(p));
+    return *p;
+}
+
 // Eight bytes times a power of two, as a matrix-core operand.
 __device__ __forceinline__ bf16x8 operand(uint32_t lo, uint32_t hi, float scale) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
@@ -505,31 +512,56 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     const Score score = score_of(a);
     const int* bt = a.table + static_cast<int64_t>(entry) * a.table_width;
 
+    // Piece n = tid + 256 i is of the tile's block n / D.  Where D is a multiple of 64 that is one block for a wavefront: its page, its
+    // scales and its address are then scalars (asked for by the scalar unit), and what is left of a lane's address never changes.  (A
+    // last turn that not all threads take brings the others a piece for nobody.)
+    constexpr bool ONE = D % 64 == 0;
+    struct Spot { int n, page_index, rest, page; };       // a block of the context: its number, its page's and its place in it, the page
     struct Raw {
         u32x4 k[TURNS], v[TURNS];
         float2 scale[TURNS];
         int there[TURNS];      // -1: beyond what the item sees, 0: not there, 1: there
     };
-    struct Pages { int p[TURNS]; };
-    // (piece n is of block n / D of the tile; a last turn that not all threads take brings the others a piece for nobody)
-    auto find = [&](int tile) __attribute__((always_inline)) {
-        Pages x;
+    Spot spot[TURNS];          // of the tile whose pages are asked for next
+    const int page_step = blocks.over(4), rest_step = 4 - page_step * blocks.b;
 #pragma unroll
-        for (int i = 0; i < TURNS; ++i) x.p[i] = bt[min(blocks.over(4 * tile + min((tid + i * THREADS) / D, 3)), a.table_width - 1)];
-        return x;
-    };
-    auto load = [&](int tile, const Pages& pages, Raw& x) __attribute__((always_inline)) {
+    for (int i = 0; i < TURNS; ++i) {
+        const int in_tile = min((tid + i * THREADS) / D, 3);
+        spot[i].n = 4 * tile_begin + (ONE ? uniform(in_tile) : in_tile);
+        spot[i].page_index = blocks.over(spot[i].n);
+        spot[i].rest = spot[i].n - spot[i].page_index * blocks.b;
+        spot[i].page = 0;
+    }
+    auto find = [&](Spot (&to)[TURNS]) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < TURNS; ++i) {
-            const int n = tid + i * THREADS, b = 4 * tile + min(n / D, 3), page = pages.p[i];
-            const bool ours = 16 * b <= hi && 16 * b + 15 >= lo;
-            const bool there = ours && page >= 0 && page < a.num_pages && blocks.over(b) < a.table_width;
+            Spot& s = spot[i];
+            to[i] = s;
+            to[i].page = read_only<ONE>(bt + min(s.page_index, a.table_width - 1));
+            if (s.page_index >= a.table_width) to[i].page = -1;
+            s.n += 4;
+            s.page_index += page_step;
+            s.rest += rest_step;
+            if (s.rest >= blocks.b) {
+                s.rest -= blocks.b;
+                ++s.page_index;
+            }
+        }
+    };
+    auto load = [&](const Spot (&from)[TURNS], Raw& x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            const Spot& s = from[i];
+            const bool ours = 16 * s.n <= hi && 16 * s.n + 15 >= lo;
+            const bool there = ours && s.page >= 0 && s.page < a.num_pages;
             x.there[i] = there ? 1 : ours ? 0 : -1;
-            const uint32_t at = there ? (static_cast<uint32_t>(page) * a.nkv + g) * blocks.b + blocks.rest(b) : 0u;
-            const uint64_t byte = static_cast<uint64_t>(at) * (16 * D) + n % D * 16;
-            x.k[i] = *reinterpret_cast<const u32x4*>(a.keys + byte);
-            x.v[i] = *reinterpret_cast<const u32x4*>(a.values + byte);
-            x.scale[i] = reinterpret_cast<const float2*>(a.scales)[at];
+            const uint32_t at = there ? (static_cast<uint32_t>(s.page) * a.nkv + g) * blocks.b + s.rest : 0u;
+            const uint64_t byte = static_cast<uint64_t>(at) * (16 * D);
+            const uint32_t mine = (tid + i * THREADS) % D * 16;
+            x.k[i] = *reinterpret_cast<const u32x4*>(a.keys + byte + mine);
+            x.v[i] = *reinterpret_cast<const u32x4*>(a.values + byte + mine);
+            const float* sc = a.scales + 2 * static_cast<uint64_t>(at);
+            x.scale[i] = make_float2(read_only<ONE>(sc), read_only<ONE>(sc + 1));
         }
     };
     auto put = [&](Raw& x, int stage, int tile) __attribute__((always_inline)) {
@@ -671,20 +703,21 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
 
     {
         Raw raw;
-        Pages pages = find(tile_begin);
+        Spot next[TURNS];
+        find(next);
         if (tid < 2) s_odd[tid] = 0;
         if (tid < 8) s_gone[tid / 4][tid % 4] = s_bad[tid / 4][tid % 4] = 0;
         __syncthreads();
-        load(tile_begin, pages, raw);
-        pages = find(tile_begin + 1);
+        load(next, raw);
+        find(next);
         put(raw, 0, tile_begin);
         __syncthreads();
         int stage = 0;
         for (int tile = tile_begin; tile < tile_end; ++tile, stage ^= 1) {
             const bool more = tile + 1 < tile_end;
             if (more) {
-                load(tile + 1, pages, raw);
-                pages = find(tile + 2);
+                load(next, raw);
+                find(next);
             }
             compute(tile, stage);
             if (more) put(raw, stage ^ 1, tile + 1);       // (that stage was read before the last barrier)
