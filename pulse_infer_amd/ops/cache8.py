@@ -35,9 +35,15 @@ def _refuse(what: str, why: str) -> None:
 # took longer than the kernels of a decoding step do.)
 def _here(what: str, tensors: Sequence[Optional[torch.Tensor]]) -> None:
     """All of them on the current GPU, whose stream the kernels are queued on."""
-    current = torch.cuda.current_device()
+    current = -1
     for t in tensors:
-        if t is not None and t.get_device() != current:
+        if t is None:
+            continue
+        index = t.get_device()
+        if current < 0:
+            _gpu(what, t)
+            current = torch.cuda.current_device()
+        if index != current:
             _gpu(what, t)
             _refuse(what, f"a tensor lies on {t.device}, the current GPU is cuda:{current}")
 
@@ -228,6 +234,7 @@ class AttentionPlan:
         self.entries = len(entries)
         self.matrix = not plain and matrix_cores(d, page_size, dtype)
         self.device = torch.device(device)
+        self.ready = not self.matrix      # whether the keys have been shared out
         self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, counters an item, cut)
         self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces)
         if not self.matrix:
@@ -275,6 +282,9 @@ class AttentionPlan:
         """Shares the keys out for the rows' ``positions``: for every step, before its first ``attention``."""
         _here("plan", (positions,))
         _ints("plan", "positions", positions, self.rows)
+        if self.device.index is not None and positions.device != self.device:
+            _refuse("plan", f"it was made for {self.device}, the positions lie on {positions.device}")
+        self.ready = True
         for items, n, slots, least, room, groups, cut in self.works:
             call("pulse_attn8_cut", _ptr(items), _i32(n), _ptr(positions), _i32(self.window), _i32(self.chunk), _i32(slots), _i32(least),
                  _i32(room), _i32(groups), _ptr(cut), _stream())
@@ -284,8 +294,10 @@ class AttentionPlan:
 def plan(entries: Sequence[Any], nq: int, nkv: int, d: int, positions: torch.Tensor, *, page_size: int, dtype: torch.dtype,
          window: int = 0, chunk: int = 0, workspace: Any = None, to_device: Optional[Callable] = None) -> AttentionPlan:
     """The attention of a step of ``entries`` (``EntryMeta``: start, count, first_row) whose rows stand at ``positions``, for layers of these
-    heads.  A step of the same shape takes the same plan, cut anew (``AttentionPlan.cut``); ``workspace`` holds the room for joined pieces
-    and serves the steps of one stream one after the other."""
+    heads.  It is made outside a recording; a step of the same shape takes the same plan, cut anew (``AttentionPlan.cut``, which may be
+    recorded).  A plan, its counters among it, serves the calls of one stream, one after the other.  ``workspace`` (a ``Workspace``):
+    where the room for joined pieces comes from, for the calls of one stream and not for two recordings at once; without one every
+    call takes it from torch's pool."""
     return AttentionPlan(entries, nq, nkv, d, page_size=page_size, dtype=dtype, window=window, chunk=chunk, device=positions.device,
                          workspace=workspace, to_device=to_device).cut(positions)
 
@@ -294,7 +306,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
               token_entry: torch.Tensor, table: torch.Tensor, scale: float, *, gate: Optional[torch.Tensor] = None, gate_width: int = 0,
               sink: Optional[torch.Tensor] = None, softcap: float = 0.0, workspace: Any = None) -> None:
     """Causal attention of a step's rows over a cache in 8 bits, as ``plan`` has it: ``q``, ``out`` [T, >= nq * d] of one storage type (bfloat16
-    or float32; rows may be strided), ``positions`` and ``token_entry`` int32 [T], ``table`` int32 [entries, width].
+    or float32; rows may be strided), ``positions`` (those that the plan was cut for) and ``token_entry`` int32 [T], ``table`` int32
+    [entries, width].
 
     A row sees the keys of its request from its window's (chunk's) first to its own position, in pages that are there: a table entry
     outside the pool hides its keys.  A row that sees none is zeros.  ``scale`` > 0; ``softcap``: scores become cap * tanh(score / cap);
@@ -316,6 +329,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
         _refuse(what, "rows that overlap")
     if plan.rows > tokens:
         _refuse(what, f"the plan has {plan.rows} rows, q {tokens}")
+    if not plan.ready:
+        _refuse(what, "the plan has not been cut for any positions")
     if not scale > 0.0 or not softcap >= 0.0:
         _refuse(what, "the scale must be positive and the cap not negative")
     _ints(what, "positions", positions, tokens)
@@ -350,6 +365,6 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
             part_o, part_ml = o.data_ptr(), ml.data_ptr()
         call(name, _ATTN.pack(
             q_at, q_stride, out_at, o_stride, view.keys.data_ptr(), view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(),
-            token_entry.data_ptr(), table.data_ptr(), _at(gate), gate_stride, _at(sink), items, cut, part_o, part_ml, plan.tag, tokens,
+            token_entry.data_ptr(), table.data_ptr(), _at(gate), gate_stride, _at(sink), items, cut, part_o, part_ml, plan.tag, plan.rows,
             table.shape[0], table.shape[1], nq, nkv, d, page, pages, plan.window, plan.chunk, gate_width, n_items, room, scale, softcap),
             _stream())

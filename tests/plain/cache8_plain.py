@@ -156,24 +156,25 @@ def attention(q, cache, entries, table, scale, window=0, chunk=0, softcap=0.0, s
         pages = [int(p) for p in table[b][:held]]
         there = torch.tensor([0 <= p < num_pages for p in pages]).repeat_interleave(cache.page)
         keys, values = cache.rows([p if 0 <= p < num_pages else 0 for p in pages])
-        j = torch.arange(held * cache.page)
-        for i in range(c):
-            pos = s + i
-            lo = pos - pos % chunk if chunk else max(0, pos - window + 1) if window else 0
-            seen = ((j >= lo) & (j <= pos) & there).nonzero()[:, 0]
-            for h in range(nq):
-                if not seen.numel():
-                    continue
-                kk, vv = keys[h * nkv // nq][seen], values[h * nkv // nq][seen]
-                x = kk @ q[row + i, h] * scale
-                size[row + i, h] = (kk.abs() @ q[row + i, h].abs()).max() * scale
-                if softcap:
-                    x = softcap * torch.tanh(x / softcap)
-                if sink is not None:
-                    x = torch.cat([x, sink[h:h + 1].cpu().to(F64)])
-                p = torch.softmax(x, 0)[:seen.numel()]
-                out[row + i, h] = p @ vv
-                mass[row + i, h] = p @ vv.abs()
+        j, pos = torch.arange(held * cache.page), torch.arange(s, s + c)[:, None]
+        lo = pos - pos % chunk if chunk else (pos - window + 1).clamp_min(0) if window else torch.zeros_like(pos)
+        seen = (j >= lo) & (j <= pos) & there
+        hides = seen[:, :, None]
+        for h in range(nq if c else 0):
+            kk, vv = keys[h * nkv // nq], values[h * nkv // nq]
+            # (what is not finite counts where it is seen alone)
+            x = torch.where(seen, q[row:row + c, h] @ torch.nan_to_num(kk).T * scale, torch.full((), -math.inf, dtype=F64))
+            x = torch.where(seen & torch.isnan(kk).any(-1), torch.full((), math.nan, dtype=F64), x)
+            size[row:row + c, h, 0] = torch.where(seen, q[row:row + c, h].abs() @ torch.nan_to_num(kk).abs().T, torch.zeros((), dtype=F64)).amax(-1) * scale
+            if softcap:
+                x = torch.where(seen, softcap * torch.tanh(x / softcap), x)
+            if sink is not None:
+                x = torch.cat([x, sink[h].cpu().to(F64).expand(c, 1)], 1)
+            p = torch.where(seen.any(-1, keepdim=True), torch.softmax(x, -1)[:, :j.numel()], torch.zeros((), dtype=F64))
+            out[row:row + c, h] = p @ torch.nan_to_num(vv)
+            mass[row:row + c, h] = p @ torch.nan_to_num(vv).abs()
+            spoilt = (hides & torch.isnan(vv)[None]).any(1) if torch.isnan(vv).any() else torch.zeros((c, d), dtype=torch.bool)
+            out[row:row + c, h][spoilt] = math.nan
         row += c
     if gate is not None:
         g = torch.sigmoid(gate.cpu().to(F64))

@@ -313,6 +313,28 @@ def test_attention_long_axis_is_joined(dtype):
     attend([(2500, 40), (0, 90), (700, 1)], 2, 1, 32, 16, dtype, seed=8, window=900)
 
 
+@pytest.mark.parametrize("entries,nq,nkv", [([(i * 7 % 300, 1) for i in range(70)], 16, 8), ([(0, 512)], 128, 32), ([(5, 600), (0, 40)], 64, 16)])
+def test_attention_of_items_that_fill_the_gpu(entries, nq, nkv):
+    """Many items: nothing is cut; with a window most of a long walk falls away."""
+    attend(entries, nq, nkv, 32, 16, seed=20)
+    attend(entries, nq, nkv, 32, 16, seed=21, window=70, sink=True)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_drawn(seed):
+    """Sizes, layouts and masks drawn over the range, odd ones among them."""
+    import random
+
+    r = random.Random(seed)
+    nq, nkv = r.choice([(4, 4), (6, 2), (7, 1), (12, 4), (20, 4), (18, 1), (5, 5)])
+    long = lambda most: int(math.exp(r.uniform(0, math.log(most))))  # noqa: E731
+    entries = [(long(1500) - 1, 1 if r.random() < 0.6 else long(200)) for _ in range(r.randint(1, 9))]
+    window, chunk = r.choice([(0, 0), (0, 0), (long(700), 0), (0, long(300))])
+    attend(entries, nq, nkv, r.choice([32, 40, 64, 96, 128, 192]), r.choice([4, 16, 16, 32, 48]), r.choice([torch.bfloat16] * 3 + [torch.float32]),
+           seed=100 + seed, window=window, chunk=chunk, softcap=r.choice([0.0, 0.0, 8.0]), sink=r.random() < 0.4,
+           gate=r.choice([None, None, 0, 16]), pad=r.choice([0, 8]), extra_rows=r.choice([0, 2]))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("sink", [False, True])
 def test_attention_rows_that_see_nothing(dtype, sink):
@@ -504,6 +526,8 @@ def test_refusals():
     bad(go, view=Paged8CacheView(0, view.keys[:, :1], view.values, view.scales, 16))
     bad(go, view=Paged8CacheView(0, view.keys.view(torch.uint8), view.values, view.scales, 16))
     bad(go, view=Paged8CacheView(0, view.keys, view.values[:3], view.scales, 16))
+    uncut = cache8.AttentionPlan(e, 4, 2, 32, page_size=16, dtype=torch.bfloat16)
+    bad(cache8.attention, q, q.clone(), uncut, view, pos, ent, table, 1.0)
     bad(cache8.plan, e, 4, 3, 32, pos, page_size=16, dtype=torch.bfloat16)
     bad(cache8.plan, e, 4, 2, 600, pos, page_size=16, dtype=torch.bfloat16)
     bad(cache8.plan, e, 4, 2, 32, pos, page_size=16, dtype=torch.bfloat16, window=3, chunk=4)
