@@ -34,8 +34,13 @@ __device__ __forceinline__ int low_key(int window, int chunk, int pos) {
 __device__ __forceinline__ float tanh_of(float x) { return 1.f - 2.f / (__expf(2.f * x) + 1.f); }
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + __expf(-x)); }
 
-// Where a cut says what it found: the number of pieces, then the pieces (item, first tile, end, the item's first piece), then for every
-// item its first piece and how many it has, then attn8_few's counters of arrived pieces.
-constexpr int CUT_HEAD = 4;
+// What a cut is: for every workgroup a piece (no rows: nothing to do), for every item its first piece and how many it has, then
+// attn8_few's counters of arrived pieces.
+struct Piece {
+    int row0, rows, entry, item;              // the item
+    int tile, tile_end, first, pieces;        // its stretch of tiles; the item's first piece and how many there are
+    int hi, pos0, unused[2];                  // the positions of the item's last and first row
+};
+constexpr int PIECE_INTS = sizeof(Piece) / 4;
 
 }  // namespace cache8

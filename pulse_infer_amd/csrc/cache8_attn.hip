@@ -7,8 +7,8 @@
 // 64 keys.  Everything is kept transposed, so that a column stays in its lanes:
 //   S^T[key, col] = K[key, :] . q[col, :]      P^T = exp2(S^T c - m[col])      O^T[ch, col] += V^T[ch, key] P^T[key, col]
 //
-// attn8_cut      shares the tiles of all items out over a number of pieces: T = the least length for which sum ceil(tiles / T) fits, an
-//                item in equal pieces of at most T.  Made on the device from the positions, once a step for all layers, so that a
+// attn8_cut      shares the tiles of all items out over a number of pieces: T = the least length for which sum ceil(tiles / T) fits (by
+//                bisection), an item in equal pieces of at most T.  Made on the device from the positions, once a step for all layers, so that a
 //                recorded step's replays bring their own lengths.
 // attn8_few      up to 16 columns an item (a decoded token's heads; a few tokens).  Its four wavefronts take every fourth tile and
 //                meet at the end.  Bound by reading the cache.
@@ -93,37 +93,72 @@ __device__ __forceinline__ void store4(bf16_t* to, f32x4 x, F factor) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------ the cut
+__device__ __forceinline__ cache8::Piece piece_of(const PulseAttn8& a, int w) {
+    cache8::Piece x;
+    const int* from = a.cut + w * cache8::PIECE_INTS;
+    int* to = &x.row0;
+#pragma unroll
+    for (int i = 0; i < 10; ++i) to[i] = read_only<true>(from + i);
+    return x;
+}
+
 __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restrict__ items, int n, const int* __restrict__ positions,
                                                             int window, int chunk, int slots, int least, int max_work, int groups, int* cut) {
-    __shared__ int s_wave[WAVES];
+    __shared__ int s_sum[WAVES], s_max[WAVES];
     const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = tid / PULSE_WAVE;
-    auto tiles = [&](int i, int& first) {
+    cache8::Piece* work = reinterpret_cast<cache8::Piece*>(cut);
+    int2* info = reinterpret_cast<int2*>(cut + cache8::PIECE_INTS * max_work);
+    int* arrived = cut + cache8::PIECE_INTS * max_work + 2 * n;
+    auto walk = [&](int i) {
         const int4 it = items[i];
-        const int hi = positions[it.x + it.y - 1], lo = cache8::low_key(window, chunk, positions[it.x]);
-        first = lo / TILE;
-        return max(hi / TILE + 1 - first, 1);
+        const int hi = positions[it.x + it.y - 1], pos0 = positions[it.x], first = cache8::low_key(window, chunk, pos0) / TILE;
+        return cache8::Piece{it.x, it.y, it.z, i, first, first + max(hi / TILE + 1 - first, 1), 0, 0, hi, pos0, {0, 0}};
     };
-    int mine = 0, unused;
-    for (int i = tid; i < n; i += THREADS) mine += tiles(i, unused);
-    mine = wave_sum(mine);
-    if (lane == 0) s_wave[wave] = mine;
-    __syncthreads();
-    int total = 0;
+    // over all threads
+    auto both = [&](int& sum, int& most) {
+        sum = wave_sum(sum);
+        most = wave_reduce(most, [](int x, int y) { return max(x, y); });
+        __syncthreads();
+        if (lane == 0) s_sum[wave] = sum, s_max[wave] = most;
+        __syncthreads();
+        sum = most = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) total += s_wave[w];
-    const int length = max(least, (total + slots - 1) / slots);
-    int4* work = reinterpret_cast<int4*>(cut + cache8::CUT_HEAD);
-    int2* info = reinterpret_cast<int2*>(cut + cache8::CUT_HEAD + 4 * max_work);
-    int* arrived = cut + cache8::CUT_HEAD + 4 * max_work + 2 * n;
-    for (int i = tid; i < n * groups; i += THREADS) arrived[i] = 0;
+        for (int w = 0; w < WAVES; ++w) sum += s_sum[w], most = max(most, s_max[w]);
+    };
+    // (a thread's first item's tiles are kept: with up to 256 items the search reads nothing)
+    cache8::Piece mine = {};
+    if (tid < n) mine = walk(tid);
+    auto tiles = [&](int i) {
+        if (i == tid) return mine.tile_end - mine.tile;
+        const cache8::Piece x = walk(i);
+        return x.tile_end - x.tile;
+    };
+    int total = 0, most = 0;
+    for (int i = tid; i < n; i += THREADS) {
+        const int t = tiles(i);
+        total += t;
+        most = max(most, t);
+    }
+    both(total, most);
+    // the least length for which the pieces are no more than the slots (where the items are more than that: nothing is cut)
+    int lo = max(least, (total + slots - 1) / slots), hi = max(lo, most);
+    if (max_work == n) lo = hi;
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        int pieces = 0, unused = 0;
+        for (int i = tid; i < n; i += THREADS) pieces += (tiles(i) + mid - 1) / mid;
+        both(pieces, unused);
+        if (pieces <= slots) hi = mid;
+        else lo = mid + 1;
+    }
     int before = 0;
     for (int base = 0; base < n; base += THREADS) {
         const int i = base + tid;
-        int first = 0, count = 0, pieces = 0, each = 1;
+        cache8::Piece x = i == tid ? mine : i < n ? walk(i) : cache8::Piece{};
+        const int count = x.tile_end - x.tile;
+        int pieces = 0, each = 1;
         if (i < n) {
-            count = tiles(i, first);
-            pieces = (count + length - 1) / length;
-            each = (count + pieces - 1) / pieces;
+            each = (count + (count + lo - 1) / lo - 1) / ((count + lo - 1) / lo);
             pieces = (count + each - 1) / each;
         }
         int sum = pieces;
@@ -133,22 +168,29 @@ __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restri
             sum += lane >= step ? other : 0;
         }
         __syncthreads();
-        if (lane == PULSE_WAVE - 1) s_wave[wave] = sum;
+        if (lane == PULSE_WAVE - 1) s_sum[wave] = sum;
         __syncthreads();
         int at = before + sum - pieces, all = 0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            at += w < wave ? s_wave[w] : 0;
-            all += s_wave[w];
+            at += w < wave ? s_sum[w] : 0;
+            all += s_sum[w];
         }
         before += all;
         if (i < n) {
             info[i] = make_int2(at, pieces);
-            for (int z = 0; z < pieces && at + z < max_work; ++z)
-                work[at + z] = make_int4(i, first + z * each, min(first + count, first + (z + 1) * each), at);
+            const int end = x.tile_end;
+            x.first = at;
+            x.pieces = pieces;
+            for (int z = 0; z < pieces && at + z < max_work; ++z) {
+                x.tile_end = min(end, x.tile + each);
+                work[at + z] = x;
+                x.tile += each;
+            }
         }
     }
-    if (tid == 0) cut[0] = min(before, max_work);
+    for (int w = before + tid; w < max_work; w += THREADS) work[w] = cache8::Piece{};
+    for (int i = tid; i < n * groups; i += THREADS) arrived[i] = 0;
 }
 
 // Two numbers to and from memory that workgroups of one launch share: past the caches that belong to one die (relaxed atomics of the
@@ -164,14 +206,15 @@ __device__ __forceinline__ float2 shared2(const float* from) {
     return make_float2(__uint_as_float(static_cast<uint32_t>(both)), __uint_as_float(static_cast<uint32_t>(both >> 32)));
 }
 
-// The join: out = sum_z w_z o_z / sum_z w_z l_z, w_z = exp2(m_z - max m), over an item's pieces in their order (pieces of one column are
-// COLS columns and the launch's `heads_x` apart).  A thread takes four channels of one of the columns c0 .. c0 + each - 1 and, where the
-// threads are more than that, every ZS-th piece; their sums meet in LDS.  SHARED: the pieces are this launch's.
+// The join: out = sum_z w_z o_z / sum_z w_z l_z, w_z = exp2(m_z - max m), over an item's pieces (pieces of one column are COLS columns
+// and the launch's `heads_x` apart).  A thread takes four channels of one of the columns c0 .. c0 + each - 1 and, where the threads are
+// more than that, every ZS-th piece, eight at a time under a running maximum: one trip to memory for eight; the threads' sums meet in LDS.
+// The order is fixed by the sizes alone.  SHARED: the pieces are this launch's.
 template <int COLS, bool SHARED>
 __device__ __forceinline__ void join_columns(const PulseAttn8& a, int first, int pieces, int heads_x, int x, int c0, int each, int row0, int cols,
                                              int head0, int heads) {
     __shared__ f32x4 s_sum[THREADS];
-    __shared__ float s_den[THREADS];
+    __shared__ float2 s_ml[THREADS];
     const int tid = threadIdx.x, d = a.d, quads = d / 4, units = each * quads, zs = max(1, THREADS / units);
     const int64_t step = static_cast<int64_t>(heads_x) * COLS, at0 = static_cast<int64_t>(first) * step + static_cast<int64_t>(x) * COLS;
     for (int u0 = 0; u0 < units; u0 += THREADS) {
@@ -181,29 +224,32 @@ __device__ __forceinline__ void join_columns(const PulseAttn8& a, int first, int
         const int64_t at = at0 + (on ? c : c0);
         float m = -INFINITY, l = 0.f;
         f32x4 all = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int z = 0; z < pieces; ++z) m = fmaxf(m, shared2<SHARED>(a.part_ml + 2 * (at + z * step)).x);
-        const float ref = m == -INFINITY ? 0.f : m;
-        if (on) {
-#pragma unroll 8
-            for (int z = z0; z < pieces; z += zs) {
-                const float2 ml = shared2<SHARED>(a.part_ml + 2 * (at + z * step));
-                const float* from = a.part_o + (at + z * step) * d + ch;
-                const float2 lo = shared2<SHARED>(from), hi = shared2<SHARED>(from + 2);
-                const f32x4 o = {lo.x, lo.y, hi.x, hi.y};
-                const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-                l += ml.y * f;
-                all += o * f;
+        auto add = [&](float pm, float pl, f32x4 po) __attribute__((always_inline)) {     // (nothing yet: all is zeros, or NaN to be kept)
+            const float now = fmaxf(m, pm), ref = now == -INFINITY ? 0.f : now;
+            const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(pm - ref);
+            l = l * f + pl * g;
+            all = all * f + po * g;
+            m = now;
+        };
+        constexpr int BATCH = 8;
+        for (int z = z0; z < pieces && on; z += BATCH * zs) {
+            float2 ml[BATCH], lo[BATCH], hi[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int64_t piece = at + min(z + i * zs, pieces - 1) * step;       // (past the last: the last again, for nobody)
+                ml[i] = shared2<SHARED>(a.part_ml + 2 * piece);
+                lo[i] = shared2<SHARED>(a.part_o + piece * d + ch);
+                hi[i] = shared2<SHARED>(a.part_o + piece * d + ch + 2);
             }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i)
+                if (z + i * zs < pieces) add(ml[i].x, ml[i].y, f32x4{lo[i].x, lo[i].y, hi[i].x, hi[i].y});
         }
         if (zs > 1) {
             s_sum[tid] = all;
-            s_den[tid] = l;
+            s_ml[tid] = make_float2(m, l);
             __syncthreads();
-            for (int z = 1; z < zs && z0 == 0 && unit < units; ++z) {
-                all += s_sum[unit + z * units];
-                l += s_den[unit + z * units];
-            }
+            for (int z = 1; z < zs && z0 == 0 && on; ++z) add(s_ml[unit + z * units].x, s_ml[unit + z * units].y, s_sum[unit + z * units]);
         }
         if (on && z0 == 0) {
             const int row = row0 + c / heads, hd = head0 + c % heads;
@@ -235,18 +281,14 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
     __shared__ float s_o[WAVES][FEW][D + 4];
     __shared__ float s_m[WAVES][FEW], s_l[WAVES][FEW];
     const int w = blockIdx.y;
-    if (w >= uniform(a.cut[0])) return;
-    const int4 job = reinterpret_cast<const int4*>(a.cut + cache8::CUT_HEAD)[w];
-    const int item = uniform(job.x), tile_end = uniform(job.z), first_piece = uniform(job.w);
-    const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::CUT_HEAD + 4 * a.max_work)[item];
-    const bool whole = uniform(info.y) == 1;
-    const int4 it = reinterpret_cast<const int4*>(a.items)[item];
-    const int row0 = uniform(it.x), ntok = uniform(it.y), entry = uniform(it.z);
+    const cache8::Piece job = piece_of(a, w);
+    if (job.rows <= 0) return;
+    const int row0 = job.row0, ntok = job.rows, entry = job.entry, tile_end = job.tile_end;
+    const bool whole = job.pieces == 1;
     const int g = blockIdx.x / head_groups, part = blockIdx.x % head_groups;
     const int group = a.nq / a.nkv, heads = min(group - part * FEW, FEW);
     const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = uniform(tid / PULSE_WAVE);
-    const int r = lane % 16, b = lane / 16;
-    const int hi = uniform(a.positions[row0 + ntok - 1]), pos0 = uniform(a.positions[row0]);
+    const int r = lane % 16, b = lane / 16, hi = job.hi, pos0 = job.pos0;
     const int lo = cache8::low_key(a.window, a.chunk, pos0), lo_last = cache8::low_key(a.window, a.chunk, hi);
 
     // this lane's column: token r / heads, head r % heads
@@ -390,7 +432,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
         }
     };
 
-    int tile = uniform(job.y) + wave;
+    int tile = job.tile + wave;
     if (tile < tile_end) {
         F now, next;
         load(tile, find(tile), now);
@@ -448,15 +490,15 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
     // next launch.  (By a release and an acquire, which write a die's cache back for every piece, 24 requests took 82 us for 42.)
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     __shared__ int s_last;
-    int* arrived = const_cast<int*>(a.cut) + cache8::CUT_HEAD + 4 * a.max_work + 2 * a.n_items + item * gridDim.x + blockIdx.x;
+    int* arrived = const_cast<int*>(a.cut) + cache8::PIECE_INTS * a.max_work + 2 * a.n_items + job.item * gridDim.x + blockIdx.x;
     __syncthreads();
     if (tid == 0) {
         const int before = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = before == info.y - 1;
+        s_last = before == job.pieces - 1;
         if (s_last) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (s_last) join_columns<FEW, true>(a, first_piece, uniform(info.y), gridDim.x, blockIdx.x, 0, ntok * heads, row0, ntok * heads, g * group + part * FEW, heads);
+    if (s_last) join_columns<FEW, true>(a, job.first, job.pieces, gridDim.x, blockIdx.x, 0, ntok * heads, row0, ntok * heads, g * group + part * FEW, heads);
 }
 
 // ------------------------------------------------------------------------------------------------------------ 128 columns
@@ -479,17 +521,13 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     __shared__ int s_odd[2], s_gone[2][4], s_bad[2][4];
     __shared__ __attribute__((aligned(8))) uint16_t s_none[2][D][4];
     const int w = blockIdx.y;
-    if (w >= uniform(a.cut[0])) return;
-    const int4 job = reinterpret_cast<const int4*>(a.cut + cache8::CUT_HEAD)[w];
-    const int item = uniform(job.x), tile_begin = uniform(job.y), tile_end = uniform(job.z);
-    const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::CUT_HEAD + 4 * a.max_work)[item];
-    const bool whole = uniform(info.y) == 1;
-    const int4 it = reinterpret_cast<const int4*>(a.items)[item];
-    const int row0 = uniform(it.x), ntok = uniform(it.y), entry = uniform(it.z);
+    const cache8::Piece job = piece_of(a, w);
+    if (job.rows <= 0) return;
+    const int row0 = job.row0, ntok = job.rows, entry = job.entry, tile_begin = job.tile, tile_end = job.tile_end;
+    const bool whole = job.pieces == 1;
     const int g = blockIdx.x, group = a.nq / a.nkv;
     const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = uniform(tid / PULSE_WAVE);
-    const int r = lane % 32, half = lane / 32;
-    const int hi = uniform(a.positions[row0 + ntok - 1]), pos0 = uniform(a.positions[row0]);
+    const int r = lane % 32, half = lane / 32, hi = job.hi, pos0 = job.pos0;
     const int lo = cache8::low_key(a.window, a.chunk, pos0);
 
     const int col = wave * 32 + r, tok = col / group;
@@ -761,7 +799,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
 // but 128 columns of a head take longer than that for one workgroup).
 __global__ __launch_bounds__(THREADS) void attn8_join_kernel(PulseAttn8 a) {
     const int item = blockIdx.y;
-    const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::CUT_HEAD + 4 * a.max_work)[item];
+    const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::PIECE_INTS * a.max_work)[item];
     const int first = uniform(info.x), pieces = uniform(info.y);
     if (pieces <= 1) return;
     const int4 it = reinterpret_cast<const int4*>(a.items)[item];
@@ -806,7 +844,7 @@ extern "C" int pulse_attn8_cut(const int* items, int n_items, const int* positio
     PULSE_REQUIRE((reinterpret_cast<uintptr_t>(items) & 15) == 0 && (reinterpret_cast<uintptr_t>(cut) & 15) == 0, "attn8_cut: lists must be aligned to 16 bytes");
     // (no room for more pieces than items: one each)
     attn8_cut_kernel<<<1, THREADS, 0, stream>>>(reinterpret_cast<const int4*>(items), n_items, positions, window, chunk, slots,
-                                                max_work == n_items ? 0x3fffffff : least, max_work, groups, cut);
+                                                least, max_work, groups, cut);
     PULSE_LAUNCH_CHECK("attn8_cut");
     return 0;
 }

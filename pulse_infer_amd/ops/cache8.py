@@ -23,6 +23,7 @@ from .library import KernelError, call
 
 MAX_REQUESTS = 4096          # of step_maps
 MAX_HEAD_DIM = 512           # of store and of attention
+PIECE_INTS = 12              # of a piece of work (csrc/cache8_attn.h)
 TILE = 64                    # keys of a step of the matrix-core kernels
 FEW, MANY = 16, 128          # columns (rows times the heads that share a kv head) of an item of the two matrix-core kernels
 
@@ -213,9 +214,10 @@ class AttentionPlan:
     alone (how many tokens each request brings); the second is made on the GPU from the positions, by ``cut``, once a step for all
     layers that are alike in heads, window and chunk.  ``plain``: everything goes to the kernel that serves every size."""
 
-    # Workgroups a compute unit that a kernel's keys are shared out over, and the fewest tiles of 64 keys of a piece.
-    FEW_SLOTS, FEW_LEAST = 4, 8
-    MANY_SLOTS, MANY_LEAST = 2, 8
+    # Workgroups a compute unit that a kernel's keys are shared out over, the fewest tiles of 64 keys of a piece, and how many times the
+    # items there may be pieces in any case.
+    FEW_SLOTS, FEW_LEAST, FEW_ROUNDS = 2, 8, 2
+    MANY_SLOTS, MANY_LEAST, MANY_ROUNDS = 2, 8, 1
     # Nothing is cut (and nothing joined) where the items fill the GPU by themselves, two workgroups a unit, and the longest is at most
     # that many times what a unit's share of them would be.
     FEW_EVEN, MANY_EVEN = 1.15, 2.2
@@ -249,28 +251,29 @@ class AttentionPlan:
         units = compute_units()
         to_device = to_device or (lambda flat: torch.tensor(flat, dtype=torch.int32, device=self.device))
 
-        def add(name: str, columns: int, items: List[Tuple], groups: int, slots: float, least: int, even: float) -> None:
+        def add(name: str, columns: int, items: List[Tuple], groups: int, slots: float, least: int, rounds: int, even: float) -> None:
             n = len(items)
             if not n:
                 return
             tiles = [(last + rows - 1) // TILE + 1 - self._low(last) // TILE for last, _, rows, _ in items]
             whole = n * groups >= 2 * units and max(tiles) * 2 * units <= even * sum(tiles) * groups
-            slots = max(1, int(slots * units) // groups)
+            slots = max(1, int(slots * units) // groups, rounds * n)
             room = n if whole else n + slots
             _need(room <= 65535, f"plan: {n} items are too many")
             on_gpu = to_device([v for _, row, rows, entry in items for v in (row, rows, entry, 0)])
             counters = n * groups if columns == FEW else 0
-            cut = torch.empty(4 + 4 * room + 2 * n + counters, dtype=torch.int32, device=self.device)
+            cut = torch.empty(PIECE_INTS * room + 2 * n + counters, dtype=torch.int32, device=self.device)
             self.works.append((on_gpu, n, slots, least, room, counters // n, cut))
             self.calls.append((name, on_gpu.data_ptr(), cut.data_ptr(), n, room, 0 if whole else room * groups * columns))
 
-        add("pulse_attn8_few", FEW, few, nkv * ((group + FEW - 1) // FEW), self.FEW_SLOTS, self.FEW_LEAST, self.FEW_EVEN)
+        add("pulse_attn8_few", FEW, few, nkv * ((group + FEW - 1) // FEW), self.FEW_SLOTS, self.FEW_LEAST,
+            self.FEW_ROUNDS, self.FEW_EVEN)
         # The longest walks first; where two workgroups share a unit, the second ones' from the other end, the shortest beside the longest.
         many.sort(key=lambda it: -it[0])
         first = max(1, units // nkv)
         if first < len(many) <= 2 * first:
             many[first:] = many[:first - 1:-1]
-        add("pulse_attn8_many", MANY, many, nkv, self.MANY_SLOTS, self.MANY_LEAST, self.MANY_EVEN)
+        add("pulse_attn8_many", MANY, many, nkv, self.MANY_SLOTS, self.MANY_LEAST, self.MANY_ROUNDS, self.MANY_EVEN)
 
     def _low(self, position: int) -> int:
         """The lowest key that a token at ``position`` sees."""
