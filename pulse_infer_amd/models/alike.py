@@ -21,7 +21,7 @@ from typing import Any, List, Optional, Tuple
 
 import torch
 
-from ..cache.specs import PagedCacheView
+from ..cache.specs import Paged8CacheView, PagedCacheView
 from ..ops import library, timing
 from ..parts import linear
 from ..parts.attention import PagedAttention
@@ -79,7 +79,7 @@ class AlikeRuns:
     def _plain(self, index: int) -> bool:
         run = self.order[index]
         block = self.blocks[run.layer]
-        return (type(self.views[index]) is PagedCacheView and run.offset is None and run.rejoin is None
+        return (type(self.views[index]) in (PagedCacheView, Paged8CacheView) and run.offset is None and run.rejoin is None
                 and type(block) is PreNormBlock and type(block.mixer) is PagedAttention and type(block.ffn) is GatedMLP
                 and type(block.mixer_norm) is RMSNorm and type(block.ffn_norm) is RMSNorm)
 
@@ -87,8 +87,8 @@ class AlikeRuns:
         """What must be equal for a run to be alike, and its tensors."""
         block, view = self.blocks[self.order[index].layer], self.views[index]
         numbers = tuple(len(vars(part)) for part in (block, *self._parts_of(block)))      # (an attribute that the first has not)
-        return ((self._plain_of(block), numbers, view.group, view.page_size, view.writable),
-                self._tensors_of(block) + (view.keys, view.values))
+        kept = (view.keys, view.values) + ((view.scales,) if type(view) is Paged8CacheView else ())
+        return (self._plain_of(block), numbers, view.group, view.page_size, view.writable), self._tensors_of(block) + kept
 
     def _alike(self, first: Tuple, index: int) -> bool:
         try:
@@ -172,11 +172,24 @@ class AlikeRuns:
         for (lib, name, fn, a_args, clean), (lib_b, name_b, fn_b, b_args, clean_b) in zip(*records):
             if lib is not lib_b or name != name_b or len(a_args) != len(b_args) or not (clean and clean_b):
                 return None
-            own = []
-            for a, b in zip(a_args, b_args):
+            own, b_args = [], list(b_args)
+            for place, (a, b) in enumerate(zip(a_args, b_args)):
                 if type(a) is not type(b):
                     return None
                 if a is None:
+                    continue
+                if isinstance(a, bytes):       # a structure's fields, put together: a copy of it that the words of pointers can be put into
+                    if len(a) != len(b) or len(b) % 8:
+                        return None
+                    b_args[place] = held = ctypes.create_string_buffer(b, len(b))
+                    for i in range(0, len(a), 8):
+                        x, y = (int.from_bytes(part[i:i + 8], "little") for part in (a, b))
+                        if x in at:
+                            if y != second[at[x]]:
+                                return None
+                            own.append((ctypes.c_uint64.from_buffer(held, i), at[x]))
+                        elif x != y or inside(x):
+                            return None
                     continue
                 if isinstance(a, ctypes._SimpleCData):
                     if isinstance(a, ctypes.c_void_p) and a.value in at:

@@ -148,3 +148,26 @@ def test_refusals(model_folders, tmp_path):
     folder = write_model_folder(TipidraConfig.from_dict(next(iter(CONFIGS.values()))), str(tmp_path / "t"), seed=1)
     with pytest.raises(ValueError, match="in 8 bits"):
         LLM.from_pretrained(folder, cache_dtype="float8_e4m3")
+
+
+@pytest.mark.parametrize("changed", [False, True])
+def test_alike_layers_are_launched_from_one_record(monkeypatch, changed):
+    """The bits of the same steps through the layers' parts; a layer that is not alike goes through its own."""
+    require_gpu()
+    from pulse_infer_amd.config import Qwen3Config
+    from pulse_infer_amd.models.causal_lm import expected_tensors
+    from pulse_infer_amd.models.factory import build_model
+    from pulse_infer_amd.weights.random_init import RandomSource
+
+    from test_gpu_alike_runs import FEW_ROWS, SIZES, counted
+
+    cfg = Qwen3Config.from_dict(SIZES)
+    model = build_model(cfg, RandomSource(expected_tensors(cfg.model_spec()), seed=3), mode="bfloat16",
+                        options={"cache_dtype": "float8_e4m3"})
+    if changed:
+        model.blocks[6].mixer.scale *= 2.0
+    recorded, few = counted(monkeypatch, model, True, FEW_ROWS)
+    through, many = counted(monkeypatch, model, False, FEW_ROWS)
+    assert few < (0.9 if changed else 0.6) * many
+    for a, b in zip(recorded, through):
+        assert torch.equal(a, b)
