@@ -221,7 +221,10 @@ class AttentionPlan:
     # Nothing is cut (and nothing joined) where the items fill the GPU by themselves, two workgroups a unit, and the longest is at most
     # that many times what a unit's share of them would be.
     FEW_EVEN, MANY_EVEN = 1.15, 2.2
-    FEW_COLUMNS = 32     # up to which a portion goes through attn8_few
+    # Portions go through attn8_few up to so many columns, and altogether while they walk no more tiles a compute unit for it.  One portion
+    # of 128 rows, 32 heads on 8, many / few, us: from the start 18.1 / 14.4, behind 1,000 tokens 22.9 / 19.0, behind 8,000 41 / 55; of
+    # 40 behind 8,000 28.9 / 28.2; sixteen of 23 behind 1,000 27.7 / 23.6, of 64 39 / 49.
+    FEW_COLUMNS, FEW_WALKS = 32, 48
 
     def __init__(self, entries: Sequence[Any], nq: int, nkv: int, d: int, *, page_size: int, dtype: torch.dtype, window: int = 0,
                  chunk: int = 0, device: Any = "cuda", workspace: Any = None, to_device: Optional[Callable] = None, plain: bool = False):
@@ -242,20 +245,22 @@ class AttentionPlan:
         if not self.matrix:
             self.calls.append(("pulse_attn8_plain", 0, 0, 0, 0, 0))
             return
-        group = nq // nkv
+        units, group = compute_units(), nq // nkv
         few, many = [], []
-        each, wide = max(1, FEW // group), MANY // group
+        each, wide, groups = max(1, FEW // group), MANY // group, nkv * ((group + FEW - 1) // FEW)
+        # every 16 columns of attn8_few walk the keys for themselves
+        walks = sum(-(-e.count // each) * (self._tiles(e.start, e.count)) for e in entries if e.count * group > self.FEW_COLUMNS) * groups
+        narrow = wide == 0 or walks <= self.FEW_WALKS * units
         for i, e in enumerate(entries):
-            to, step = (few, each) if e.count * group <= self.FEW_COLUMNS or wide == 0 else (many, wide)
+            to, step = (few, each) if narrow or e.count * group <= self.FEW_COLUMNS else (many, wide)
             to += [(e.start + at, e.first_row + at, min(step, e.count - at), i) for at in range(0, e.count, step)]
-        units = compute_units()
         to_device = to_device or (lambda flat: torch.tensor(flat, dtype=torch.int32, device=self.device))
 
         def add(name: str, columns: int, items: List[Tuple], groups: int, slots: float, least: int, rounds: int, even: float) -> None:
             n = len(items)
             if not n:
                 return
-            tiles = [(last + rows - 1) // TILE + 1 - self._low(last) // TILE for last, _, rows, _ in items]
+            tiles = [self._tiles(start, rows) for start, _, rows, _ in items]
             whole = n * groups >= 2 * units and max(tiles) * 2 * units <= even * sum(tiles) * groups
             slots = max(1, int(slots * units) // groups, rounds * n)
             room = n if whole else n + slots
@@ -266,7 +271,7 @@ class AttentionPlan:
             self.works.append((on_gpu, n, slots, least, room, counters // n, cut))
             self.calls.append((name, on_gpu.data_ptr(), cut.data_ptr(), n, room, 0 if whole else room * groups * columns))
 
-        add("pulse_attn8_few", FEW, few, nkv * ((group + FEW - 1) // FEW), self.FEW_SLOTS, self.FEW_LEAST,
+        add("pulse_attn8_few", FEW, few, groups, self.FEW_SLOTS, self.FEW_LEAST,
             self.FEW_ROUNDS, self.FEW_EVEN)
         # The longest walks first; where two workgroups share a unit, the second ones' from the other end, the shortest beside the longest.
         many.sort(key=lambda it: -it[0])
@@ -275,11 +280,10 @@ class AttentionPlan:
             many[first:] = many[:first - 1:-1]
         add("pulse_attn8_many", MANY, many, nkv, self.MANY_SLOTS, self.MANY_LEAST, self.MANY_ROUNDS, self.MANY_EVEN)
 
-    def _low(self, position: int) -> int:
-        """The lowest key that a token at ``position`` sees."""
-        if self.chunk:
-            return position - position % self.chunk
-        return max(0, position - self.window + 1) if self.window else 0
+    def _tiles(self, start: int, count: int) -> int:
+        """Tiles that hold keys of ``count`` tokens from position ``start`` on."""
+        low = start - start % self.chunk if self.chunk else max(0, start - self.window + 1) if self.window else 0
+        return (start + count - 1) // TILE + 1 - low // TILE
 
     def cut(self, positions: torch.Tensor) -> "AttentionPlan":
         """Shares the keys out for the rows' ``positions``: for every step, before its first ``attention``."""
