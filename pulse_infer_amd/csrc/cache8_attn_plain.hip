@@ -4,7 +4,7 @@
 //   s_j = scale * q . k_j, capped: cap * tanh(s_j / cap);  seen: low <= j <= position, in pages that are there
 //   o = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink - m)), one pass with the running maximum m and sum
 //
-// A lane takes a key's score (its row of bytes in pieces of 16) and then channels of the sum, for which the weights go from lane to lane.
+// A lane takes a key's score (its row of bytes in pieces of 16) and then channels of the sum, for which the weights come as scalars.
 // A row that sees no key is zeros; a row of no entry (token_entry outside the table) is left as it is.  Keys and values that a row does
 // not see are not multiplied, so that what is not finite stays with those who see it.
 // It serves what the matrix-core kernels do not: float32 rows, heads that are no multiple of 32 channels, pages that are no multiple
@@ -15,21 +15,16 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / PULSE_WAVE, MAX_DIM = 512;
 
-// 16 bytes from their place, whatever its alignment
-template <bool WHOLE>
-__device__ __forceinline__ uint4 piece(const uint8_t* p, int stride) {
-    if constexpr (WHOLE) return *reinterpret_cast<const uint4*>(p);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = p[(4 * i) * stride] | (p[(4 * i + 1) * stride] << 8) | (p[(4 * i + 2) * stride] << 16) | (static_cast<uint32_t>(p[(4 * i + 3) * stride]) << 24);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
+__device__ __forceinline__ float of_lane(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
 
-// CH: channels a lane sums.  WHOLE: blocks of 16 tokens and heads of a multiple of 16 channels.
-template <typename T, int CH, bool WHOLE>
+// 0xff in the bytes whose bit is set
+__device__ __forceinline__ uint32_t spread(uint32_t bits) { return ((bits * 0x00204081u) & 0x01010101u) * 0xffu; }
+
+// CH: channels a lane sums.  WIDE: heads of a multiple of 16 channels, a key's row in pieces of 16 bytes.  VQ: tokens of a channel that are
+// read together: 16 (blocks of 16), 4 (blocks of a multiple of 4) or 1.
+template <typename T, int CH, bool WIDE, int VQ>
 __global__ __launch_bounds__(THREADS) void attn8_plain_kernel(PulseAttn8 a) {
-    __shared__ float s_q[MAX_DIM];
+    __shared__ __attribute__((aligned(16))) float s_q[MAX_DIM];
     __shared__ float s_o[WAVES][MAX_DIM];
     __shared__ float s_m[WAVES], s_l[WAVES];
     const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = tid / PULSE_WAVE;
@@ -52,27 +47,34 @@ __global__ __launch_bounds__(THREADS) void attn8_plain_kernel(PulseAttn8 a) {
         const int pi = j / a.page_size;
         const int page = pi < a.table_width ? bt[pi] : -1;
         const bool seen = j >= lo && j <= pos && page >= 0 && page < a.num_pages;
-        const int64_t head = static_cast<int64_t>(seen ? page : 0) * a.nkv + g;
+        const uint64_t seen_keys = __ballot(seen);
+        if (seen_keys == 0) continue;
         const int slot = seen ? j - pi * a.page_size : 0;
+        // the key's number in the cache, and its block's
+        const int64_t head = static_cast<int64_t>(seen ? page : 0) * a.nkv + g;
         const int64_t bn = head * nb + slot / block;
+        const float ks = a.scales[2 * bn], vs = a.scales[2 * bn + 1];
         float s = 0.f;
         const uint8_t* k = a.keys + (head * a.page_size + slot) * d;
-        if (WHOLE) {
+        if constexpr (WIDE) {
             for (int c = 0; c < d; c += 16) {
-                const uint4 u = piece<true>(k + c, 1);
+                const uint4 u = *reinterpret_cast<const uint4*>(k + c);
                 const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float x[4];
                     cache8::from_e4m3x4(w[i], x);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s += x[e] * s_q[c + 4 * i + e];
+                    const float4 y = *reinterpret_cast<const float4*>(&s_q[c + 4 * i]);
+                    s += x[0] * y.x;
+                    s += x[1] * y.y;
+                    s += x[2] * y.z;
+                    s += x[3] * y.w;
                 }
             }
         } else {
             for (int c = 0; c < d; ++c) s += cache8::from_e4m3(k[c]) * s_q[c];
         }
-        s *= a.scales[2 * bn] * a.scale;
+        s *= ks * a.scale;
         if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
         s = seen ? s : -INFINITY;
         const float top = fmaxf(m, wave_max(s));
@@ -83,43 +85,42 @@ __global__ __launch_bounds__(THREADS) void attn8_plain_kernel(PulseAttn8 a) {
         m = top;
 #pragma unroll
         for (int i = 0; i < CH; ++i) acc[i] *= again;
-        const uint64_t seen_keys = __ballot(seen);
-        const float pv = seen ? p * fabsf(a.scales[2 * bn + 1]) : 0.f;
-        if constexpr (WHOLE) {
+        const float pv = seen ? p * fabsf(vs) : 0.f;
+        // (VQ keys from a multiple of VQ on are of one block: the first that is seen says where it lies)
+        const uint32_t place_lo = static_cast<uint32_t>(bn), place_hi = static_cast<uint32_t>(bn >> 32);
+        const int in_block = slot % block;
+        for (int b = 0; b < PULSE_WAVE; b += VQ) {
+            const uint32_t some = static_cast<uint32_t>(seen_keys >> b) & ((1u << VQ) - 1u);
+            if (!some) continue;
+            const int one = b + __builtin_ctz(some);
+            const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(place_hi, one))) << 32 |
+                                                    static_cast<uint32_t>(__builtin_amdgcn_readlane(place_lo, one)));
+            const uint8_t* v = a.values + at * block * d + (__builtin_amdgcn_readlane(in_block, one) - (one - b));
+            float w[VQ];
 #pragma unroll
-            for (int b = 0; b < PULSE_WAVE / 16; ++b) {
-                const uint32_t some = static_cast<uint32_t>(seen_keys >> (16 * b)) & 0xffffu;
-                if (!some) continue;
-                // (a block's keys lie in one page: the first that is seen says where)
-                const int64_t at = __shfl(head, 16 * b + __builtin_ctz(some));
-                const int inner = __shfl(slot, 16 * b + __builtin_ctz(some)) / 16;
-                const uint8_t* v = a.values + (at * a.page_size + inner * 16) * d;
+            for (int e = 0; e < VQ; ++e) w[e] = of_lane(pv, b + e);
 #pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const int c = lane + i * PULSE_WAVE;
-                    const uint4 u = piece<true>(v + (c < d ? c : 0) * 16, 1);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x[4];
-                        cache8::from_e4m3x4(w[e], x);
-#pragma unroll
-                        for (int f = 0; f < 4; ++f)
-                            if (some >> (4 * e + f) & 1) acc[i] += __shfl(pv, 16 * b + 4 * e + f) * x[f];
+            for (int i = 0; i < CH; ++i) {
+                const int c = lane + i * PULSE_WAVE;
+                const uint8_t* from = v + static_cast<int64_t>(c < d ? c : 0) * block;
+                if constexpr (VQ == 1) {
+                    acc[i] += w[0] * cache8::from_e4m3(*from);
+                } else {
+                    uint32_t bytes[VQ / 4];
+                    if constexpr (VQ == 16) {
+                        const uint4 u = *reinterpret_cast<const uint4*>(from);
+                        bytes[0] = u.x, bytes[1] = u.y, bytes[2] = u.z, bytes[3] = u.w;
+                    } else {
+                        bytes[0] = *reinterpret_cast<const uint32_t*>(from);
                     }
-                }
-            }
-        } else {
-            for (uint64_t left = seen_keys; left; left &= left - 1) {
-                const int n = __builtin_ctzll(left);
-                const int64_t at = __shfl(head, n);
-                const int sl = __shfl(slot, n);
-                const float w = __shfl(pv, n);
-                const uint8_t* v = a.values + (at * a.page_size + sl / block * block) * d + sl % block;
 #pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const int c = lane + i * PULSE_WAVE;
-                    if (c < d) acc[i] += w * cache8::from_e4m3(v[static_cast<int64_t>(c) * block]);
+                    for (int e = 0; e < VQ / 4; ++e) {
+                        float x[4];
+                        // what is not seen is not multiplied: its bytes are zeros (a block that is seen whole keeps its own)
+                        cache8::from_e4m3x4(bytes[e] & spread(some >> (4 * e) & 15u), x);
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) acc[i] += w[4 * e + f] * x[f];
+                    }
                 }
             }
         }
@@ -173,18 +174,23 @@ extern "C" int pulse_attn8_plain(const PulseAttn8* a, hipStream_t stream) {
     PULSE_REQUIRE(a->d <= MAX_DIM, "attn8_plain: heads of %d channels (up to %d)", a->d, MAX_DIM);
     PULSE_REQUIRE(a->nq <= 65535, "attn8_plain: too many heads");
     if (a->tokens == 0) return 0;
-    const bool whole = a->page_size % cache8::BLOCK == 0 && a->d % 16 == 0;
-    auto go = [&](auto t, auto ch, auto w) {
-        attn8_plain_kernel<decltype(t), decltype(ch)::value, decltype(w)::value><<<dim3(a->tokens, a->nq), THREADS, 0, stream>>>(*a);
+    const int block = cache8::block_tokens(a->page_size);
+    auto go = [&](auto t, auto ch, auto wide, auto vq) {
+        attn8_plain_kernel<decltype(t), decltype(ch)::value, decltype(wide)::value, decltype(vq)::value><<<dim3(a->tokens, a->nq), THREADS, 0, stream>>>(*a);
     };
-    auto by_width = [&](auto t, auto w) {
-        if (a->d <= 64) go(t, std::integral_constant<int, 1>(), w);
-        else if (a->d <= 128) go(t, std::integral_constant<int, 2>(), w);
-        else if (a->d <= 256) go(t, std::integral_constant<int, 4>(), w);
-        else go(t, std::integral_constant<int, 8>(), w);
+    auto by_block = [&](auto t, auto ch, auto wide) {
+        if (block == 16) go(t, ch, wide, std::integral_constant<int, 16>());
+        else if (block % 4 == 0) go(t, ch, wide, std::integral_constant<int, 4>());
+        else go(t, ch, wide, std::integral_constant<int, 1>());
+    };
+    auto by_width = [&](auto t, auto wide) {
+        if (a->d <= 64) by_block(t, std::integral_constant<int, 1>(), wide);
+        else if (a->d <= 128) by_block(t, std::integral_constant<int, 2>(), wide);
+        else if (a->d <= 256) by_block(t, std::integral_constant<int, 4>(), wide);
+        else by_block(t, std::integral_constant<int, 8>(), wide);
     };
     auto by_form = [&](auto t) {
-        if (whole) by_width(t, std::true_type());
+        if (a->d % 16 == 0) by_width(t, std::true_type());
         else by_width(t, std::false_type());
     };
     if (a->dtype == PULSE_F32) by_form(float());

@@ -57,9 +57,10 @@ def _ints(what: str, name: str, t: torch.Tensor, n: int) -> None:
 def _pages(what: str, view: Paged8CacheView, nkv: int, d: int) -> Tuple[int, int]:
     """(pages, tokens a page) of a cache that is what the kernels take it for."""
     keys, values, scales, page = view.keys, view.values, view.scales, view.page_size
-    block = block_tokens(page)
-    pages = keys.shape[0]
-    if keys.shape != (pages, nkv, page, d) or values.shape != (pages, nkv, page // block, d, block) or scales.shape != (pages, nkv, page // block, 2):
+    block = 16 if page % 16 == 0 else page      # (block_tokens)
+    shape = keys.shape
+    pages = shape[0]
+    if shape != (pages, nkv, page, d) or values.shape != (pages, nkv, page // block, d, block) or scales.shape != (pages, nkv, page // block, 2):
         _refuse(what, f"the cache is {tuple(keys.shape)}, {tuple(values.shape)}, {tuple(scales.shape)}, expected {(pages, nkv, page, d)}, "
                       f"{(pages, nkv, page // block, d, block)}, {(pages, nkv, page // block, 2)}")
     if keys.dtype != torch.float8_e4m3fn or values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
@@ -80,9 +81,10 @@ def _at(t: Optional[torch.Tensor]) -> int:
 
 
 def _block_list(what: str, blocks: torch.Tensor) -> int:
-    if blocks.dtype != torch.int32 or blocks.dim() != 2 or blocks.shape[1] != 4 or not blocks.is_contiguous() or blocks.data_ptr() % 16:
+    shape = blocks.shape
+    if blocks.dtype != torch.int32 or len(shape) != 2 or shape[1] != 4 or not blocks.is_contiguous() or blocks.data_ptr() % 16:
         _refuse(what, "blocks must be contiguous int32 [n, 4], aligned to 16 bytes")
-    return blocks.shape[0]
+    return shape[0]
 
 
 # ------------------------------------------------------------------------------------------------------------- the maps
@@ -126,9 +128,10 @@ def step_maps(start: torch.Tensor, count: torch.Tensor, *, page_size: int, num_p
         _ints(what, "pages", pages, 1)
         listed = pages.numel()
     if table is not None:
-        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] != n or table.shape[1] < 1:
+        shape = table.shape
+        if table.dtype != torch.int32 or len(shape) != 2 or not table.is_contiguous() or shape[0] != n or shape[1] < 1:
             _refuse(what, f"the table must be contiguous int32 [{n}, width]")
-        width = table.shape[1]
+        width = shape[1]
     if pages is None and table is None and not (slots is None and blocks is None):
         _refuse(what, "slots and blocks need the pages or the table")
     if blocks is not None:
@@ -165,10 +168,11 @@ def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, vie
     pages, page = _pages(what, view, nkv, d)
     v_head0 = nq + nkv if v_head0 is None else int(v_head0)
     columns = max(nq + nkv, v_head0 + nkv) * d
-    if qkv.dim() != 2 or v_head0 < 0 or qkv.shape[1] < columns or qkv.stride(1) != 1:
+    shape, to = qkv.shape, q_out.shape
+    if len(shape) != 2 or v_head0 < 0 or shape[1] < columns or qkv.stride(1) != 1:
         _refuse(what, f"qkv must be [T, {columns}] with contiguous rows")
-    tokens = qkv.shape[0]
-    if q_out.dim() != 2 or q_out.shape[0] != tokens or q_out.shape[1] < nq * d or q_out.stride(1) != 1 or q_out.dtype != qkv.dtype:
+    tokens = shape[0]
+    if len(to) != 2 or to[0] != tokens or to[1] < nq * d or q_out.stride(1) != 1 or q_out.dtype != qkv.dtype:
         _refuse(what, f"q_out must be [{tokens}, {nq * d}] of qkv's storage type with contiguous rows")
     stride, q_stride = qkv.stride(0), q_out.stride(0)
     if tokens > 1 and (stride < columns or q_stride < nq * d):
@@ -189,9 +193,10 @@ def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, vie
         rotated = rotary_dim
         if rotary_dim % 2 or not 0 < rotary_dim <= d or pairing not in (0, 1):
             _refuse(what, f"bad rotation of {rotary_dim} channels")
-        for t in (cos, sin):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[0] < tokens or t.shape[1] != rotary_dim // 2 or not t.is_contiguous():
-                _refuse(what, f"cos/sin must be float32 [T, {rotary_dim // 2}]")
+        shape = cos.shape
+        if (shape != sin.shape or len(shape) != 2 or shape[0] < tokens or shape[1] != rotary_dim // 2 or cos.dtype != torch.float32
+                or sin.dtype != torch.float32 or not cos.is_contiguous() or not sin.is_contiguous()):
+            _refuse(what, f"cos/sin must be float32 [T, {rotary_dim // 2}]")
     coef, every = 0.0, 0
     if q_temperature is not None:
         coef, every = float(q_temperature[0]), int(q_temperature[1])
@@ -327,10 +332,11 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     pages, page = _pages(what, view, nkv, d)
     if page != plan.page_size or q.dtype != plan.dtype:
         _refuse(what, f"the plan is for pages of {plan.page_size} and {plan.dtype}")
-    if (q.dim() != 2 or out.dim() != 2 or q.dtype != out.dtype or q.shape[0] != out.shape[0] or q.shape[1] < nq * d or out.shape[1] < nq * d
+    shape, to = q.shape, out.shape
+    if (len(shape) != 2 or len(to) != 2 or q.dtype != out.dtype or shape[0] != to[0] or shape[1] < nq * d or to[1] < nq * d
             or q.stride(1) != 1 or out.stride(1) != 1):
         _refuse(what, f"q and out must be [T, {nq * d}] of one storage type with contiguous rows")
-    tokens = q.shape[0]
+    tokens = shape[0]
     q_stride, o_stride = (q.stride(0), out.stride(0)) if tokens > 1 else (nq * d, nq * d)
     if q_stride < nq * d or o_stride < nq * d:
         _refuse(what, "rows that overlap")
@@ -342,7 +348,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
         _refuse(what, "the scale must be positive and the cap not negative")
     _ints(what, "positions", positions, tokens)
     _ints(what, "token_entry", token_entry, tokens)
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.numel() == 0 or table.shape[0] < plan.entries:
+    shape = table.shape
+    if table.dtype != torch.int32 or len(shape) != 2 or not table.is_contiguous() or shape[0] < max(1, plan.entries) or shape[1] < 1:
         _refuse(what, f"the table must be contiguous int32 [{plan.entries}, width]")
     gate_stride = 0
     if gate is None:
@@ -373,5 +380,5 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
         call(name, _ATTN.pack(
             q_at, q_stride, out_at, o_stride, view.keys.data_ptr(), view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(),
             token_entry.data_ptr(), table.data_ptr(), _at(gate), gate_stride, _at(sink), items, cut, part_o, part_ml, plan.tag, plan.rows,
-            table.shape[0], table.shape[1], nq, nkv, d, page, pages, plan.window, plan.chunk, gate_width, n_items, room, scale, softcap),
+            shape[0], shape[1], nq, nkv, d, page, pages, plan.window, plan.chunk, gate_width, n_items, room, scale, softcap),
             _stream())
