@@ -102,6 +102,11 @@ __device__ __forceinline__ cache8::Piece piece_of(const PulseAttn8& a, int w) {
     return x;
 }
 
+// Where a piece's tiles end: at the table's end at the latest, however far on the positions are.
+__device__ __forceinline__ int tiles_end(const PulseAttn8& a, const cache8::Piece& job, const cache8::Div& blocks) {
+    return static_cast<int>(min(static_cast<int64_t>(job.tile_end), (static_cast<int64_t>(a.table_width) * blocks.b + 3) / 4));
+}
+
 __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restrict__ items, int n, const int* __restrict__ positions,
                                                             int window, int chunk, int slots, int least, int max_work, int groups, int* cut) {
     __shared__ int s_sum[WAVES], s_max[WAVES];
@@ -109,10 +114,12 @@ __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restri
     cache8::Piece* work = reinterpret_cast<cache8::Piece*>(cut);
     int2* info = reinterpret_cast<int2*>(cut + cache8::PIECE_INTS * max_work);
     int* arrived = cut + cache8::PIECE_INTS * max_work + 2 * n;
+    const int at_most = 0x7fffffff / n;       // (so that no sum leaves 32 bits, whatever the positions are: 2 million tokens for 65,535 items)
     auto walk = [&](int i) {
         const int4 it = items[i];
         const int hi = positions[it.x + it.y - 1], pos0 = positions[it.x], first = cache8::low_key(window, chunk, pos0) / TILE;
-        return cache8::Piece{it.x, it.y, it.z, i, first, first + max(hi / TILE + 1 - first, 1), 0, 0, hi, pos0, {0, 0}};
+        const int count = min(max(hi / TILE + 1 - first, 1), at_most);
+        return cache8::Piece{it.x, it.y, it.z, i, first, first + count, 0, 0, hi, pos0, {0, 0}};
     };
     // over all threads
     auto both = [&](int& sum, int& most) {
@@ -283,7 +290,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
     const int w = blockIdx.y;
     const cache8::Piece job = piece_of(a, w);
     if (job.rows <= 0) return;
-    const int row0 = job.row0, ntok = job.rows, entry = job.entry, tile_end = job.tile_end;
+    const int row0 = job.row0, ntok = job.rows, entry = job.entry, tile_end = tiles_end(a, job, blocks);
     const bool whole = job.pieces == 1;
     const int g = blockIdx.x / head_groups, part = blockIdx.x % head_groups;
     const int group = a.nq / a.nkv, heads = min(group - part * FEW, FEW);
@@ -402,7 +409,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
                 l += e;
                 p[t / 2][4 * (t % 2) + i] = static_cast<__bf16>(e);
             }
-        const float vs = fabsf(x.vs);
+        const float vs = x.there ? fabsf(x.vs) : 1.f;       // (in the place of a block that is not there one was read that nobody need have written)
         if (__builtin_expect(__any(x.there && x.vs < 0.f), 0)) {
             asm volatile("");
             // Values that are not finite belong to those who see them alone: they are left out of the sums, and a column that sees one
@@ -523,7 +530,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     const int w = blockIdx.y;
     const cache8::Piece job = piece_of(a, w);
     if (job.rows <= 0) return;
-    const int row0 = job.row0, ntok = job.rows, entry = job.entry, tile_begin = job.tile, tile_end = job.tile_end;
+    const int row0 = job.row0, ntok = job.rows, entry = job.entry, tile_begin = job.tile, tile_end = tiles_end(a, job, blocks);
     const bool whole = job.pieces == 1;
     const int g = blockIdx.x, group = a.nq / a.nkv;
     const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = uniform(tid / PULSE_WAVE);
@@ -610,7 +617,10 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
                 const int kr = n / (D / 16), kc = n % (D / 16), vb = n / D, vc = n % D;
                 if (__builtin_expect(x.there[i] <= 0 || x.scale[i].y < 0.f, 0)) {
                     asm volatile("");
-                    if (x.there[i] <= 0) x.k[i] = x.v[i] = u32x4{0u, 0u, 0u, 0u};
+                    if (x.there[i] <= 0) {       // (what was read in its place nobody need have written)
+                        x.k[i] = x.v[i] = u32x4{0u, 0u, 0u, 0u};
+                        x.scale[i] = make_float2(1.f, 1.f);
+                    }
                     if (x.there[i] >= 0) s_odd[stage] = tile + 1;       // (every thread that writes it writes the same)
                     if (x.there[i] == 0) s_gone[stage][vb] = tile + 1;
                     if (x.there[i] > 0) {

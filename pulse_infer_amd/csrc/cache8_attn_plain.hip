@@ -30,13 +30,15 @@ __global__ __launch_bounds__(THREADS) void attn8_plain_kernel(PulseAttn8 a) {
     const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = tid / PULSE_WAVE;
     const int entry = a.token_entry[row];
     if (entry < 0 || entry >= a.entries) return;
-    const int pos = a.positions[row];
+    // (no key lies behind the table, and no position so far on that the next one leaves 32 bits)
+    const int pos = static_cast<int>(min(static_cast<int64_t>(a.positions[row]),
+                                         min(static_cast<int64_t>(a.table_width) * a.page_size, static_cast<int64_t>(0x7fffffff - 2 * THREADS)) - 1));
     const int g = h / (a.nq / a.nkv), d = a.d;
     const T* q = static_cast<const T*>(a.q) + row * a.q_stride + static_cast<int64_t>(h) * d;
     for (int c = tid; c < MAX_DIM; c += THREADS) s_q[c] = c < d ? to_f32<T>(q[c]) : 0.f;
     __syncthreads();
     const int block = cache8::block_tokens(a.page_size), nb = a.page_size / block;
-    const int lo = cache8::low_key(a.window, a.chunk, pos);
+    const int lo = cache8::low_key(a.window, a.chunk, a.positions[row]);
     const int* bt = a.table + static_cast<int64_t>(entry) * a.table_width;
     float m = -INFINITY, l = 0.f, acc[CH];
 #pragma unroll

@@ -103,8 +103,8 @@ __global__ __launch_bounds__(THREADS) void step_maps_kernel(MapArgs a) {
         int p = -1;
         if (a.pages) {
             const int at = page0[b] + j;
-            if (at < min(page0[b + 1], a.n_pages)) p = a.pages[at];
-        } else if (j < a.width) {
+            if (at >= 0 && at < min(page0[b + 1], a.n_pages)) p = a.pages[at];
+        } else if (j >= 0 && j < a.width) {
             p = a.table[static_cast<int64_t>(b) * a.width + j];
         }
         return p;

@@ -210,7 +210,9 @@ __device__ __forceinline__ bool job_of(const StoreArgs& a, const int4* work, uin
     const int4 w = work[blockIdx.x / a.nkv];
     j.g = blockIdx.x % a.nkv;
     j.first = w.x, j.rows = w.y, j.at = w.w;
-    if (w.y <= 0 || w.z < 0 || w.z >= a.all_blocks || w.w < 0 || w.w + w.y > a.block || w.x < 0 || w.x + w.y > a.tokens) return false;
+    if (w.y <= 0 || w.z < 0 || w.z >= a.all_blocks || w.w < 0 || w.w >= a.block || w.y > a.block - w.w || w.x < 0 || w.y > a.tokens ||
+        w.x > a.tokens - w.y)
+        return false;
     const int64_t page = w.z / a.blocks_per_page, head = page * a.nkv + j.g;
     const int inner = w.z - static_cast<int>(page) * a.blocks_per_page;
     j.keys = keys + (head * a.page_size + static_cast<int64_t>(inner) * a.block) * a.d;

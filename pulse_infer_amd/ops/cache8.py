@@ -240,8 +240,11 @@ class AttentionPlan:
         self.nq, self.nkv, self.d, self.page_size, self.dtype = nq, nkv, d, int(page_size), dtype
         self.window, self.chunk, self.workspace = int(window), int(chunk), workspace
         self.tag = _TAG[dtype]
-        self.rows = max((e.first_row + e.count for e in entries), default=0)
-        self.entries = len(entries)
+        self.rows, self.entries = 0, len(entries)
+        for e in entries:
+            if e.first_row != self.rows or e.count < 0 or e.start < 0:
+                _refuse("plan", f"an entry of {e.count} rows from position {e.start} on, at row {e.first_row}: expected the next, row {self.rows}")
+            self.rows += e.count
         self.matrix = not plain and matrix_cores(d, page_size, dtype)
         self.device = torch.device(device)
         self.ready = not self.matrix      # whether the keys have been shared out
@@ -305,8 +308,8 @@ class AttentionPlan:
 
 def plan(entries: Sequence[Any], nq: int, nkv: int, d: int, positions: torch.Tensor, *, page_size: int, dtype: torch.dtype,
          window: int = 0, chunk: int = 0, workspace: Any = None, to_device: Optional[Callable] = None) -> AttentionPlan:
-    """The attention of a step of ``entries`` (``EntryMeta``: start, count, first_row) whose rows stand at ``positions``, for layers of these
-    heads.  It is made outside a recording; a step of the same shape takes the same plan, cut anew (``AttentionPlan.cut``, which may be
+    """The attention of a step of ``entries`` (``EntryMeta``: start, count, first_row; one's rows behind the other's from row 0 on, at
+    positions that follow each other) whose rows stand at ``positions``, for layers of these heads.  It is made outside a recording; a step of the same shape takes the same plan, cut anew (``AttentionPlan.cut``, which may be
     recorded).  A plan, its counters among it, serves the calls of one stream, one after the other.  ``workspace`` (a ``Workspace``):
     where the room for joined pieces comes from, for the calls of one stream and not for two recordings at once; without one every
     call takes it from torch's pool."""
@@ -330,6 +333,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     _here(what, (q, out, view.keys, view.values, view.scales, positions, token_entry, table, gate, sink))
     nq, nkv, d = plan.nq, plan.nkv, plan.d
     pages, page = _pages(what, view, nkv, d)
+    if plan.device.index is not None and plan.device.index != q.get_device():
+        _refuse(what, f"the plan was made for {plan.device}, q lies on {q.device}")
     if page != plan.page_size or q.dtype != plan.dtype:
         _refuse(what, f"the plan is for pages of {plan.page_size} and {plan.dtype}")
     shape, to = q.shape, out.shape

@@ -96,6 +96,14 @@ def test_refusals_without_a_gpu():
         cache8.AttentionPlan(metas([(0, 1)] * 70000), 4, 2, 32, page_size=16, dtype=torch.bfloat16, device="cpu")
 
 
+@pytest.mark.parametrize("entries", [[(0, 3, 1)], [(0, 3, 0), (5, 2, 2)], [(0, 3, 0), (5, 2, 4)], [(-1, 2, 0)], [(0, 2, 0), (0, -1, 2)]])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_that_do_not_follow_each_other_are_refused(entries, dtype):
+    step = [EntryMeta(i, i, start, count, row) for i, (start, count, row) in enumerate(entries)]
+    with pytest.raises(KernelError, match="expected the next"):
+        cache8.AttentionPlan(step, 4, 2, 32, page_size=16, dtype=dtype, device="cpu")
+
+
 def test_options():
     from pulse_infer_amd.cli import build_parser
     from pulse_infer_amd.models.causal_lm import CausalLM

@@ -98,6 +98,17 @@ def test_maps_of_pages_that_are_none():
     assert -1 in want["slots"]
 
 
+def test_maps_of_lengths_whose_pages_leave_32_bits():
+    """Four requests of 2^30 + 1 pages of one token each, and a list of three pages: all but the first two of the first's are none."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    slots, blocks, table = ints([5] * 4), torch.zeros((4, 4), dtype=torch.int32, device=DEV), ints([[7, 7]] * 4)
+    cache8.step_maps(ints([1 << 30] * 4), ints([1] * 4), page_size=1, num_pages=4, pages=ints([3, 1, 2]), table=table, slots=slots, blocks=blocks)
+    assert slots.tolist() == [-1] * 4 and blocks.tolist() == [[i, 1, -1, 0] for i in range(4)]
+    assert table.tolist() == [[3, 1], [-1, -1], [-1, -1], [-1, -1]]
+
+
 # --------------------------------------------------------------------------------------------------------------- store
 STORE = [   # nq, nkv, d, page, dtype, norm, rotary, pairing, entries
     (4, 2, 128, 16, torch.bfloat16, True, 128, 1, [(0, 40), (15, 1), (16, 1), (33, 20)]),
@@ -214,14 +225,21 @@ def test_store_leaves_other_blocks_alone():
     view = view_of(cache)
     before = [t.clone() for t in (view.keys.view(torch.uint8), view.values.view(torch.uint8), view.scales)]
     x = torch.randn((4, 96), device=DEV)
-    cache8.store(x, torch.empty((4, 32), device=DEV), 1, 1, 32, view, ints([0] * 4), ints([[0, 4, -1, 0], [0, 0, 1, 0], [0, 4, 2, 0], [0, 4, 1, 13], [2, 3, 1, 0]]))
+    cache8.store(x, torch.empty((4, 32), device=DEV), 1, 1, 32, view, ints([0] * 4), ints([[0, 4, -1, 0], [0, 0, 1, 0], [0, 4, 2, 0], [0, 4, 1, 13], [2, 3, 1, 0],
+                                                                                             [2 ** 31 - 2, 4, 1, 0], [0, 4, 1, 2 ** 31 - 2], [0, 2 ** 31 - 1, 1, 1]]))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(before, (view.keys.view(torch.uint8), view.values.view(torch.uint8), view.scales)))
 
 
 # ----------------------------------------------------------------------------------------------------------- attention
+def bound_of(dtype, d, want, mass, size):
+    if dtype == torch.float32:
+        return (2 * 2.0 ** -24 * (d + 2) * size + 1e-6) * mass + 2.0 ** -24 * want.abs()
+    return 2.0 ** -8 * (mass + want.abs()) + (1e-5 + 2.0 ** -22 * size) * mass
+
+
 def attend(entries, nq, nkv, d, page, dtype=torch.bfloat16, seed=0, window=0, chunk=0, softcap=0.0, sink=False, gate=None, none=(), pad=0,
-           spoil=None, extra_rows=0):
+           spoil=None, extra_rows=0, unwritten=None):
     """Kernel and plain on one random cache; asserts the bound and returns (got, want)."""
     require_gpu()
     from pulse_infer_amd.ops import cache8
@@ -229,6 +247,8 @@ def attend(entries, nq, nkv, d, page, dtype=torch.bfloat16, seed=0, window=0, ch
 
     g = torch.Generator().manual_seed(seed + d + nq)
     pages, pool, rows = layout(entries, page, seed)
+    if unwritten is not None:      # nobody has the first page, nor the last ones
+        pool, rows = pool + 1, [[p + 1 for p in r] for r in rows]
     total = sum(c for _, c in entries)
     cache = plain.Cache(pool, nkv, page, d)
     k, v = (torch.randn((pool * page, nkv, d), generator=g, dtype=F64) * torch.exp(torch.randn((1, nkv, d), generator=g, dtype=F64) * 0.4) for _ in range(2))
@@ -236,6 +256,10 @@ def attend(entries, nq, nkv, d, page, dtype=torch.bfloat16, seed=0, window=0, ch
         spoil(k, v, rows, page)
     cache.store(k, v, [[i * cache.block, cache.block, i, 0] for i in range(pool * cache.nb)])
     view = view_of(cache)
+    if unwritten is not None:
+        free = sorted(set(range(pool)) - {p for r in rows for p in r})
+        view.scales[free] = unwritten
+        view.keys.view(torch.uint8)[free] = view.values.view(torch.uint8)[free] = 0x7f
     width = max(len(r) for r in rows) + 1
     table = [r + [-1] * (width - len(r)) for r in rows]
     for b, j in none:
@@ -264,10 +288,7 @@ def attend(entries, nq, nkv, d, page, dtype=torch.bfloat16, seed=0, window=0, ch
         cache8.AttentionPlan.FEW_WALKS = was
     want, mass, size = plain.attention(q[:total].cpu().to(F64).reshape(total, nq, d), cache, entries, table, scale, window, chunk, softcap,
                                        sinks, gates[:total] if gates is not None else None, width_g, pool)
-    if dtype == torch.float32:
-        bound = (2 * 2.0 ** -24 * (d + 2) * size + 1e-6) * mass + 2.0 ** -24 * want.abs()
-    else:
-        bound = 2.0 ** -8 * (mass + want.abs()) + (1e-5 + 2.0 ** -22 * size) * mass
+    bound = bound_of(dtype, d, want, mass, size)
     fine = torch.isfinite(want)
     for got in outs:
         assert torch.equal(fine, torch.isfinite(got)), (fine != torch.isfinite(got)).nonzero()[:5]
@@ -366,6 +387,35 @@ def test_attention_what_is_not_finite_stays_with_those_who_see_it(dtype, page):
     bad = torch.isnan(got)
     assert not bad[:30].any() and bad[30:60, :, 3].all() and not bad[30:60, :, 4].any()
     assert not bad[60:80].any() and bad[80:110].all() and not bad[120:].any()
+
+
+@pytest.mark.parametrize("d,page,dtype", [(32, 16, torch.bfloat16), (96, 48, torch.bfloat16), (128, 32, torch.bfloat16), (40, 12, torch.float32)])
+@pytest.mark.parametrize("scale", [math.nan, -math.inf, -3.0e38])
+def test_attention_of_a_pool_with_pages_that_nobody_wrote(d, page, dtype, scale):
+    attend([(70, 1), (0, 140), (0, 1), (333, 40), (15, 1)], 4, 2, d, page, dtype, seed=12, none=((0, 1), (3, 2)), unwritten=scale)
+
+
+@pytest.mark.parametrize("d,page,dtype", [(32, 16, torch.bfloat16), (32, 20, torch.bfloat16), (64, 32, torch.float32)])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_of_positions_far_behind_the_table(d, page, dtype, rows):
+    """Rows at the last positions that 32 bits have see what the table has, as rows right behind it do.  (The two are cut differently, and portions among them take
+    kernels that round their weights at different maxima: each is held to the bound that a kernel's result has.)"""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    pages = 9
+    cache = plain.Cache(pages, 2, page, d)
+    x = torch.randn((pages * page, 2, d), generator=torch.Generator().manual_seed(5), dtype=F64)
+    cache.store(x, x.flip(0), [[i * cache.block, cache.block, i, 0] for i in range(pages * cache.nb)])
+    view, table = view_of(cache), ints([list(range(pages))])
+    q = torch.randn((rows, 4 * d), generator=torch.Generator().manual_seed(6)).to(dtype).to(DEV)
+    want, mass, size = plain.attention(q.cpu().to(F64).reshape(rows, 4, d), cache, [(pages * page, rows)], [list(range(pages)) + [-1] * rows], d ** -0.5)
+    for start in (pages * page, 2 ** 31 - 1 - rows):
+        positions = torch.arange(start, start + rows, dtype=torch.int64).to(torch.int32).to(DEV)
+        made = cache8.plan(metas([(start, rows)]), 4, 2, d, positions, page_size=page, dtype=dtype)
+        out = torch.full_like(q, 7.0)
+        cache8.attention(q, out, made, view, positions, ints([0] * rows), table, d ** -0.5)
+        assert ((out.cpu().to(F64).reshape(rows, 4, d) - want).abs() <= bound_of(dtype, d, want, mass, size) + 1e-12).all()
 
 
 def test_attention_of_pages_beyond_32_bits():
