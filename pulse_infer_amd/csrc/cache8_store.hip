@@ -7,8 +7,12 @@
 //
 // A workgroup takes a (block, kv head): a block's scale needs all of its tokens, and its earlier bytes move when the scale grows, so
 // whoever else wrote to the block in the same step would race.  Workgroups behind those take q's heads.  All arithmetic is float32; k and
-// v are rounded once, to 8 bits, and never to bfloat16 in between.  Bound: decoding, a launch's latency and the chain work list ->
-// rows -> largest value -> bytes; prompts, the reading of the projection and the writing of q.
+// v are rounded once, to 8 bits, and never to bfloat16 in between.  Some tens to 256 rows may come as the projection's shares: a prompt of
+// 23 tokens, 36 layers of 32 heads on 8 of 128, takes 3,640 us with them and 4,048 from a product that adds them up itself.
+//
+// Bound: decoding, a launch's latency and the chain work list -> rows -> largest value -> bytes (32 heads on 8 of 128, one token 5.0 us, 32
+// tokens 5.6; an empty launch 2 to 3); prompts, the reading of the projection and the writing of q (2,048 tokens 15.8 us, 46 MB: 2.9 TB/s
+// of the 4.8 that a copy of 2 GB reaches; these 46 MB come from the product before and lie in the last cache as often as not).
 #include "cache8.h"
 
 #include <algorithm>
@@ -30,6 +34,9 @@ struct StoreArgs {
     int n_blocks, blocks_per_page, block, page_size;
     int64_t all_blocks;          // of the pool
     int lanes;                   // lanes a head, a power of two: 8 channels each
+    const float* parts;          // the rows as float32 shares of the projection, added up here in their order; null: qkv's
+    int shares;
+    int64_t part_stride, part_row;
 };
 
 // Channels of the pair p: neighbours, or half the rotated channels apart; behind the rotated ones neighbours again.
@@ -78,6 +85,26 @@ __device__ __forceinline__ void read_pairs(const StoreArgs& a, const T* row, int
             y[i] = on ? to_f32<T>(row[ib]) : 0.f;
         }
     }
+}
+
+// The same of a row that comes as shares: whole pieces, the shares asked for together.
+__device__ __forceinline__ void read_shares(const StoreArgs& a, const float* row, int c, float (&x)[4], float (&y)[4]) {
+    read_pairs<float, true>(a, row, c, x, y);
+#pragma unroll 4
+    for (int s = 1; s < a.shares; ++s) {
+        float u[4], v[4];
+        read_pairs<float, true>(a, row + s * a.part_stride, c, u, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] += u[i];
+            y[i] += v[i];
+        }
+    }
+}
+template <typename T, bool WHOLE, bool PARTS>
+__device__ __forceinline__ void read_head(const StoreArgs& a, const T* qkv, int64_t t, int64_t head, int c, float (&x)[4], float (&y)[4]) {
+    if constexpr (PARTS) read_shares(a, a.parts + t * a.part_row + head * a.d, c, x, y);
+    else read_pairs<T, WHOLE>(a, qkv + t * a.row_stride + head * a.d, c, x, y);
 }
 
 // Norm and rotation of those pairs; the sum of squares runs over the head's `lanes` neighbouring lanes.
@@ -159,7 +186,7 @@ __device__ __forceinline__ void write_pairs(const StoreArgs& a, T* to, int c, co
 }
 
 // A workgroup's share of q: neighbouring groups of lanes take neighbouring heads of the rows in turn.
-template <typename T, typename TW, bool WHOLE>
+template <typename T, typename TW, bool WHOLE, bool PARTS>
 __device__ __forceinline__ void rows_of_q(const StoreArgs& a, int64_t first, const T* qkv, T* q_out, const TW* q_w, const float* cos_t,
                                           const float* sin_t, const int* positions) {
     const int tid = threadIdx.x, c = tid % a.lanes;
@@ -168,7 +195,7 @@ __device__ __forceinline__ void rows_of_q(const StoreArgs& a, int64_t first, con
     const int64_t t = live ? i / a.nq : 0;
     const int h = live ? static_cast<int>(i - t * a.nq) : 0;
     float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-    if (on) read_pairs<T, WHOLE>(a, qkv + t * a.row_stride + static_cast<int64_t>(h) * a.d, c, x, y);
+    if (on) read_head<T, WHOLE, PARTS>(a, qkv, t, h, c, x, y);
     float factor = 1.f;
     if (a.temp_every > 0) factor = 1.f + a.temp_coef * logf(static_cast<float>((positions[t] + 1) / a.temp_every) + 1.f);
     prepare_pairs<TW, WHOLE>(a, q_w, cos_t, sin_t, t, c, factor, x, y);
@@ -223,15 +250,15 @@ __device__ __forceinline__ bool job_of(const StoreArgs& a, const int4* work, uin
 
 // Blocks of 16 tokens and heads of a multiple of 8 channels, NP * 128 at most, in whole pieces: what is read is kept in registers until
 // the scale is known.  Keys: a group of lanes takes a token's row.  Values: a thread takes a pair of channels and four of the block's
-// tokens, whose bytes are a word; a word that holds earlier tokens too is put together with them.
-template <typename T, typename TW, int NP>
+// tokens, whose bytes are a word; a word that holds earlier tokens too is put together with them.  PARTS: the rows are shares.
+template <typename T, typename TW, int NP, bool PARTS>
 __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T* q_out, const TW* __restrict__ q_w, const TW* __restrict__ k_w,
                                                                 const float* __restrict__ cos_t, const float* __restrict__ sin_t,
                                                                 uint8_t* keys, uint8_t* values, float* scales, const int* __restrict__ positions,
                                                                 const int4* __restrict__ work, StoreArgs a) {
     const int tid = threadIdx.x, block_groups = a.n_blocks * a.nkv;
     if (static_cast<int>(blockIdx.x) >= block_groups) {
-        rows_of_q<T, TW, true>(a, blockIdx.x - block_groups, qkv, q_out, q_w, cos_t, sin_t, positions);
+        rows_of_q<T, TW, true, PARTS>(a, blockIdx.x - block_groups, qkv, q_out, q_w, cos_t, sin_t, positions);
         return;
     }
     Job j;
@@ -250,7 +277,7 @@ __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T*
         const int i = n * at_once + tid / a.lanes;
 #pragma unroll
         for (int e = 0; e < 4; ++e) kx[n][e] = ky[n][e] = vx[n][e] = vy[n][e] = 0.f;
-        if (on && i < j.rows) read_pairs<T, true>(a, qkv + static_cast<int64_t>(j.first + i) * a.row_stride + static_cast<int64_t>(a.nq + j.g) * d, c, kx[n], ky[n]);
+        if (on && i < j.rows) read_head<T, true, PARTS>(a, qkv, j.first + i, a.nq + j.g, c, kx[n], ky[n]);
         const int qd = quad + n * quads_at_once;
         old[n][0] = old[n][1] = 0;
         if (quad < quads_at_once && qd < 4) {
@@ -262,8 +289,16 @@ __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T*
             for (int e = 0; e < 4; ++e) {
                 const int row = 4 * qd + e - j.at;
                 if (row >= 0 && row < j.rows) {
-                    const T* v = qkv + static_cast<int64_t>(j.first + row) * a.row_stride + static_cast<int64_t>(a.v_head0 + j.g) * d + vc;
-                    if constexpr (sizeof(T) == 2) {
+                    const int64_t column = static_cast<int64_t>(a.v_head0 + j.g) * d + vc;
+                    const T* v = qkv + static_cast<int64_t>(j.first + row) * a.row_stride + column;
+                    if constexpr (PARTS) {
+                        const float* part = a.parts + static_cast<int64_t>(j.first + row) * a.part_row + column;
+#pragma unroll 4
+                        for (int s = 0; s < a.shares; ++s) {
+                            const float2 u = *reinterpret_cast<const float2*>(part + s * a.part_stride);
+                            vx[n][e] += u.x, vy[n][e] += u.y;
+                        }
+                    } else if constexpr (sizeof(T) == 2) {
                         const uint32_t u = *reinterpret_cast<const uint32_t*>(v);
                         vx[n][e] = __uint_as_float(u << 16), vy[n][e] = __uint_as_float(u & 0xffff0000u);
                     } else {
@@ -348,7 +383,7 @@ __global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out,
                                                          const int4* __restrict__ work, StoreArgs a) {
     const int tid = threadIdx.x, block_groups = a.n_blocks * a.nkv;
     if (static_cast<int>(blockIdx.x) >= block_groups) {
-        rows_of_q<T, TW, false>(a, blockIdx.x - block_groups, qkv, q_out, q_w, cos_t, sin_t, positions);
+        rows_of_q<T, TW, false, false>(a, blockIdx.x - block_groups, qkv, q_out, q_w, cos_t, sin_t, positions);
         return;
     }
     Job j;
@@ -437,6 +472,8 @@ struct PulseStore8 {
     const int *positions, *work;
     int x_dtype, w_dtype, rotary_dim, pairing, num_pages, page_size, n_blocks, tokens, nq, nkv, d, plain_norm, v_head0, temp_every;
     float eps, temp_coef;
+    const float* parts;
+    int64_t part_stride, part_row, shares;
 };
 
 extern "C" int pulse_store8(const PulseStore8* args, hipStream_t stream) {
@@ -460,13 +497,15 @@ extern "C" int pulse_store8(const PulseStore8* args, hipStream_t stream) {
     PULSE_REQUIRE(!(q_w == nullptr) == !(k_w == nullptr) && !(plain_norm && q_w), "store8: bad norm options");
     PULSE_REQUIRE(temp_every >= 0 && (temp_every == 0 || positions), "store8: bad query temperature");
     PULSE_REQUIRE(qkv && q_out && keys && values && scales && (n_blocks == 0 || work), "store8: an operand is missing");
+    const int64_t columns = static_cast<int64_t>(std::max(nq + nkv, v_head0 + nkv)) * d;
     PULSE_REQUIRE((reinterpret_cast<uintptr_t>(work) & 15) == 0, "store8: the work list must be aligned to 16 bytes");
     if (tokens == 0) return 0;
     const int block = cache8::block_tokens(page_size);
     int lanes = 1;
     while (lanes * 8 < d) lanes *= 2;
     StoreArgs a{nq, nkv, d, tokens, row_stride, q_stride, eps, rotary_dim, pairing, q_w ? 1 : plain_norm ? 2 : 0, v_head0, temp_coef, temp_every,
-                n_blocks, page_size / block, block, page_size, static_cast<int64_t>(num_pages) * (page_size / block), lanes};
+                n_blocks, page_size / block, block, page_size, static_cast<int64_t>(num_pages) * (page_size / block), lanes,
+                in.parts, static_cast<int>(in.shares), in.part_stride, in.part_row};
     const int64_t q_groups = (static_cast<int64_t>(tokens) * nq + THREADS / lanes - 1) / (THREADS / lanes);
     const int64_t grid = q_groups + static_cast<int64_t>(n_blocks) * nkv;
     PULSE_REQUIRE(grid <= 0x7fffffff, "store8: too many rows");
@@ -475,6 +514,9 @@ extern "C" int pulse_store8(const PulseStore8* args, hipStream_t stream) {
     const bool whole = block == cache8::BLOCK && d % 8 == 0 && rotary_dim % 8 == 0 && row_stride % 4 == 0 && q_stride % 4 == 0 &&
                        aligned(qkv, 4 * size) && aligned(q_out, 4 * size) && aligned(q_w, 4 * w_size) && aligned(k_w, 4 * w_size) &&
                        aligned(cos_t, 16) && aligned(sin_t, 16) && aligned(keys, 4) && aligned(values, 4);
+    PULSE_REQUIRE(!in.parts || (whole && x_dtype == PULSE_BF16 && in.shares > 0 && in.shares <= 64 && in.part_row >= columns &&
+                                in.part_row % 4 == 0 && in.part_stride % 4 == 0 && aligned(in.parts, 16)),
+                  "store8: shares need bfloat16 rows, aligned, in chunks of eight channels, and pages of a multiple of 16 tokens");
     auto go = [&](auto x, auto w) {
         using T = decltype(x);
         using TW = decltype(w);
@@ -483,10 +525,19 @@ extern "C" int pulse_store8(const PulseStore8* args, hipStream_t stream) {
                 static_cast<const T*>(qkv), static_cast<T*>(q_out), static_cast<const TW*>(q_w), static_cast<const TW*>(k_w), cos_t, sin_t,
                 static_cast<uint8_t*>(keys), static_cast<uint8_t*>(values), scales, positions, reinterpret_cast<const int4*>(work), a);
         };
-        if (!whole) run(store8_kernel<T, TW>);
-        else if (d <= 128) run(store8_blocks_kernel<T, TW, 1>);
-        else if (d <= 256) run(store8_blocks_kernel<T, TW, 2>);
-        else run(store8_blocks_kernel<T, TW, 4>);
+        auto by_width = [&](auto parts) {
+            if (d <= 128) run(store8_blocks_kernel<T, TW, 1, decltype(parts)::value>);
+            else if (d <= 256) run(store8_blocks_kernel<T, TW, 2, decltype(parts)::value>);
+            else run(store8_blocks_kernel<T, TW, 4, decltype(parts)::value>);
+        };
+        if (!whole) {
+            run(store8_kernel<T, TW>);
+        } else {
+            if constexpr (sizeof(T) == 2) {
+                if (in.parts) return by_width(std::true_type());
+            }
+            by_width(std::false_type());
+        }
     };
     auto by_weight = [&](auto x) {
         if (w_dtype == PULSE_F32) go(x, float());

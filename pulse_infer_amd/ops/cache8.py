@@ -72,7 +72,7 @@ def _pages(what: str, view: Paged8CacheView, nkv: int, d: int) -> Tuple[int, int
 
 # The arguments of the entry points as the structures of csrc/cache8_maps.hip, cache8_store.hip and cache8_attn.h, put together at once.
 _MAPS = struct.Struct("@9Q8i")
-_STORE = struct.Struct("@QqQq9Q14i2f")
+_STORE = struct.Struct("@QqQq9Q14i2fQ3q")
 _ATTN = struct.Struct("@QqQq7Qq5Q14i2f")
 
 
@@ -151,16 +151,18 @@ def blocks_touched(entries: Sequence[Any], page_size: int) -> int:
 def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, view: Paged8CacheView, positions: torch.Tensor,
           blocks: torch.Tensor, *, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 0.0,
           cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, rotary_dim: int = 0, pairing: int = 0,
-          plain_norm: bool = False, v_head0: Optional[int] = None, q_temperature: Optional[tuple] = None) -> None:
+          plain_norm: bool = False, v_head0: Optional[int] = None, q_temperature: Optional[tuple] = None,
+          parts: Optional[torch.Tensor] = None) -> None:
     """A step's rows of the fused projection: norm and rotation of q (to ``q_out`` [T, >= nq * d], which may be the front of ``qkv``) and k,
     k and v into the blocks that ``step_maps`` listed.  The options are those of ``kernels.qk_rope_kv``.
 
     Of a block that is begun (its first token among the new ones) nothing that it held before stays; behind the new tokens it holds
     zeros.  Of another the earlier bytes stay, moved to the new scale where that has grown.  A block may be listed once: requests do
     not share pages that a step writes to.  ``qkv`` [T, columns] bfloat16 or float32 with contiguous rows; heads of an even number of
-    channels up to 512."""
+    channels up to 512.  ``parts`` float32 [shares, T, columns]: the rows are the sum of these shares, in their order, and of ``qkv``
+    nothing is read (``store_takes_parts``)."""
     what = "store"
-    _here(what, (qkv, q_out, view.keys, view.values, view.scales, positions, blocks, q_weight, k_weight, cos, sin))
+    _here(what, (qkv, q_out, view.keys, view.values, view.scales, positions, blocks, q_weight, k_weight, cos, sin, parts))
     if not view.writable:
         _refuse(what, "the cache is another run's")
     if nq <= 0 or nkv <= 0 or d <= 0 or d % 2 or d > MAX_HEAD_DIM:
@@ -202,10 +204,24 @@ def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, vie
         coef, every = float(q_temperature[0]), int(q_temperature[1])
         if every <= 0:
             _refuse(what, "the query temperature's interval must be positive")
+    shares = part_stride = part_row = 0
+    if parts is not None:
+        if parts.dtype != torch.float32 or parts.dim() != 3 or parts.shape[1] != tokens or parts.shape[2] < columns or not parts.is_contiguous():
+            _refuse(what, f"the shares must be contiguous float32 [shares, {tokens}, {columns}]")
+        shares, part_stride, part_row = parts.shape[0], parts.stride(0), parts.shape[2]
+        if not store_takes_parts(qkv, d, rotated, page, parts, q_out, q_weight, k_weight, cos, sin) or part_row % 4 or q_stride % 4 or shares < 1:
+            _refuse(what, "shares need bfloat16 rows, aligned, in chunks of eight channels, and pages of a multiple of 16 tokens")
     call("pulse_store8", _STORE.pack(
         qkv.data_ptr(), stride, q_out.data_ptr(), q_stride, _at(q_weight), _at(k_weight), _at(cos), _at(sin), view.keys.data_ptr(),
         view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(), blocks.data_ptr(), _tag(qkv, what), w_tag, rotated, pairing,
-        pages, page, places, tokens, nq, nkv, d, plain_norm, v_head0, every, eps, coef), _stream())
+        pages, page, places, tokens, nq, nkv, d, plain_norm, v_head0, every, eps, coef, _at(parts), part_stride, part_row, shares), _stream())
+
+
+def store_takes_parts(qkv: torch.Tensor, d: int, rotary_dim: int, page_size: int, *others: Optional[torch.Tensor]) -> bool:
+    """Whether ``store`` takes these rows as float32 shares: in pieces that neither heads nor rotation cut (``others``: the norms' weights
+    and the rotation's tables)."""
+    return (qkv.dtype == torch.bfloat16 and d % 8 == 0 and rotary_dim % 8 == 0 and page_size % 16 == 0 and qkv.stride(0) % 4 == 0
+            and all(t is None or t.data_ptr() % 16 == 0 for t in (qkv, *others)))
 
 
 # --------------------------------------------------------------------------------------------------------- the attention

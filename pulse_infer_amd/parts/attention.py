@@ -218,14 +218,17 @@ class PagedAttention(Part):
         from_raw = not eight and self.decodes_from_raw(ctx, cache, qkv, tables)
         # (of the projection only q, k and v are read behind the rotation, which may take them as shares; a gate lies beside them)
         parts = None
-        if self.qkv.may_part(tokens) and not from_raw and not eight and rows is None and not self.output_gate and not isinstance(x, LazyNorm) \
-                and kernels.qk_rope_takes_parts(qkv, self.d, tables.rotary_dim if tables is not None else 0, cache.keys, self.q_w, self.k_w,
-                                                *((tables.cos, tables.sin) if tables is not None else ())):
-            parts = self.qkv.forward_parts(x, ws)
+        if self.qkv.may_part(tokens) and not from_raw and rows is None and not self.output_gate and not isinstance(x, LazyNorm):
+            rotary_dim, others = 0, (self.q_w, self.k_w)
+            if tables is not None:
+                rotary_dim, others = tables.rotary_dim, (*others, tables.cos, tables.sin)
+            if (cache.writable and cache8.store_takes_parts(qkv, self.d, rotary_dim, cache.page_size, *others) if eight
+                    else kernels.qk_rope_takes_parts(qkv, self.d, rotary_dim, cache.keys, *others)):
+                parts = self.qkv.forward_parts(x, ws)
         if parts is None:
             self.qkv.forward(x, qkv, rows=rows)
         if eight:
-            self.attend8(qkv, attn, ctx, cache, table, tables, gate)
+            self.attend8(qkv, attn, ctx, cache, table, tables, gate, parts)
         elif from_raw:
             # decoded tokens only: the attention kernel prepares q and each token's own key itself
             self.attend(qkv, attn, ctx, cache, table, raw=(tables, write), gate=gate)
@@ -268,8 +271,8 @@ class PagedAttention(Part):
                 and attention_mfma.decode_takes(self.d, tables.rotary_dim, tables.pairing))
 
     def attend8(self, qkv: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: Paged8CacheView, table: torch.Tensor, tables: Any,
-                gate: Optional[torch.Tensor]) -> None:
-        """q, k and v of the projection's rows prepared, k and v stored in 8 bits, and ``out`` = attention over the cache."""
+                gate: Optional[torch.Tensor], parts: Optional[torch.Tensor] = None) -> None:
+        """q, k and v of the projection's rows (or of its shares) prepared, k and v stored in 8 bits, and ``out`` = attention over the cache."""
         rotation = dict(cos=tables.cos, sin=tables.sin, rotary_dim=tables.rotary_dim, pairing=tables.pairing) if tables is not None else {}
         if cache.writable:
             key = f"attention8.blocks:{cache.group}"
@@ -280,7 +283,7 @@ class PagedAttention(Part):
                                  blocks=blocks)
                 ctx.extras[key] = blocks
             cache8.store(qkv, qkv, self.nq, self.nkv, self.d, cache, ctx.positions, ctx.extras[key], q_weight=self.q_w, k_weight=self.k_w,
-                         eps=self.eps, plain_norm=self.plain_norm, v_head0=self.v_head0, q_temperature=self.q_temperature, **rotation)
+                         eps=self.eps, plain_norm=self.plain_norm, v_head0=self.v_head0, q_temperature=self.q_temperature, parts=parts, **rotation)
         else:
             kernels.qk_rope_kv(qkv, self.nq, self.nkv, self.d, self.q_w, self.k_w, self.eps, rotation.get("cos"), rotation.get("sin"),
                                rotation.get("rotary_dim", 0), rotation.get("pairing", 0), None, None, ctx.positions, ctx.token_entry, None,

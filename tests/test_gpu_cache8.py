@@ -163,6 +163,41 @@ def test_store(nq, nkv, d, page, dtype, norm, rotary, pairing, entries, in_place
         assert (a != b).double().mean() < 1e-3
 
 
+@pytest.mark.parametrize("nq,nkv,d,page,norm,rotary,pairing,shares,entries", [
+    (4, 2, 128, 16, True, 128, 1, 4, [(0, 40), (15, 1), (16, 1), (33, 20)]), (4, 1, 64, 32, False, 0, 0, 1, [(0, 16), (7, 9)]),
+    (2, 2, 256, 48, "plain", 64, 1, 7, [(0, 50), (31, 2)]), (1, 1, 512, 16, True, 512, 0, 2, [(3, 20)]), (3, 3, 40, 16, False, 16, 1, 9, [(0, 33)])])
+def test_store_of_rows_in_shares(nq, nkv, d, page, norm, rotary, pairing, shares, entries):
+    """Shares that are multiples of 2^-10 below 8: their sums are exact, and what is stored is what the plain form stores of the sums."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    g = torch.Generator().manual_seed(shares)
+    pages, pool, _ = layout(entries, page, 6)
+    want = plain.maps(entries, pages, page, pool, 1)
+    total, columns = sum(c for _, c in entries), (nq + 2 * nkv) * d
+    cache = plain.Cache(pool, nkv, page, d)
+    old = torch.randn((pool * page, nkv, d), generator=g, dtype=F64) * 0.3
+    cache.store(old, old * 5, [[i * cache.block, cache.block, i, 0] for i in range(pool * cache.nb)])
+    view = view_of(cache)
+    parts = torch.round(torch.randn((shares, total, columns + 4), generator=g).clamp(-7, 7) * 1024) / 1024
+    w = [(1 + 0.2 * torch.rand(d, generator=g)).to(torch.bfloat16).to(DEV) for _ in range(2)] if norm is True else [None, None]
+    angles = torch.tensor(want["positions"], dtype=F64)[:, None] * 10.0 ** -(torch.arange(rotary // 2, dtype=F64) / 9) if rotary else None
+    cos, sin = (torch.cos(angles).float().to(DEV), torch.sin(angles).float().to(DEV)) if rotary else (None, None)
+    q, k, v = plain.prepared(parts.to(F64).sum(0)[:, :columns], nq, nkv, d, None, w[0], w[1], 1e-6, norm == "plain", angles, rotary, pairing, None,
+                             torch.tensor(want["positions"]))
+    cache.store(k, v, want["blocks"])
+    qkv = torch.full((total, columns), math.nan, dtype=torch.bfloat16, device=DEV)
+    cache8.store(qkv, qkv, nq, nkv, d, view, ints(want["positions"]), ints(want["blocks"]), q_weight=w[0], k_weight=w[1], eps=1e-6, cos=cos, sin=sin,
+                 rotary_dim=rotary, pairing=pairing, plain_norm=norm == "plain", parts=parts.to(DEV))
+    got_q = qkv[:, :nq * d].cpu().to(F64).view(total, nq, d)
+    assert ((got_q - q).abs() <= 2.0 ** -8 * q.abs() + 1e-5 * q.abs().amax(-1, keepdim=True)).all() and torch.isnan(qkv[:, nq * d:]).all()
+    keys, values, scales = cache.tensors()
+    assert torch.equal(view.scales.cpu(), scales) and torch.equal(view.values.cpu().view(torch.uint8), values.view(torch.uint8))
+    a, b = plain.decode(view.keys), plain.decode(keys)
+    assert ((a - b).abs() <= torch.maximum(b.abs() * 2.0 ** -3, torch.tensor(2.0 ** -9, dtype=F64))).all()
+    assert (a != b).double().mean() < 1e-3 and (norm or rotary or torch.equal(a, b))
+
+
 def test_store_token_by_token_grows_its_scale():
     """One token after the other, each larger than those before: what the block holds is what the plain form's appends give, byte by
     byte, and within one rounding of the token at the final scale."""
@@ -604,6 +639,12 @@ def test_refusals():
     bad(put, cos=torch.zeros((3, 16), device=DEV), sin=torch.zeros((3, 16), device=DEV), rotary_dim=30)
     bad(put, cos=torch.zeros((3, 16), device=DEV), sin=torch.zeros((3, 16), device=DEV), rotary_dim=32, pairing=2)
     bad(put, q_temperature=(0.1, 0))
+    put(parts=torch.zeros((2, 3, 256), device=DEV))
+    bad(put, parts=torch.zeros((2, 3, 252), device=DEV))
+    bad(put, parts=torch.zeros((2, 3, 258), device=DEV))
+    bad(put, parts=torch.zeros((3, 256), device=DEV))
+    bad(put, parts=torch.zeros((2, 3, 256), dtype=torch.bfloat16, device=DEV))
+    bad(put, parts=torch.zeros((2, 3, 256), device=DEV), qkv=qkv.float(), q=q.float())
     bad(put, view=Paged8CacheView(0, view.keys, view.values, view.scales, 16, writable=False))
     maps = lambda **k: cache8.step_maps(k.pop("start", ints([0])), k.pop("count", ints([3])), page_size=k.pop("page_size", 16), num_pages=k.pop("num_pages", 4), **k)  # noqa: E731
     maps(pages=ints([1]), slots=ints([0] * 3))
