@@ -10,16 +10,17 @@
 // v are rounded once, to 8 bits, and never to bfloat16 in between.  Some tens to 256 rows may come as the projection's shares: a prompt of
 // 23 tokens, 36 layers of 32 heads on 8 of 128, takes 3,640 us with them and 4,048 from a product that adds them up itself.
 //
-// Bound: decoding, a launch's latency and the chain work list -> rows -> largest value -> bytes (32 heads on 8 of 128, one token 5.0 us, 32
-// tokens 5.6; an empty launch 2 to 3); prompts, the reading of the projection and the writing of q (2,048 tokens 15.8 us, 46 MB: 2.9 TB/s
-// of the 4.8 that a copy of 2 GB reaches; these 46 MB come from the product before and lie in the last cache as often as not).
+// Bound: decoding, a launch's latency and the chain work list -> rows -> largest value -> bytes (32 heads on 8 of 128, in a recording: one
+// token 4.4 us, 64 tokens 5.7); prompts, the reading of the projection and the writing of q (2,048 tokens 14.3 us for 46 MB, 3.2 TB/s of
+// the 4.8 that a copy of 2 GB reaches; 15.3 with the hardware's divisions in the place of multiplications and shifts).  Two or four heads
+// of q a thread: 15.6 and 17.8 us for 15.3.
 #include "cache8.h"
 
 #include <algorithm>
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREAD_BITS = 8, THREADS = 1 << THREAD_BITS;
 constexpr int MAX_DIM = 512;
 
 struct StoreArgs {
@@ -31,9 +32,10 @@ struct StoreArgs {
     int v_head0;                 // the values of kv head g are columns (v_head0 + g) * d .. of a row
     float temp_coef;             // q *= 1 + temp_coef * ln(floor((pos + 1) / temp_every) + 1); temp_every 0: none
     int temp_every;
-    int n_blocks, blocks_per_page, block, page_size;
+    int n_blocks, block, page_size;
+    cache8::Div blocks_per_page, q_heads, kv_heads, pairs;      // (pairs: d / 2)
     int64_t all_blocks;          // of the pool
-    int lanes;                   // lanes a head, a power of two: 8 channels each
+    int lanes, lane_bits;        // lanes a head, a power of two: 8 channels each
     const float* parts;          // the rows as float32 shares of the projection, added up here in their order; null: qkv's
     int shares;
     int64_t part_stride, part_row;
@@ -187,13 +189,13 @@ __device__ __forceinline__ void write_pairs(const StoreArgs& a, T* to, int c, co
 
 // A workgroup's share of q: neighbouring groups of lanes take neighbouring heads of the rows in turn.
 template <typename T, typename TW, bool WHOLE, bool PARTS>
-__device__ __forceinline__ void rows_of_q(const StoreArgs& a, int64_t first, const T* qkv, T* q_out, const TW* q_w, const float* cos_t,
+__device__ __forceinline__ void rows_of_q(const StoreArgs& a, int first, const T* qkv, T* q_out, const TW* q_w, const float* cos_t,
                                           const float* sin_t, const int* positions) {
-    const int tid = threadIdx.x, c = tid % a.lanes;
-    const int64_t i = first * (THREADS / a.lanes) + tid / a.lanes;
-    const bool live = i < static_cast<int64_t>(a.tokens) * a.nq, on = 8 * c < a.d;
-    const int64_t t = live ? i / a.nq : 0;
-    const int h = live ? static_cast<int>(i - t * a.nq) : 0;
+    const int tid = threadIdx.x, c = tid & (a.lanes - 1);
+    const int i = (first << (THREAD_BITS - a.lane_bits)) + (tid >> a.lane_bits);       // (rows times heads are less than 2^31)
+    const bool live = i < a.tokens * a.nq, on = 8 * c < a.d;
+    const int row = live ? a.q_heads.over(i) : 0, h = live ? i - row * a.nq : 0;
+    const int64_t t = row;
     float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
     if (on) read_head<T, WHOLE, PARTS>(a, qkv, t, h, c, x, y);
     float factor = 1.f;
@@ -234,17 +236,18 @@ struct Job {
     float* scale;
 };
 __device__ __forceinline__ bool job_of(const StoreArgs& a, const int4* work, uint8_t* keys, uint8_t* values, float* scales, Job& j) {
-    const int4 w = work[blockIdx.x / a.nkv];
-    j.g = blockIdx.x % a.nkv;
+    const int place = a.kv_heads.over(blockIdx.x);
+    const int4 w = work[place];
+    j.g = blockIdx.x - place * a.nkv;
     j.first = w.x, j.rows = w.y, j.at = w.w;
     if (w.y <= 0 || w.z < 0 || w.z >= a.all_blocks || w.w < 0 || w.w >= a.block || w.y > a.block - w.w || w.x < 0 || w.y > a.tokens ||
         w.x > a.tokens - w.y)
         return false;
-    const int64_t page = w.z / a.blocks_per_page, head = page * a.nkv + j.g;
-    const int inner = w.z - static_cast<int>(page) * a.blocks_per_page;
+    const int page = a.blocks_per_page.over(w.z), inner = w.z - page * a.blocks_per_page.b;
+    const int64_t head = static_cast<int64_t>(page) * a.nkv + j.g;
     j.keys = keys + (head * a.page_size + static_cast<int64_t>(inner) * a.block) * a.d;
     j.values = values + (head * a.page_size + static_cast<int64_t>(inner) * a.block) * a.d;
-    j.scale = scales + (head * a.blocks_per_page + inner) * 2;
+    j.scale = scales + (head * a.blocks_per_page.b + inner) * 2;
     return true;
 }
 
@@ -263,18 +266,18 @@ __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T*
     }
     Job j;
     if (!job_of(a, work, keys, values, scales, j)) return;
-    const int c = tid % a.lanes, at_once = THREADS / a.lanes, d = a.d;
+    const int c = tid & (a.lanes - 1), at_once = THREADS >> a.lane_bits, of_lanes = tid >> a.lane_bits, d = a.d;
     const bool on = 8 * c < d, fresh = j.at == 0;
     const float had_k = fresh ? 0.f : j.scale[0], had_v = fresh ? 0.f : j.scale[1];
-    const int pairs = d / 2, quad = tid / pairs, vc = 2 * (tid % pairs);      // (of the first NP; the others are THREADS / pairs quads further on)
-    const int quads_at_once = THREADS / pairs;
+    const int pairs = d / 2, quad = a.pairs.over(tid), vc = 2 * (tid - quad * pairs);      // (of the first NP; the others are THREADS / pairs quads further on)
+    const int quads_at_once = a.pairs.over(THREADS);
 
     // everything that is read is asked for before anything waits
     float kx[NP][4], ky[NP][4], vx[NP][4], vy[NP][4];
     uint32_t old[NP][2];
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-        const int i = n * at_once + tid / a.lanes;
+        const int i = n * at_once + of_lanes;
 #pragma unroll
         for (int e = 0; e < 4; ++e) kx[n][e] = ky[n][e] = vx[n][e] = vy[n][e] = 0.f;
         if (on && i < j.rows) read_head<T, true, PARTS>(a, qkv, j.first + i, a.nq + j.g, c, kx[n], ky[n]);
@@ -313,7 +316,7 @@ __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T*
     bool bad = false;
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-        const int i = n * at_once + tid / a.lanes;
+        const int i = n * at_once + of_lanes;
         prepare_pairs<TW, true>(a, k_w, cos_t, sin_t, j.first + min(i, j.rows - 1), c, 1.f, kx[n], ky[n]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -331,7 +334,7 @@ __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T*
 
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
-        const int i = n * at_once + tid / a.lanes;
+        const int i = n * at_once + of_lanes;
         if (on && i < j.rows) {
             const bool apart = a.pairing == 1 && 8 * c < a.rotary_dim;
             const int first = apart ? 4 * c : 8 * c, second = apart ? first + a.rotary_dim / 2 : first + 4;
@@ -388,7 +391,7 @@ __global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out,
     }
     Job j;
     if (!job_of(a, work, keys, values, scales, j)) return;
-    const int c = tid % a.lanes, at_once = THREADS / a.lanes, d = a.d;
+    const int c = tid & (a.lanes - 1), at_once = THREADS >> a.lane_bits, of_lanes = tid >> a.lane_bits, d = a.d;
     const bool on = 8 * c < d, fresh = j.at == 0;
     const float had_k = fresh ? 0.f : j.scale[0], had_v = fresh ? 0.f : j.scale[1];
     auto key_pairs = [&](int i, float (&x)[4], float (&y)[4]) {
@@ -399,13 +402,13 @@ __global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out,
         prepare_pairs<TW, false>(a, k_w, cos_t, sin_t, t, c, 1.f, x, y);
     };
     // values: a thread takes a pair of neighbouring channels and every `groups`-th token
-    const int pairs = d / 2, groups = THREADS / pairs, vc = 2 * (tid % pairs), vg = tid / pairs;
+    const int groups = a.pairs.over(THREADS), vg = a.pairs.over(tid), vc = 2 * (tid - vg * (d / 2));
     const T* vrow = qkv + static_cast<int64_t>(j.first) * a.row_stride + static_cast<int64_t>(a.v_head0 + j.g) * d + vc;
     float kmax = 0.f, vmax = 0.f;
     bool bad = false;
     for (int i0 = 0; i0 < j.rows; i0 += at_once) {
         float x[4], y[4];
-        key_pairs(i0 + tid / a.lanes, x, y);
+        key_pairs(i0 + of_lanes, x, y);
 #pragma unroll
         for (int e = 0; e < 4; ++e) kmax = fmaxf(kmax, fmaxf(size_of(x[e]), size_of(y[e])));
     }
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out,
     if (fresh || ev != was_v) around(j.values, true, cache8::pow2(max(was_v - ev, -126)));
     for (int i0 = 0; i0 < j.rows; i0 += at_once) {
         float x[4], y[4];
-        const int i = i0 + tid / a.lanes;
+        const int i = i0 + of_lanes;
         key_pairs(i, x, y);
         if (i >= j.rows || !on) continue;
         uint8_t* to = j.keys + static_cast<int64_t>(j.at + i) * d;
@@ -501,10 +504,12 @@ extern "C" int pulse_store8(const PulseStore8* args, hipStream_t stream) {
     PULSE_REQUIRE((reinterpret_cast<uintptr_t>(work) & 15) == 0, "store8: the work list must be aligned to 16 bytes");
     if (tokens == 0) return 0;
     const int block = cache8::block_tokens(page_size);
-    int lanes = 1;
-    while (lanes * 8 < d) lanes *= 2;
+    int lanes = 1, lane_bits = 0;
+    while (lanes * 8 < d) lanes *= 2, ++lane_bits;
+    PULSE_REQUIRE(static_cast<int64_t>(tokens) * nq + THREADS <= 0x7fffffff, "store8: too many rows");
     StoreArgs a{nq, nkv, d, tokens, row_stride, q_stride, eps, rotary_dim, pairing, q_w ? 1 : plain_norm ? 2 : 0, v_head0, temp_coef, temp_every,
-                n_blocks, page_size / block, block, page_size, static_cast<int64_t>(num_pages) * (page_size / block), lanes,
+                n_blocks, block, page_size, cache8::div_by(page_size / block), cache8::div_by(nq), cache8::div_by(nkv), cache8::div_by(d / 2),
+                static_cast<int64_t>(num_pages) * (page_size / block), lanes, lane_bits,
                 in.parts, static_cast<int>(in.shares), in.part_stride, in.part_row};
     const int64_t q_groups = (static_cast<int64_t>(tokens) * nq + THREADS / lanes - 1) / (THREADS / lanes);
     const int64_t grid = q_groups + static_cast<int64_t>(n_blocks) * nkv;
