@@ -439,18 +439,26 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
         }
     };
 
-    int tile = job.tile + wave;
-    if (tile < tile_end) {
+    // A wavefront takes its tiles in turn from one on that differs from item to item: where requests' pages lie one after the other, walks
+    // that all start at their first tile ask the same channels of memory at the same time (64 contexts of 8,192, pages in order, 202 -> 185 us;
+    // of 4,096 109 -> 101; pages at random, or fewer requests than fill the GPU: no difference).
+    const int mine = (tile_end - job.tile - wave + WAVES - 1) / WAVES;
+    if (mine > 0) {
+        const int turn = job.item % mine;
+        auto at = [&](int i) {
+            const int n = min(i, mine - 1) + turn;
+            return job.tile + wave + WAVES * (n < mine ? n : n - mine);
+        };
         F now, next;
-        load(tile, find(tile), now);
-        Place ahead = find(tile + WAVES);
-        for (; tile < tile_end; tile += WAVES) {
-            const bool more = tile + WAVES < tile_end;
+        load(at(0), find(at(0)), now);
+        Place ahead = find(at(1));
+        for (int i = 0; i < mine; ++i) {
+            const bool more = i + 1 < mine;
             if (more) {
-                load(tile + WAVES, ahead, next);
-                ahead = find(tile + 2 * WAVES);
+                load(at(i + 1), ahead, next);
+                ahead = find(at(i + 2));
             }
-            compute(tile, now);
+            compute(at(i), now);
             if (more) now = next;
         }
     }
