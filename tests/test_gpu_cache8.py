@@ -545,6 +545,48 @@ def test_a_step_recorded_and_replayed():
         assert torch.equal(view.scales, eager_view.scales)
 
 
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 48)])
+def test_two_steps_on_two_streams_at_once(d, page):
+    """Plans, workspaces and outputs of their own over one cache: whatever runs beside them, the results are those of each alone, bit for bit."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+    from pulse_infer_amd.parts.base import Workspace
+
+    nq, nkv = 8, 2
+    steps = [[(3000, 1), (17, 1), (2500, 1), (700, 1)], [(1200, 200), (64, 1), (900, 33)]]
+    pages, pool, _ = layout([(max(s[i][0] + s[i][1] if i < len(s) else 1 for s in steps), 0) for i in range(4)], page, 8)
+    cache = plain.Cache(pool, nkv, page, d)
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn((pool * page, nkv, d), generator=g, dtype=F64) for _ in range(2))
+    cache.store(k, v, [[i * cache.block, cache.block, i, 0] for i in range(pool * cache.nb)])
+    view, runs = view_of(cache), []
+    for entries in steps:
+        total, held = sum(c for _, c in entries), [-(-(s + c) // page) for s, c in entries]
+        at = [sum(held[:i]) for i in range(len(held))]
+        table = ints([(pages[a:a + h] + [-1] * max(held))[:max(held)] for a, h in zip(at, held)])
+        q = torch.randn((total, nq * d), generator=g).to(torch.bfloat16).to(DEV)
+        positions = ints([p for s, c in entries for p in range(s, s + c)])
+        token_entry = ints([b for b, (_, c) in enumerate(entries) for _ in range(c)])
+        made = cache8.plan(metas(entries), nq, nkv, d, positions, page_size=page, dtype=torch.bfloat16, workspace=Workspace(torch.device(DEV)))
+        runs.append((q, made, positions, token_entry, table, torch.cuda.Stream()))
+
+    def go(run):
+        q, made, positions, token_entry, table, _ = run
+        out = torch.empty_like(q)
+        cache8.attention(q, out, made.cut(positions), view, positions, token_entry, table, d ** -0.5)
+        return out
+
+    alone = [go(run) for run in runs]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(10):
+        for n, run in enumerate(runs):
+            with torch.cuda.stream(run[-1]):
+                outs.append((n, go(run)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, alone[n]) for n, out in outs) and all(torch.isfinite(out).all() for out in alone)
+
+
 def test_prompts_and_decoding_on_another_stream():
     """A prompt whole, then tokens one by one, on a stream of the program's own, against the plain forms of the same steps."""
     require_gpu()
