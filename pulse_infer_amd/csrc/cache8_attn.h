@@ -18,7 +18,7 @@ struct PulseAttn8 {
     const int* items;            // the matrix-core kernels' work: (first row, rows, entry, 0) a piece, and how it is cut (attn8_cut)
     const int* cut;
     float *part_o, *part_ml;
-    int dtype, tokens, entries, table_width, nq, nkv, d, page_size, num_pages, window, chunk, gate_width, n_items, max_work;
+    int dtype, tokens, entries, table_width, nq, nkv, d, page_size, num_pages, window, chunk, gate_width, n_items, max_work, join_here, unused;
     float scale, softcap;
 };
 
@@ -35,7 +35,7 @@ __device__ __forceinline__ float tanh_of(float x) { return 1.f - 2.f / (__expf(2
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + __expf(-x)); }
 
 // What a cut is: for every workgroup a piece (no rows: nothing to do), for every item its first piece and how many it has, then
-// attn8_few's counters of arrived pieces.
+// the counters of arrived pieces where the last one joins them.
 struct Piece {
     int row0, rows, entry, item;              // the item
     int tile, tile_end, first, pieces;        // its stretch of tiles; the item's first piece and how many there are

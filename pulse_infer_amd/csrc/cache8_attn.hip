@@ -13,7 +13,7 @@
 // attn8_few      up to 16 columns an item (a decoded token's heads; a few tokens).  Its four wavefronts take every fourth tile and
 //                meet at the end.  Bound by reading the cache.
 // attn8_many     128 columns an item (portions of prompts).  A tile is converted once for all and lies in LDS as bfloat16.
-// attn8_join     joins the pieces of items that were cut.
+// attn8_join     joins the pieces of items of attn8_many that were cut into many; else the piece that comes last does.
 #include "cache8_attn.h"
 
 #include <algorithm>
@@ -211,6 +211,23 @@ __device__ __forceinline__ float2 shared2(const float* from) {
     if constexpr (!SHARED) return *reinterpret_cast<const float2*>(from);
     const uint64_t both = __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return make_float2(__uint_as_float(static_cast<uint32_t>(both)), __uint_as_float(static_cast<uint32_t>(both >> 32)));
+}
+
+// Whether this workgroup's piece is the last of its item's (in column `x` of `width`).  A wavefront has its sums where all dies see them
+// before it meets the others, and only then is the piece counted; the counter is left at zero for the next launch.  (By a release and an
+// acquire, which write a die's cache back for every piece, 24 requests of one token took 82 us for 42.)
+__device__ __forceinline__ bool arrive_last(const PulseAttn8& a, const cache8::Piece& job, int width, int x) {
+    __shared__ int s_last;
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    int* arrived = const_cast<int*>(a.cut) + cache8::PIECE_INTS * a.max_work + 2 * a.n_items + job.item * width + x;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int before = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = before == job.pieces - 1;
+        if (s_last) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return s_last != 0;
 }
 
 // The join: out = sum_z w_z o_z / sum_z w_z l_z, w_z = exp2(m_z - max m), over an item's pieces (pieces of one column are COLS columns
@@ -500,20 +517,9 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
         }
     }
     if (whole) return;
-    // The piece that comes last joins them all.  (Its sums go by the pieces' order: who comes last changes nothing.)  A wavefront has
-    // its sums where all dies see them before it meets the others, and only then is the piece counted; the counter is left at zero for the
-    // next launch.  (By a release and an acquire, which write a die's cache back for every piece, 24 requests took 82 us for 42.)
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-    __shared__ int s_last;
-    int* arrived = const_cast<int*>(a.cut) + cache8::PIECE_INTS * a.max_work + 2 * a.n_items + job.item * gridDim.x + blockIdx.x;
-    __syncthreads();
-    if (tid == 0) {
-        const int before = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = before == job.pieces - 1;
-        if (s_last) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (s_last) join_columns<FEW, true>(a, job.first, job.pieces, gridDim.x, blockIdx.x, 0, ntok * heads, row0, ntok * heads, g * group + part * FEW, heads);
+    // The piece that comes last joins them all.  (Its sums go by the pieces' order: who comes last changes nothing.)
+    if (arrive_last(a, job, gridDim.x, blockIdx.x))
+        join_columns<FEW, true>(a, job.first, job.pieces, gridDim.x, blockIdx.x, 0, ntok * heads, row0, ntok * heads, g * group + part * FEW, heads);
 }
 
 // ------------------------------------------------------------------------------------------------------------ 128 columns
@@ -782,8 +788,55 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     }
     const WaveTwo two = wave_two<32>(__float_as_uint(l));
     l = __uint_as_float(two.a) + __uint_as_float(two.b);
+    if (!whole && a.join_here) {
+        // The piece that comes last joins them, as in attn8_few; the others' sums lie in the order of the threads, a pair of channels each.
+        const int64_t step = static_cast<int64_t>(gridDim.x) * MANY, first = static_cast<int64_t>(job.first) * step + static_cast<int64_t>(blockIdx.x) * MANY;
+        const int own = w - job.first;
+        auto sums_of = [&](int z) __attribute__((always_inline)) { return a.part_o + (first + z * step) * D + 2 * tid; };
+        auto state_of = [&](int z) __attribute__((always_inline)) { return a.part_ml + 2 * (first + z * step + col); };
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) share2(sums_of(own) + (8 * m + i) * (2 * THREADS), o[m][2 * i], o[m][2 * i + 1]);
+        if (half == 0) share2(state_of(own), top, l);
+        if (!arrive_last(a, job, gridDim.x, blockIdx.x)) return;
+        float most = top;
+        for (int z = 0; z < job.pieces; ++z) most = fmaxf(most, shared2<true>(state_of(z)).x);
+        const float shift = most == -INFINITY ? 0.f : most;
+        f32x16 all[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) all[m] = f32x16{};
+        float sum = 0.f;
+        for (int z = 0; z < job.pieces; ++z) {       // (in their order, whoever came last)
+            const float2 ml = shared2<true>(state_of(z));
+            const float f = __builtin_amdgcn_exp2f(ml.x - shift);
+            sum += ml.y * f;
+            if (z == own) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) all[m][i] = fmaf(o[m][i], f, all[m][i]);
+            } else {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    float2 x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = shared2<true>(sums_of(z) + (8 * m + i) * (2 * THREADS));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        all[m][2 * i] = fmaf(x[i].x, f, all[m][2 * i]);
+                        all[m][2 * i + 1] = fmaf(x[i].y, f, all[m][2 * i + 1]);
+                    }
+                }
+            }
+        }
+        top = most;
+        l = sum;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) o[m] = all[m];
+    }
     if (!col_ok) return;
-    if (whole) {
+    if (whole || a.join_here) {
         const float inv = finish(a, top, l, col_row, head);
         bf16_t* to = static_cast<bf16_t*>(a.out) + col_row * a.o_stride + static_cast<int64_t>(head) * D;
         if (__builtin_expect(a.gate_width > 0, 0)) {
@@ -813,8 +866,8 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     }
 }
 
-// The portions' pieces, 16 columns a workgroup (two thirds of a launch's time is that it is one: the few's last piece joins them itself,
-// but 128 columns of a head take longer than that for one workgroup).
+// The portions' pieces where there are many of an item, 16 columns a workgroup (128 columns of ten pieces take one workgroup longer
+// than a launch and its spread).
 __global__ __launch_bounds__(THREADS) void attn8_join_kernel(PulseAttn8 a) {
     const int item = blockIdx.y;
     const int2 info = reinterpret_cast<const int2*>(a.cut + cache8::PIECE_INTS * a.max_work)[item];
@@ -890,7 +943,7 @@ extern "C" int pulse_attn8_many(const PulseAttn8* a, hipStream_t stream) {
         else attn8_many_kernel<decltype(d)::value, false><<<grid, THREADS, 0, stream>>>(*a, blocks);
     });
     PULSE_LAUNCH_CHECK("attn8_many");
-    if (a->max_work > a->n_items) {
+    if (a->max_work > a->n_items && !a->join_here) {
         attn8_join_kernel<<<dim3(a->nkv, a->n_items, MANY / 16), THREADS, 0, stream>>>(*a);
         PULSE_LAUNCH_CHECK("attn8_join");
     }

@@ -73,7 +73,7 @@ def _pages(what: str, view: Paged8CacheView, nkv: int, d: int) -> Tuple[int, int
 # The arguments of the entry points as the structures of csrc/cache8_maps.hip, cache8_store.hip and cache8_attn.h, put together at once.
 _MAPS = struct.Struct("@9Q8i")
 _STORE = struct.Struct("@QqQq9Q14i2fQ3q")
-_ATTN = struct.Struct("@QqQq7Qq5Q14i2f")
+_ATTN = struct.Struct("@QqQq7Qq5Q16i2f")
 
 
 def _at(t: Optional[torch.Tensor]) -> int:
@@ -236,16 +236,21 @@ class AttentionPlan:
     layers that are alike in heads, window and chunk.  ``plain``: everything goes to the kernel that serves every size."""
 
     # Workgroups a compute unit that a kernel's keys are shared out over, the fewest tiles of 64 keys of a piece, and how many times the
-    # items there may be pieces in any case.
+    # items there may be pieces in any case.  Of attn8_many's a unit's registers hold three where heads have up to 64 channels (two / three,
+    # us: 2,048 tokens 42 / 34.5, 2 portions of 509 behind 7,000 at 40 heads 133 / 107); attn8_few reads no faster with three (64 contexts of
+    # 4,096 46.5 / 53).
     FEW_SLOTS, FEW_LEAST, FEW_ROUNDS = 2, 8, 2
-    MANY_SLOTS, MANY_LEAST, MANY_ROUNDS = 2, 8, 1
-    # Nothing is cut (and nothing joined) where the items fill the GPU by themselves, two workgroups a unit, and the longest is at most
-    # that many times what a unit's share of them would be.
+    MANY_SLOTS, MANY_NARROW_SLOTS, MANY_LEAST, MANY_ROUNDS = 2, 3, 8, 1
+    # Up to so many pieces an item on the average the last one joins them (in a launch of its own / by the last, us: 1,024 tokens 39 / 28, 3
+    # portions of 300 behind 2,000 59 / 48, 512 behind 8,192 98 / 96; at 10 an item 74 / 109).
+    MANY_HERE = 6
+    # Nothing is cut (and nothing joined) where the items fill the GPU by themselves and the longest is at most that many times what a
+    # workgroup's share of them would be.
     FEW_EVEN, MANY_EVEN = 1.15, 2.2
     # Portions go through attn8_few up to so many columns, and altogether while they walk no more tiles a compute unit for it.  One portion
-    # of 128 rows, 32 heads on 8, many / few, us: from the start 18.1 / 14.4, behind 1,000 tokens 22.9 / 19.0, behind 8,000 41 / 55; of
-    # 40 behind 8,000 28.9 / 28.2; sixteen of 23 behind 1,000 27.7 / 23.6, of 64 39 / 49.
-    FEW_COLUMNS, FEW_WALKS = 32, 48
+    # of 128 rows, 32 heads on 8, many / few, us: from the start 14.2 / 11.6, behind 1,000 tokens 22.4 / 18.7, behind 8,000 42 / 57; of 300
+    # from the start 16.2 / 13.4; of 200 behind 1,000 24.0 / 32.6; of 40 behind 8,000 28.9 / 28.4; sixteen of 64 behind 1,000 31 / 47.
+    FEW_COLUMNS, FEW_WALKS = 32, 24
 
     def __init__(self, entries: Sequence[Any], nq: int, nkv: int, d: int, *, page_size: int, dtype: torch.dtype, window: int = 0,
                  chunk: int = 0, device: Any = "cuda", workspace: Any = None, to_device: Optional[Callable] = None, plain: bool = False):
@@ -265,9 +270,9 @@ class AttentionPlan:
         self.device = torch.device(device)
         self.ready = not self.matrix      # whether the keys have been shared out
         self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, counters an item, cut)
-        self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces)
+        self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces, joined by the last)
         if not self.matrix:
-            self.calls.append(("pulse_attn8_plain", 0, 0, 0, 0, 0))
+            self.calls.append(("pulse_attn8_plain", 0, 0, 0, 0, 0, 0))
             return
         units, group = compute_units(), nq // nkv
         few, many = [], []
@@ -280,29 +285,39 @@ class AttentionPlan:
             to += [(e.start + at, e.first_row + at, min(step, e.count - at), i) for at in range(0, e.count, step)]
         to_device = to_device or (lambda flat: torch.tensor(flat, dtype=torch.int32, device=self.device))
 
-        def add(name: str, columns: int, items: List[Tuple], groups: int, slots: float, least: int, rounds: int, even: float) -> None:
+        def add(name: str, columns: int, items: List[Tuple], groups: int, slots: int, least: int, rounds: int, even: float) -> None:
             n = len(items)
             if not n:
                 return
             tiles = [self._tiles(start, rows) for start, _, rows, _ in items]
-            whole = n * groups >= 2 * units and max(tiles) * 2 * units <= even * sum(tiles) * groups
-            slots = max(1, int(slots * units) // groups, rounds * n)
+            whole = n * groups >= slots * units and max(tiles) * slots * units <= even * sum(tiles) * groups
+            slots = max(1, slots * units // groups, rounds * n)
             room = n if whole else n + slots
             _need(room <= 65535, f"plan: {n} items are too many")
+            if not whole and columns == MANY:      # the longest pieces first, as far as can be told from the starts
+                low = max(least, -(-sum(tiles) // slots))
+                high = max(low, max(tiles))
+                while low < high:                  # (the length that attn8_cut finds)
+                    middle = (low + high) // 2
+                    if sum(-(-t // middle) for t in tiles) <= slots:
+                        high = middle
+                    else:
+                        low = middle + 1
+                items = [it for _, it in sorted(zip(tiles, items), key=lambda x: -(-x[0] // -(-x[0] // low)), reverse=True)]
             on_gpu = to_device([v for _, row, rows, entry in items for v in (row, rows, entry, 0)])
-            counters = n * groups if columns == FEW else 0
+            here = int(columns == FEW or slots <= self.MANY_HERE * n)
+            counters = n * groups if here else 0
             cut = torch.empty(PIECE_INTS * room + 2 * n + counters, dtype=torch.int32, device=self.device)
             self.works.append((on_gpu, n, slots, least, room, counters // n, cut))
-            self.calls.append((name, on_gpu.data_ptr(), cut.data_ptr(), n, room, 0 if whole else room * groups * columns))
+            self.calls.append((name, on_gpu.data_ptr(), cut.data_ptr(), n, room, 0 if whole else room * groups * columns, here))
 
-        add("pulse_attn8_few", FEW, few, groups, self.FEW_SLOTS, self.FEW_LEAST,
-            self.FEW_ROUNDS, self.FEW_EVEN)
+        add("pulse_attn8_few", FEW, few, groups, self.FEW_SLOTS, self.FEW_LEAST, self.FEW_ROUNDS, self.FEW_EVEN)
         # The longest walks first; where two workgroups share a unit, the second ones' from the other end, the shortest beside the longest.
         many.sort(key=lambda it: -it[0])
         first = max(1, units // nkv)
         if first < len(many) <= 2 * first:
             many[first:] = many[:first - 1:-1]
-        add("pulse_attn8_many", MANY, many, nkv, self.MANY_SLOTS, self.MANY_LEAST, self.MANY_ROUNDS, self.MANY_EVEN)
+        add("pulse_attn8_many", MANY, many, nkv, self.MANY_NARROW_SLOTS if d <= 64 else self.MANY_SLOTS, self.MANY_LEAST, self.MANY_ROUNDS, self.MANY_EVEN)
 
     def _tiles(self, start: int, count: int) -> int:
         """Tiles that hold keys of ``count`` tokens from position ``start`` on."""
@@ -388,7 +403,7 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     q_at, out_at = q.data_ptr(), out.data_ptr()
     if plan.matrix and (q_at % 16 or q_stride % 8 or out_at % 8 or o_stride % 4):
         _refuse(what, "rows must be aligned to 16 bytes")
-    for name, items, cut, n_items, room, rows in plan.calls:
+    for name, items, cut, n_items, room, rows, here in plan.calls:
         part_o = part_ml = 0
         if rows:
             if workspace is not None:
@@ -401,5 +416,5 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
         call(name, _ATTN.pack(
             q_at, q_stride, out_at, o_stride, view.keys.data_ptr(), view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(),
             token_entry.data_ptr(), table.data_ptr(), _at(gate), gate_stride, _at(sink), items, cut, part_o, part_ml, plan.tag, plan.rows,
-            shape[0], shape[1], nq, nkv, d, page, pages, plan.window, plan.chunk, gate_width, n_items, room, scale, softcap),
+            shape[0], shape[1], nq, nkv, d, page, pages, plan.window, plan.chunk, gate_width, n_items, room, here, 0, scale, softcap),
             _stream())

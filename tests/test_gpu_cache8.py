@@ -309,10 +309,10 @@ def attend(entries, nq, nkv, d, page, dtype=torch.bfloat16, seed=0, window=0, ch
     token_entry = ints([b for b, (_, c) in enumerate(entries) for _ in range(c)] + [-1] * extra_rows)
     scale = 1.3 * d ** -0.5
     ws = Workspace(torch.device(DEV))
-    # as the plan has it, and every portion that can be in items of 128 columns
-    was, outs = cache8.AttentionPlan.FEW_WALKS, []
+    # as the plan has it, and every portion that can be in items of 128 columns, joined by a launch and by their last pieces
+    was, outs = (cache8.AttentionPlan.FEW_WALKS, cache8.AttentionPlan.MANY_HERE), []
     try:
-        for cache8.AttentionPlan.FEW_WALKS in (was, 0):
+        for cache8.AttentionPlan.FEW_WALKS, cache8.AttentionPlan.MANY_HERE in (was, (0, 0), (0, 10 ** 6)):
             out.fill_(7.0)
             made = cache8.plan(m, nq, nkv, d, positions, page_size=page, dtype=dtype, window=window, chunk=chunk, workspace=ws)
             cache8.attention(q, out, made, view, positions, token_entry, ints(table), scale, gate=gates, gate_width=width_g, sink=sinks,
@@ -320,7 +320,7 @@ def attend(entries, nq, nkv, d, page, dtype=torch.bfloat16, seed=0, window=0, ch
             outs.append(out[:total].cpu().to(F64).reshape(total, nq, d))
             assert not extra_rows or (out[total:] == 7.0).all()
     finally:
-        cache8.AttentionPlan.FEW_WALKS = was
+        cache8.AttentionPlan.FEW_WALKS, cache8.AttentionPlan.MANY_HERE = was
     want, mass, size = plain.attention(q[:total].cpu().to(F64).reshape(total, nq, d), cache, entries, table, scale, window, chunk, softcap,
                                        sinks, gates[:total] if gates is not None else None, width_g, pool)
     bound = bound_of(dtype, d, want, mass, size)
