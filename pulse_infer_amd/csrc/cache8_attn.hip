@@ -17,6 +17,7 @@
 #include "cache8_attn.h"
 
 #include <algorithm>
+#include <type_traits>
 
 int pulse_attn8_check(const PulseAttn8* a, const char* what);
 
@@ -532,19 +533,27 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_few_kernel(Pu
 // channel's 16 tokens), asked for while the tile before is computed, and converts them into the other of two stages.  What is rare (caps,
 // masks, blocks that are not there or hold what is not finite, a maximum that grew) stands behind real branches: left to itself the
 // compiler computes both sides.
+// Heads of 160 to 224 channels take 32 keys at a time, for which a unit's registers hold two workgroups (with 64, one; 2 portions of 600 behind
+// 2,000, 16 heads on 4 of 160 / 192 / 224 channels 80 / 89 / 105 -> 60 / 66 / 83 us).  256 channels have no room for two either way (32
+// keys, spilled: 2,048 tokens 94 -> 99), and up to 128 fewer keys a step cost more than a third workgroup gives (128 channels, 512 tokens behind
+// 8,192 98 -> 106, 2,048 alone 62 -> 58).
+template <int D>
+constexpr bool SMALL_STEPS = D > 128 && D < 256;
 template <int D, bool CAP>
-__global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(PulseAttn8 a, cache8::Div blocks) {
-    constexpr int KROW = D + 8, VROW = TILE + 8;                 // in bfloat16 numbers
-    constexpr int PIECES = 4 * D, TURNS = (PIECES + THREADS - 1) / THREADS, STEPS = D / 16, MT = D / 32;
-    __shared__ __attribute__((aligned(16))) bf16_t s_k[2][TILE * KROW];
+__global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void attn8_many_kernel(PulseAttn8 a, cache8::Div blocks) {
+    constexpr int KEYS = SMALL_STEPS<D> ? 32 : 64, BLOCKS = KEYS / 16, HALVES = KEYS / 32;
+    constexpr int KROW = D + 8, VROW = KEYS + 8;                 // in bfloat16 numbers
+    constexpr int PIECES = BLOCKS * D, TURNS = (PIECES + THREADS - 1) / THREADS, STEPS = D / 16, MT = D / 32;
+    using NoneWord = std::conditional_t<BLOCKS == 4, uint64_t, uint32_t>;
+    __shared__ __attribute__((aligned(16))) bf16_t s_k[2][KEYS * KROW];
     __shared__ __attribute__((aligned(16))) bf16_t s_v[2][D * VROW];
     // the tile + 1 in which something is out of the ordinary; in which a block is not there; in which it holds values that are none, and which
-    __shared__ int s_odd[2], s_gone[2][4], s_bad[2][4];
-    __shared__ __attribute__((aligned(8))) uint16_t s_none[2][D][4];
+    __shared__ int s_odd[2], s_gone[2][BLOCKS], s_bad[2][BLOCKS];
+    __shared__ __attribute__((aligned(8))) uint16_t s_none[2][D][BLOCKS];
     const int w = blockIdx.y;
     const cache8::Piece job = piece_of(a, w);
     if (job.rows <= 0) return;
-    const int row0 = job.row0, ntok = job.rows, entry = job.entry, tile_begin = job.tile, tile_end = tiles_end(a, job, blocks);
+    const int row0 = job.row0, ntok = job.rows, entry = job.entry, begin = job.tile * (TILE / KEYS), end = tiles_end(a, job, blocks) * (TILE / KEYS);
     const bool whole = job.pieces == 1;
     const int g = blockIdx.x, group = a.nq / a.nkv;
     const int tid = threadIdx.x, lane = tid % PULSE_WAVE, wave = uniform(tid / PULSE_WAVE);
@@ -582,11 +591,11 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
         int there[TURNS];      // -1: beyond what the item sees, 0: not there, 1: there
     };
     Spot spot[TURNS];          // of the tile whose pages are asked for next
-    const int page_step = blocks.over(4), rest_step = 4 - page_step * blocks.b;
+    const int page_step = blocks.over(BLOCKS), rest_step = BLOCKS - page_step * blocks.b;
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-        const int in_tile = min((tid + i * THREADS) / D, 3);
-        spot[i].n = 4 * tile_begin + (ONE ? uniform(in_tile) : in_tile);
+        const int in_tile = min((tid + i * THREADS) / D, BLOCKS - 1);
+        spot[i].n = BLOCKS * begin + (ONE ? uniform(in_tile) : in_tile);
         spot[i].page_index = blocks.over(spot[i].n);
         spot[i].rest = spot[i].n - spot[i].page_index * blocks.b;
         spot[i].page = 0;
@@ -598,7 +607,7 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
             to[i] = s;
             to[i].page = read_only<ONE>(bt + min(s.page_index, a.table_width - 1));
             if (s.page_index >= a.table_width) to[i].page = -1;
-            s.n += 4;
+            s.n += BLOCKS;
             s.page_index += page_step;
             s.rest += rest_step;
             if (s.rest >= blocks.b) {
@@ -668,28 +677,28 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
     float top = -INFINITY, l = 0.f;
 
     auto compute = [&](int tile, int stage) __attribute__((always_inline)) {
-        const int j0 = tile * TILE;
-        if (j0 > w_last || j0 + TILE - 1 < w_low) return;       // no column of this wavefront sees a key of the tile
+        const int j0 = tile * KEYS;
+        if (j0 > w_last || j0 + KEYS - 1 < w_low) return;       // no column of this wavefront sees a key of the tile
         const bf16_t* sk = s_k[stage] + r * KROW + 8 * half;
         const bf16_t* sv = s_v[stage] + r * VROW + 8 * half;
         const bool odd = uniform(s_odd[stage]) == tile + 1;
-        constexpr int AHEAD = 4;       // operand reads run that many products ahead
+        constexpr int AHEAD = SMALL_STEPS<D> ? 2 : 4;       // operand reads run that many products ahead
         auto key = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<const bf16x8*>(sk + i / STEPS * (32 * KROW) + i % STEPS * 16); };
-        auto value = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<const bf16x8*>(sv + i / 4 * (32 * VROW) + i % 4 * 16); };
-        bf16x8 ak[2 * STEPS], av[4 * MT];
+        auto value = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<const bf16x8*>(sv + i / BLOCKS * (32 * VROW) + i % BLOCKS * 16); };
+        bf16x8 ak[HALVES * STEPS], av[BLOCKS * MT];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) ak[i] = key(i);
-        f32x16 s[2] = {f32x16{}, f32x16{}};
+        f32x16 s[HALVES] = {};
 #pragma unroll
-        for (int i = 0; i < 2 * STEPS; ++i) {
-            if (i + AHEAD < 2 * STEPS) ak[i + AHEAD] = key(i + AHEAD);
-            else if (i + AHEAD - 2 * STEPS < 4 * MT) av[i + AHEAD - 2 * STEPS] = value(i + AHEAD - 2 * STEPS);
+        for (int i = 0; i < HALVES * STEPS; ++i) {
+            if (i + AHEAD < HALVES * STEPS) ak[i + AHEAD] = key(i + AHEAD);
+            else if (i + AHEAD - HALVES * STEPS < BLOCKS * MT) av[i + AHEAD - HALVES * STEPS] = value(i + AHEAD - HALVES * STEPS);
             s[i / STEPS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ak[i], q[i % STEPS], s[i / STEPS], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (CAP) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < HALVES; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[t][i] = score(s[t][i]);
         }
@@ -700,20 +709,20 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
             const int j = 32 * t + 8 * (i / 4) + i % 4;
             return j >= from && j <= to && !(gone >> (2 * t + i / 8) & 1u);
         };
-        if (j0 + TILE - 1 > w_first || j0 < w_low_last || !w_any || odd) {
+        if (j0 + KEYS - 1 > w_first || j0 < w_low_last || !w_any || odd) {
             asm volatile("");
             if (odd) {
 #pragma unroll
-                for (int b = 0; b < 4; ++b) gone |= (uniform(s_gone[stage][b]) == tile + 1 ? 1u : 0u) << b;
+                for (int b = 0; b < BLOCKS; ++b) gone |= (uniform(s_gone[stage][b]) == tile + 1 ? 1u : 0u) << b;
             }
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < HALVES; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[t][i] = seen(t, i) ? s[t][i] : -INFINITY;
         }
         float best = s[0][0];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < HALVES; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) best = fmaxf(best, s[t][i]);
         const WaveTwo two = wave_two<32>(__float_as_uint(best));
@@ -729,9 +738,9 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
             top = now;
         }
         const float shift = top == -INFINITY ? 0.f : -top;
-        bf16x8 p[4];
+        bf16x8 p[BLOCKS];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < HALVES; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i], score.factor, shift));
@@ -740,25 +749,25 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
             }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 4 * MT; ++i) {
-            if (i + AHEAD < 4 * MT) av[i + AHEAD] = value(i + AHEAD);
-            o[i / 4] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av[i], p[i % 4], o[i / 4], 0, 0, 0);
+        for (int i = 0; i < BLOCKS * MT; ++i) {
+            if (i + AHEAD < BLOCKS * MT) av[i + AHEAD] = value(i + AHEAD);
+            o[i / BLOCKS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av[i], p[i % BLOCKS], o[i / BLOCKS], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (__builtin_expect(odd, 0)) {
             asm volatile("");
             // the keys of the tile that this column sees, and of those the ones whose value in a channel is none
-            const int begin = max(low - j0, 0), end = min(pos - j0 + 1, TILE);
-            uint64_t seen_keys = end > begin ? (~0ull >> (TILE - (end - begin))) << begin : 0ull;
+            const int first = max(low - j0, 0), last = min(pos - j0 + 1, KEYS);
+            uint64_t seen_keys = last > first ? (~0ull >> (64 - (last - first))) << first : 0ull;
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+            for (int b = 0; b < BLOCKS; ++b)
                 if (uniform(s_gone[stage][b]) == tile + 1 || uniform(s_bad[stage][b]) != tile + 1) seen_keys &= ~(0xffffull << (16 * b));
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const uint64_t none = *reinterpret_cast<const uint64_t*>(s_none[stage][32 * m + 8 * (i / 4) + 4 * half + i % 4]);
-                    if (none & seen_keys) o[m][i] = __builtin_nanf("");
+                    const NoneWord none = *reinterpret_cast<const NoneWord*>(s_none[stage][32 * m + 8 * (i / 4) + 4 * half + i % 4]);
+                    if (none & static_cast<NoneWord>(seen_keys)) o[m][i] = __builtin_nanf("");
                 }
         }
     };
@@ -768,15 +777,15 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
         Spot next[TURNS];
         find(next);
         if (tid < 2) s_odd[tid] = 0;
-        if (tid < 8) s_gone[tid / 4][tid % 4] = s_bad[tid / 4][tid % 4] = 0;
+        if (tid < 2 * BLOCKS) s_gone[tid / BLOCKS][tid % BLOCKS] = s_bad[tid / BLOCKS][tid % BLOCKS] = 0;
         __syncthreads();
         load(next, raw);
         find(next);
-        put(raw, 0, tile_begin);
+        put(raw, 0, begin);
         __syncthreads();
         int stage = 0;
-        for (int tile = tile_begin; tile < tile_end; ++tile, stage ^= 1) {
-            const bool more = tile + 1 < tile_end;
+        for (int tile = begin; tile < end; ++tile, stage ^= 1) {
+            const bool more = tile + 1 < end;
             if (more) {
                 load(next, raw);
                 find(next);
@@ -803,37 +812,39 @@ __global__ __launch_bounds__(THREADS, D <= 128 ? 2 : 1) void attn8_many_kernel(P
         float most = top;
         for (int z = 0; z < job.pieces; ++z) most = fmaxf(most, shared2<true>(state_of(z)).x);
         const float shift = most == -INFINITY ? 0.f : most;
-        f32x16 all[MT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) all[m] = f32x16{};
+        constexpr int SOME = D <= 128 ? MT : 1;       // (32 channels at a time: wider heads have no registers for more)
         float sum = 0.f;
-        for (int z = 0; z < job.pieces; ++z) {       // (in their order, whoever came last)
-            const float2 ml = shared2<true>(state_of(z));
-            const float f = __builtin_amdgcn_exp2f(ml.x - shift);
-            sum += ml.y * f;
-            if (z == own) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+        for (int m0 = 0; m0 < MT; m0 += SOME) {
+            f32x16 all[SOME] = {};
+            for (int z = 0; z < job.pieces; ++z) {       // (in their order, whoever came last)
+                const float2 ml = shared2<true>(state_of(z));
+                const float f = __builtin_amdgcn_exp2f(ml.x - shift);
+                if (m0 == 0) sum += ml.y * f;
+                if (z == own) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) all[m][i] = fmaf(o[m][i], f, all[m][i]);
-            } else {
+                    for (int m = 0; m < SOME; ++m)
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    float2 x[8];
+                        for (int i = 0; i < 16; ++i) all[m][i] = fmaf(o[m0 + m][i], f, all[m][i]);
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = shared2<true>(sums_of(z) + (8 * m + i) * (2 * THREADS));
+                    for (int m = 0; m < SOME; ++m) {
+                        float2 x[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        all[m][2 * i] = fmaf(x[i].x, f, all[m][2 * i]);
-                        all[m][2 * i + 1] = fmaf(x[i].y, f, all[m][2 * i + 1]);
+                        for (int i = 0; i < 8; ++i) x[i] = shared2<true>(sums_of(z) + (8 * (m0 + m) + i) * (2 * THREADS));
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            all[m][2 * i] = fmaf(x[i].x, f, all[m][2 * i]);
+                            all[m][2 * i + 1] = fmaf(x[i].y, f, all[m][2 * i + 1]);
+                        }
                     }
                 }
             }
+#pragma unroll
+            for (int m = 0; m < SOME; ++m) o[m0 + m] = all[m];
         }
         top = most;
         l = sum;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) o[m] = all[m];
     }
     if (!col_ok) return;
     if (whole || a.join_here) {
