@@ -237,8 +237,8 @@ class AttentionPlan:
 
     # Workgroups a compute unit that a kernel's keys are shared out over, the fewest tiles of 64 keys of a piece, and how many times the
     # items there may be pieces in any case.  Of attn8_many's a unit's registers hold three where heads have up to 64 channels (two / three,
-    # us: 2,048 tokens 42 / 34.5, 2 portions of 509 behind 7,000 at 40 heads 133 / 107); attn8_few reads no faster with three (64 contexts of
-    # 4,096 46.5 / 53).
+    # us: 2,048 tokens 42 / 34.5, 2 portions of 509 behind 7,000 at 40 heads 133 / 107); pieces for as many in
+    # attn8_few read no faster (64 contexts of 4,096 95 / 104).
     FEW_SLOTS, FEW_LEAST, FEW_ROUNDS = 2, 8, 2
     MANY_SLOTS, MANY_NARROW_SLOTS, MANY_LEAST, MANY_ROUNDS = 2, 3, 8, 1
     # Up to so many pieces an item on the average the last one joins them (in a launch of its own / by the last, us: 1,024 tokens 39 / 28, 3
