@@ -247,6 +247,10 @@ class AttentionPlan:
     # Nothing is cut (and nothing joined) where the items fill the GPU by themselves and the longest is at most that many times what a
     # workgroup's share of them would be.
     FEW_EVEN, MANY_EVEN = 1.15, 2.2
+    # Of attn8_few, where every unit has an item, neither are those whose lengths are (on the GPU, in a step's own positions) within so many
+    # hundredths of their mean, unless some units had two and most one: 32 / 48 / 56 contexts of 4,000, 32 heads on 8 of 128, cut / whole, us: 45.9 /
+    # 42.9, 76.7 / 78.9, 94 / 83 (of 1,000 17.7 / 14.8, 22.3 / 20.7, 27.7 / 21.8); 40 66 / 72; 40 of 64 channels 33.6 / 30.4.
+    FEW_ALIKE = 110
     # Portions go through attn8_few up to so many columns, and altogether while they walk no more tiles a compute unit for it.  One portion
     # of 128 rows, 32 heads on 8, many / few, us: from the start 14.2 / 11.6, behind 1,000 tokens 22.4 / 18.7, behind 8,000 42 / 57; of 300
     # from the start 16.2 / 13.4; of 200 behind 1,000 24.0 / 32.6; of 40 behind 8,000 28.9 / 28.4; sixteen of 64 behind 1,000 31 / 47.
@@ -269,7 +273,7 @@ class AttentionPlan:
         self.matrix = not plain and matrix_cores(d, page_size, dtype)
         self.device = torch.device(device)
         self.ready = not self.matrix      # whether the keys have been shared out
-        self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, counters an item, cut)
+        self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, counters an item, hundredths of the mean, longer pieces, cut)
         self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces, joined by the last)
         if not self.matrix:
             self.calls.append(("pulse_attn8_plain", 0, 0, 0, 0, 0, 0))
@@ -308,7 +312,10 @@ class AttentionPlan:
             here = int(columns == FEW or slots <= self.MANY_HERE * n)
             counters = n * groups if here else 0
             cut = torch.empty(PIECE_INTS * room + 2 * n + counters, dtype=torch.int32, device=self.device)
-            self.works.append((on_gpu, n, slots, least, room, counters // n, cut))
+            # (what the units' turns at n * groups workgroups are above what they would be if these could be shared out evenly)
+            turns = -(-n * groups // units) * units / (n * groups)
+            alike = self.FEW_ALIKE if columns == FEW and n * groups >= units and turns <= (1.7 if d <= 64 else 1.35) else 0
+            self.works.append((on_gpu, n, slots, least, room, counters // n, alike, int(columns == FEW), cut))
             self.calls.append((name, on_gpu.data_ptr(), cut.data_ptr(), n, room, 0 if whole else room * groups * columns, here))
 
         add("pulse_attn8_few", FEW, few, groups, self.FEW_SLOTS, self.FEW_LEAST, self.FEW_ROUNDS, self.FEW_EVEN)
@@ -331,9 +338,9 @@ class AttentionPlan:
         if self.device.index is not None and positions.device != self.device:
             _refuse("plan", f"it was made for {self.device}, the positions lie on {positions.device}")
         self.ready = True
-        for items, n, slots, least, room, groups, cut in self.works:
+        for items, n, slots, least, room, groups, even, shrink, cut in self.works:
             call("pulse_attn8_cut", _ptr(items), _i32(n), _ptr(positions), _i32(self.window), _i32(self.chunk), _i32(slots), _i32(least),
-                 _i32(room), _i32(groups), _ptr(cut), _stream())
+                 _i32(room), _i32(groups), _i32(even), _i32(shrink), _ptr(cut), _stream())
         return self
 
 
