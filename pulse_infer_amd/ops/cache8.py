@@ -252,9 +252,9 @@ class AttentionPlan:
     # 42.9, 76.7 / 78.9, 94 / 83 (of 1,000 17.7 / 14.8, 22.3 / 20.7, 27.7 / 21.8); 40 66 / 72; 40 of 64 channels 33.6 / 30.4.
     FEW_ALIKE = 110
     # Portions go through attn8_few up to so many columns, and altogether while they walk no more tiles a compute unit for it.  One portion
-    # of 128 rows, 32 heads on 8, many / few, us: from the start 14.2 / 11.6, behind 1,000 tokens 22.4 / 18.7, behind 8,000 42 / 57; of 300
-    # from the start 16.2 / 13.4; of 200 behind 1,000 24.0 / 32.6; of 40 behind 8,000 28.9 / 28.4; sixteen of 64 behind 1,000 31 / 47.
-    FEW_COLUMNS, FEW_WALKS = 32, 24
+    # of 128 rows, 32 heads on 8, many / few, us: from the start 14.5 / 11.6, behind 1,000 tokens 22.1 / 12.7, behind 8,000 42.5 / 47; of 200
+    # behind 1,000 23.9 / 19.3, of 240 24.4 / 32.2; of 300 from the start 16.0 / 11.6, of 500 19.6 / 16.6; sixteen of 64 behind 1,000 31 / 40.
+    FEW_COLUMNS, FEW_WALKS = 32, 36
 
     def __init__(self, entries: Sequence[Any], nq: int, nkv: int, d: int, *, page_size: int, dtype: torch.dtype, window: int = 0,
                  chunk: int = 0, device: Any = "cuda", workspace: Any = None, to_device: Optional[Callable] = None, plain: bool = False):
