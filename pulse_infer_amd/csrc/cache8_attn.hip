@@ -1,5 +1,5 @@
-// Attention over a cache in 8 bits (cache8.h) on the matrix cores: bfloat16 rows, heads of a multiple of 32 channels up to 256, pages of a
-// multiple of 16 tokens.  Bytes become bfloat16 on their way into the matrix cores' operands (three bits of fraction: exactly), with the
+// Attention over a cache in 8 bits (cache8.h) on the matrix cores: bfloat16 rows, heads of a multiple of 16 channels from 32 to 128 and of 32 up
+// to 256, pages of a multiple of 16 tokens.  Bytes become bfloat16 on their way into the matrix cores' operands (three bits of fraction: exactly), with the
 // block's scale applied by the same instruction; products, maxima, sums and accumulators are float32.  Weights are rounded to bfloat16
 // for the second product (a relative 2^-8 at most, as q was), the sum that divides them is of the unrounded ones.
 //
@@ -296,7 +296,9 @@ __device__ __forceinline__ void join_columns(const PulseAttn8& a, int first, int
 // b; those are, eight by eight, the numbers of the second product, whose other operand is a channel's 16 bytes of the block.
 template <int D>
 struct Few {
-    static constexpr int K16 = D / 64, K8 = D % 64 / 32, STEPS = D / 32, MT = D / 16;
+    // (What is left behind 64s: 48 channels are three quarters of such a piece, 32 one of 8 bytes a lane, 16 half of that.  The lanes beyond
+    // hold numbers of q that are zero, against others of the key's own row.)
+    static constexpr int LEFT = D % 64, K16 = D / 64 + (LEFT == 48 ? 1 : 0), K8 = LEFT == 16 || LEFT == 32 ? 1 : 0, STEPS = 2 * K16 + K8, MT = D / 16;
     u32x4 k[4][K16 ? K16 : 1];
     uint2 k8[4];
     u32x4 v[MT];
@@ -332,11 +334,12 @@ __global__ __launch_bounds__(THREADS, 2) void attn8_few_kernel(PulseAttn8 a, cac
 #pragma unroll
         for (int j = 0; j < F::K16; ++j)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) q[2 * j + s] = col_ok ? *reinterpret_cast<const bf16x8*>(from + 64 * j + 16 * b + 8 * s) : none;
-        if constexpr (F::K8) q[F::STEPS - 1] = col_ok ? *reinterpret_cast<const bf16x8*>(from + 64 * F::K16 + 8 * b) : none;
+            for (int s = 0; s < 2; ++s) q[2 * j + s] = col_ok && 64 * j + 16 * b < D ? *reinterpret_cast<const bf16x8*>(from + 64 * j + 16 * b + 8 * s) : none;
+        if constexpr (F::K8) q[F::STEPS - 1] = col_ok && 64 * F::K16 + 8 * b < D ? *reinterpret_cast<const bf16x8*>(from + 64 * F::K16 + 8 * b) : none;
     }
     const Score score = score_of(a);
     const int* bt = a.table + static_cast<int64_t>(entry) * a.table_width;
+    const int b_last = F::LEFT == 48 && b == 3 ? 0 : b, b_8 = F::LEFT == 16 ? b % 2 : b;      // (a lane's part of a key's last piece)
 
     // where a tile's blocks lie: of the lane's row (block r / 4) and its own (block b)
     struct Place { int pk, pv; };
@@ -358,8 +361,8 @@ __global__ __launch_bounds__(THREADS, 2) void attn8_few_kernel(PulseAttn8 a, cac
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int j = 0; j < F::K16; ++j) x.k[t][j] = *reinterpret_cast<const u32x4*>(kp + 4 * t * D + 64 * j + 16 * b);
-            if constexpr (F::K8) x.k8[t] = *reinterpret_cast<const uint2*>(kp + 4 * t * D + 64 * F::K16 + 8 * b);
+            for (int j = 0; j < F::K16; ++j) x.k[t][j] = *reinterpret_cast<const u32x4*>(kp + 4 * t * D + 64 * j + 16 * (j == F::K16 - 1 ? b_last : b));
+            if constexpr (F::K8) x.k8[t] = *reinterpret_cast<const uint2*>(kp + 4 * t * D + 64 * F::K16 + 8 * b_8);
         }
 #pragma unroll
         for (int m = 0; m < F::MT; ++m) x.v[m] = *reinterpret_cast<const u32x4*>(vp + m * 256);
@@ -545,13 +548,13 @@ template <int D, bool CAP>
 __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void attn8_many_kernel(PulseAttn8 a, cache8::Div blocks) {
     constexpr int KEYS = SMALL_STEPS<D> ? 32 : 64, BLOCKS = KEYS / 16, HALVES = KEYS / 32;
     constexpr int KROW = D + 8, VROW = KEYS + 8;                 // in bfloat16 numbers
-    constexpr int PIECES = BLOCKS * D, TURNS = (PIECES + THREADS - 1) / THREADS, STEPS = D / 16, MT = D / 32;
+    constexpr int PIECES = BLOCKS * D, TURNS = (PIECES + THREADS - 1) / THREADS, STEPS = D / 16, MT = (D + 31) / 32;
     using NoneWord = std::conditional_t<BLOCKS == 4, uint64_t, uint32_t>;
     __shared__ __attribute__((aligned(16))) bf16_t s_k[2][KEYS * KROW];
-    __shared__ __attribute__((aligned(16))) bf16_t s_v[2][D * VROW];
+    __shared__ __attribute__((aligned(16))) bf16_t s_v[2][MT * 32 * VROW];      // (of 16 channels too many nothing is kept)
     // the tile + 1 in which something is out of the ordinary; in which a block is not there; in which it holds values that are none, and which
     __shared__ int s_odd[2], s_gone[2][BLOCKS], s_bad[2][BLOCKS];
-    __shared__ __attribute__((aligned(8))) uint16_t s_none[2][D][BLOCKS];
+    __shared__ __attribute__((aligned(8))) uint16_t s_none[2][MT * 32][BLOCKS];
     const int w = blockIdx.y;
     const cache8::Piece job = piece_of(a, w);
     if (job.rows <= 0) return;
@@ -808,7 +811,8 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void attn8_many_kernel(Pu
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) share2(sums_of(own) + (8 * m + i) * (2 * THREADS), o[m][2 * i], o[m][2 * i + 1]);
+            for (int i = 0; i < 8; ++i)
+                if (32 * m + 8 * (i / 2) < D) share2(sums_of(own) + (8 * m + i) * (2 * THREADS), o[m][2 * i], o[m][2 * i + 1]);
         if (half == 0) share2(state_of(own), top, l);
         if (!arrive_last(a, job, gridDim.x, blockIdx.x)) return;
         float most = top;
@@ -831,9 +835,10 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void attn8_many_kernel(Pu
                 } else {
 #pragma unroll
                     for (int m = 0; m < SOME; ++m) {
-                        float2 x[8];
+                        float2 x[8] = {};
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = shared2<true>(sums_of(z) + (8 * (m0 + m) + i) * (2 * THREADS));
+                        for (int i = 0; i < 8; ++i)
+                            if (32 * (m0 + m) + 8 * (i / 2) < D) x[i] = shared2<true>(sums_of(z) + (8 * (m0 + m) + i) * (2 * THREADS));
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             all[m][2 * i] = fmaf(x[i].x, f, all[m][2 * i]);
@@ -862,14 +867,14 @@ __global__ __launch_bounds__(THREADS, D < 256 ? 2 : 1) void attn8_many_kernel(Pu
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4 && 32 * m + 8 * c < D; ++c)
                 store4(to + 32 * m + 8 * c + 4 * half, f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]}, [&](int) { return inv; });
     } else {
         const int64_t at = (static_cast<int64_t>(w) * gridDim.x + blockIdx.x) * MANY + col;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4 && 32 * m + 8 * c < D; ++c)
                 *reinterpret_cast<f32x4*>(a.part_o + at * D + 32 * m + 8 * c + 4 * half) =
                     f32x4{o[m][4 * c], o[m][4 * c + 1], o[m][4 * c + 2], o[m][4 * c + 3]};
         if (half == 0) {
@@ -893,8 +898,8 @@ __global__ __launch_bounds__(THREADS) void attn8_join_kernel(PulseAttn8 a) {
 
 int check_matrix(const PulseAttn8* a, const char* what) {
     if (int rc = pulse_attn8_check(a, what)) return rc;
-    PULSE_REQUIRE(a->dtype == PULSE_BF16 && a->d % 32 == 0 && a->d <= 256 && a->page_size % cache8::BLOCK == 0,
-                  "%s: bfloat16 rows, heads of a multiple of 32 channels up to 256 and pages of a multiple of 16 tokens are served", what);
+    PULSE_REQUIRE(a->dtype == PULSE_BF16 && a->d % 16 == 0 && a->d >= 32 && (a->d % 32 == 0 || a->d < 128) && a->d <= 256 && a->page_size % cache8::BLOCK == 0,
+                  "%s: bfloat16 rows, heads of a multiple of 16 channels from 32 to 128, of 32 up to 256, and pages of a multiple of 16 tokens are served", what);
     PULSE_REQUIRE(static_cast<int64_t>(a->num_pages) * a->nkv * (a->page_size / cache8::BLOCK) <= 0x7fffffff, "%s: too many pages", what);
     PULSE_REQUIRE(a->items && a->cut && a->n_items > 0 && a->max_work > 0 && a->max_work <= 65535 && a->n_items <= 65535, "%s: bad work list", what);
     PULSE_REQUIRE(a->q_stride % 8 == 0 && a->o_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a->q) & 15) == 0 &&
@@ -907,8 +912,11 @@ template <typename F>
 int by_width(int d, F go) {
     switch (d) {
         case 32: go(std::integral_constant<int, 32>()); break;
+        case 48: go(std::integral_constant<int, 48>()); break;
         case 64: go(std::integral_constant<int, 64>()); break;
+        case 80: go(std::integral_constant<int, 80>()); break;
         case 96: go(std::integral_constant<int, 96>()); break;
+        case 112: go(std::integral_constant<int, 112>()); break;
         case 128: go(std::integral_constant<int, 128>()); break;
         case 160: go(std::integral_constant<int, 160>()); break;
         case 192: go(std::integral_constant<int, 192>()); break;

@@ -7,8 +7,8 @@
 // A lane takes a key's score (its row of bytes in pieces of 16) and then channels of the sum, for which the weights come as scalars.
 // A row that sees no key is zeros; a row of no entry (token_entry outside the table) is left as it is.  Keys and values that a row does
 // not see are not multiplied, so that what is not finite stays with those who see it.
-// It serves what the matrix-core kernels do not: float32 rows, heads that are no multiple of 32 channels, pages that are no multiple
-// of 16 tokens.
+// It serves what the matrix-core kernels do not: float32 rows, heads that are no multiple of 16 channels from 32 on (of 32 above 128), pages that are
+// no multiple of 16 tokens.
 #include "cache8_attn.h"
 
 namespace {

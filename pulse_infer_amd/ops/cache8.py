@@ -227,7 +227,7 @@ def store_takes_parts(qkv: torch.Tensor, d: int, rotary_dim: int, page_size: int
 # --------------------------------------------------------------------------------------------------------- the attention
 def matrix_cores(d: int, page_size: int, dtype: torch.dtype) -> bool:
     """Whether attention runs on the matrix cores; anything else goes to the kernel that serves every size."""
-    return dtype == torch.bfloat16 and d % 32 == 0 and d <= 256 and page_size % 16 == 0
+    return dtype == torch.bfloat16 and d % 16 == 0 and 32 <= d <= 256 and (d % 32 == 0 or d < 128) and page_size % 16 == 0
 
 
 class AttentionPlan:
@@ -236,7 +236,7 @@ class AttentionPlan:
     layers that are alike in heads, window and chunk.  ``plain``: everything goes to the kernel that serves every size."""
 
     # Workgroups a compute unit that a kernel's keys are shared out over, the fewest tiles of 64 keys of a piece, and how many times the
-    # items there may be pieces in any case.  Of attn8_many's a unit's registers hold three where heads have up to 64 channels (two / three,
+    # items there may be pieces in any case.  Of attn8_many's a unit's registers hold three where heads have 32 or 64 channels (two / three,
     # us: 2,048 tokens 42 / 34.5, 2 portions of 509 behind 7,000 at 40 heads 133 / 107); pieces for as many in
     # attn8_few read no faster (64 contexts of 4,096 95 / 104).
     FEW_SLOTS, FEW_LEAST, FEW_ROUNDS = 2, 8, 2
@@ -324,7 +324,7 @@ class AttentionPlan:
         first = max(1, units // nkv)
         if first < len(many) <= 2 * first:
             many[first:] = many[:first - 1:-1]
-        add("pulse_attn8_many", MANY, many, nkv, self.MANY_NARROW_SLOTS if d <= 64 else self.MANY_SLOTS, self.MANY_LEAST, self.MANY_ROUNDS, self.MANY_EVEN)
+        add("pulse_attn8_many", MANY, many, nkv, self.MANY_NARROW_SLOTS if d in (32, 64) else self.MANY_SLOTS, self.MANY_LEAST, self.MANY_ROUNDS, self.MANY_EVEN)
 
     def _tiles(self, start: int, count: int) -> int:
         """Tiles that hold keys of ``count`` tokens from position ``start`` on."""

@@ -336,10 +336,25 @@ ONE = [(0, 1), (1, 1), (15, 1), (16, 1), (62, 1), (63, 1), (64, 1), (200, 1)]
 MIX = [(0, 1), (0, 5), (40, 3), (0, 33), (130, 70), (17, 1)]
 
 
-@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128, 144, 160, 192, 224, 256])
 def test_attention_head_sizes(d):
     attend(ONE, 4, 2, d, 16)
     attend(MIX, 4, 2, d, 16, seed=1)
+
+
+@pytest.mark.parametrize("d", [48, 80, 112])
+def test_attention_of_heads_that_end_inside_an_operand(d):
+    """Heads whose channels do not fill the last operand: keys and values that are not finite reach their own heads and channels only."""
+    def spoil(k, v, rows, page):
+        k[rows[3][130 // page] * page + 130 % page, 0, :] = math.nan      # a key of one head that rows of request 3 see from position 130 on
+        v[rows[5][9 // page] * page + 9 % page, 1, d - 1] = math.nan      # the last channel of the other head
+
+    entries = [(700, 1), (0, 150), (63, 1), (100, 64), (5, 1), (9, 1)]
+    got, _ = attend(entries, 6, 2, d, 32, seed=21, spoil=spoil, gate=16, sink=True)
+    bad = torch.isnan(got)
+    assert bad[182:216, :3].all() and not bad[182:216, 3:].any() and not bad[:182].any() and not bad[216].any()
+    assert bad[217, 3:, d - 1].all() and not bad[217, :, :d - 1].any() and not bad[217, :3].any()
+    attend([(900, 1), (1300, 300)], 8, 1, d, 16, seed=22, window=500, pad=8)
 
 
 @pytest.mark.parametrize("nq,nkv", [(1, 1), (3, 3), (6, 2), (7, 1), (16, 1), (20, 1), (32, 2), (33, 1), (130, 1)])
