@@ -1,4 +1,4 @@
-// Attention over a cache in 8 bits (cache8.h) for every size and storage type: a workgroup a (row, head), its four wavefronts share the
+// Attention over a cache in 8 bits (cache8.h) for every size and storage type: a workgroup a (row, head), its wavefronts share the
 // keys, float32 throughout.
 //
 //   s_j = scale * q . k_j, capped: cap * tanh(s_j / cap);  seen: low <= j <= position, in pages that are there
@@ -7,13 +7,15 @@
 // A lane takes a key's score (its row of bytes in pieces of 16) and then channels of the sum, for which the weights come as scalars.
 // A row that sees no key is zeros; a row of no entry (token_entry outside the table) is left as it is.  Keys and values that a row does
 // not see are not multiplied, so that what is not finite stays with those who see it.
+// Bound by trips to memory (keys, then values, a wavefront's 64 keys at a time) and, with many rows, by its own arithmetic: nothing is shared
+// between rows (280 rows of up to 90 keys, 6 heads of 32, float32, 8.0 us; 24 tokens behind up to 2,000, pages of 8, 42).
 // It serves what the matrix-core kernels do not: float32 rows, heads that are no multiple of 16 channels from 32 on (of 32 above 128), pages that are
 // no multiple of 16 tokens.
 #include "cache8_attn.h"
 
 namespace {
 
-constexpr int THREADS = 256, WAVES = THREADS / PULSE_WAVE, MAX_DIM = 512;
+constexpr int MAX_DIM = 512;
 
 __device__ __forceinline__ float of_lane(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
 
@@ -22,8 +24,9 @@ __device__ __forceinline__ uint32_t spread(uint32_t bits) { return ((bits * 0x00
 
 // CH: channels a lane sums.  WIDE: heads of a multiple of 16 channels, a key's row in pieces of 16 bytes.  VQ: tokens of a channel that are
 // read together: 16 (blocks of 16), 4 (blocks of a multiple of 4) or 1.
-template <typename T, int CH, bool WIDE, int VQ>
-__global__ __launch_bounds__(THREADS) void attn8_plain_kernel(PulseAttn8 a) {
+template <typename T, int CH, bool WIDE, int VQ, int WAVES>
+__global__ __launch_bounds__(WAVES * PULSE_WAVE) void attn8_plain_kernel(PulseAttn8 a) {
+    constexpr int THREADS = WAVES * PULSE_WAVE;
     __shared__ __attribute__((aligned(16))) float s_q[MAX_DIM];
     __shared__ float s_o[WAVES][MAX_DIM];
     __shared__ float s_m[WAVES], s_l[WAVES];
@@ -59,6 +62,7 @@ __global__ __launch_bounds__(THREADS) void attn8_plain_kernel(PulseAttn8 a) {
         float s = 0.f;
         const uint8_t* k = a.keys + (head * a.page_size + slot) * d;
         if constexpr (WIDE) {
+#pragma unroll 4
             for (int c = 0; c < d; c += 16) {
                 const uint4 u = *reinterpret_cast<const uint4*>(k + c);
                 const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -91,37 +95,49 @@ __global__ __launch_bounds__(THREADS) void attn8_plain_kernel(PulseAttn8 a) {
         // (VQ keys from a multiple of VQ on are of one block: the first that is seen says where it lies)
         const uint32_t place_lo = static_cast<uint32_t>(bn), place_hi = static_cast<uint32_t>(bn >> 32);
         const int in_block = slot % block;
-        for (int b = 0; b < PULSE_WAVE; b += VQ) {
-            const uint32_t some = static_cast<uint32_t>(seen_keys >> b) & ((1u << VQ) - 1u);
-            if (!some) continue;
-            const int one = b + __builtin_ctz(some);
-            const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(place_hi, one))) << 32 |
-                                                    static_cast<uint32_t>(__builtin_amdgcn_readlane(place_lo, one)));
-            const uint8_t* v = a.values + at * block * d + (__builtin_amdgcn_readlane(in_block, one) - (one - b));
-            float w[VQ];
+        // so many groups of VQ keys are asked for together (a trip to memory for all of them, registers allowing)
+        constexpr int WORDS = VQ < 4 ? 1 : VQ / 4, SOME = WORDS * CH >= 16 ? 1 : 16 / (WORDS * CH) < 8 ? 16 / (WORDS * CH) : 8;
+        constexpr uint64_t MASK = SOME * VQ >= 64 ? ~0ull : (1ull << (SOME * VQ % 64)) - 1;
+        const int any = __builtin_ctzll(seen_keys);
+        for (int b0 = 0; b0 < PULSE_WAVE; b0 += SOME * VQ) {
+            if (!(seen_keys >> b0 & MASK)) continue;
+            uint32_t bytes[SOME][CH][WORDS], some[SOME];
 #pragma unroll
-            for (int e = 0; e < VQ; ++e) w[e] = of_lane(pv, b + e);
+            for (int u = 0; u < SOME; ++u) {
+                const int b = b0 + u * VQ;
+                some[u] = static_cast<uint32_t>(seen_keys >> b) & ((1u << VQ) - 1u);
+                const int one = some[u] ? b + __builtin_ctz(some[u]) : any;      // (none is seen: others are read, and count as zeros)
+                const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(place_hi, one))) << 32 |
+                                                        static_cast<uint32_t>(__builtin_amdgcn_readlane(place_lo, one)));
+                const uint8_t* v = a.values + at * block * d + (__builtin_amdgcn_readlane(in_block, one) & ~(VQ - 1));
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int c = lane + i * PULSE_WAVE;
-                const uint8_t* from = v + static_cast<int64_t>(c < d ? c : 0) * block;
-                if constexpr (VQ == 1) {
-                    acc[i] += w[0] * cache8::from_e4m3(*from);
-                } else {
-                    uint32_t bytes[VQ / 4];
+                for (int i = 0; i < CH; ++i) {
+                    const int c = lane + i * PULSE_WAVE;
+                    const uint8_t* from = v + static_cast<int64_t>(c < d ? c : 0) * block;
                     if constexpr (VQ == 16) {
-                        const uint4 u = *reinterpret_cast<const uint4*>(from);
-                        bytes[0] = u.x, bytes[1] = u.y, bytes[2] = u.z, bytes[3] = u.w;
+                        const uint4 w = *reinterpret_cast<const uint4*>(from);
+                        bytes[u][i][0] = w.x, bytes[u][i][1] = w.y, bytes[u][i][2] = w.z, bytes[u][i][3] = w.w;
+                    } else if constexpr (VQ == 4) {
+                        bytes[u][i][0] = *reinterpret_cast<const uint32_t*>(from);
                     } else {
-                        bytes[0] = *reinterpret_cast<const uint32_t*>(from);
+                        bytes[u][i][0] = *from;
                     }
+                }
+            }
 #pragma unroll
-                    for (int e = 0; e < VQ / 4; ++e) {
+            for (int u = 0; u < SOME; ++u) {
+                float w[VQ];
+#pragma unroll
+                for (int e = 0; e < VQ; ++e) w[e] = of_lane(pv, b0 + u * VQ + e);
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+#pragma unroll
+                    for (int e = 0; e < WORDS; ++e) {
                         float x[4];
                         // what is not seen is not multiplied: its bytes are zeros (a block that is seen whole keeps its own)
-                        cache8::from_e4m3x4(bytes[e] & spread(some >> (4 * e) & 15u), x);
+                        cache8::from_e4m3x4(bytes[u][i][e] & spread(some[u] >> (4 * e) & 15u), x);
 #pragma unroll
-                        for (int f = 0; f < 4; ++f) acc[i] += w[4 * e + f] * x[f];
+                        for (int f = 0; f < (VQ < 4 ? 1 : 4); ++f) acc[i] += w[VQ < 4 ? 0 : 4 * e + f] * x[f];
                     }
                 }
             }
@@ -177,8 +193,13 @@ extern "C" int pulse_attn8_plain(const PulseAttn8* a, hipStream_t stream) {
     PULSE_REQUIRE(a->nq <= 65535, "attn8_plain: too many heads");
     if (a->tokens == 0) return 0;
     const int block = cache8::block_tokens(a->page_size);
+    // Few rows: as many wavefronts as a workgroup can have share a row's keys, so that each walks a quarter (a token behind 2,000, 32 heads on 8
+    // of 128, us: pages of 8 40.5 -> 20, float32 rows 25.4 -> 15.4; the same for more rows than fill the GPU, 18.5 for 10.5 at 1,700).
+    const bool few = static_cast<int64_t>(a->tokens) * a->nq <= 512;
     auto go = [&](auto t, auto ch, auto wide, auto vq) {
-        attn8_plain_kernel<decltype(t), decltype(ch)::value, decltype(wide)::value, decltype(vq)::value><<<dim3(a->tokens, a->nq), THREADS, 0, stream>>>(*a);
+        const dim3 grid(a->tokens, a->nq);
+        if (few) attn8_plain_kernel<decltype(t), decltype(ch)::value, decltype(wide)::value, decltype(vq)::value, 16><<<grid, 16 * PULSE_WAVE, 0, stream>>>(*a);
+        else attn8_plain_kernel<decltype(t), decltype(ch)::value, decltype(wide)::value, decltype(vq)::value, 4><<<grid, 4 * PULSE_WAVE, 0, stream>>>(*a);
     };
     auto by_block = [&](auto t, auto ch, auto wide) {
         if (block == 16) go(t, ch, wide, std::integral_constant<int, 16>());
