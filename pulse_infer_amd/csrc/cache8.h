@@ -2,8 +2,9 @@
 //
 // Pages of `page_size` tokens.  A block is 16 tokens of a page, the whole page where 16 does not divide its size.  Of a (block, kv
 // head) the keys have one scale and the values one, powers of two: s = 2^e with the least e >= LEAST for which every finite |x| that
-// the block holds is at most 448 s (448: the largest e4m3 number).  A byte is the e4m3 number nearest to x / s, ties to even; what is
-// not finite is kept as NaN, and a block whose values hold one says so by a negative scale.
+// the block holds is at most 448 s (448: the largest e4m3 number).  A byte is the e4m3 number nearest to x / s, ties to even (with e = 120, the
+// greatest, of those up to 240: 256 s is no float32 number any more, and less than 256 s is off by less than 2^-4 of itself); what is not finite
+// is kept as NaN, and a block whose values hold one says so by a negative scale.
 //   keys   [page, head, token, channel]
 //   values [page, head, block, channel, token]   16 bytes: a channel's tokens of a block, a matrix-core operand's own order
 //   scales [page, head, block, (key, value)]     float32
@@ -16,6 +17,7 @@
 namespace cache8 {
 
 constexpr int LEAST = -118;        // 2^-118 and 2^118 are normal float32 numbers, and 2^-118 times the smallest e4m3 number is none that matters
+constexpr int MOST = 120;          // of the largest float32 numbers
 constexpr int BLOCK = 16;
 
 __host__ __device__ inline int block_tokens(int page_size) { return page_size % BLOCK == 0 ? BLOCK : page_size; }
@@ -39,6 +41,13 @@ __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
     return both | (finite(lo) ? 0u : 0x7fu) | (finite(hi) ? 0u : 0x7f00u);
 }
 __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) { return to_e4m3x2(a, b) | (to_e4m3x2(c, d) << 16); }
+
+// Bytes of a block of exponent e: 240 where 256 (0x78, the largest there) would stand, if 256 * 2^e is no float32 number.
+__device__ __forceinline__ uint32_t at_exponent(int e, uint32_t w) {
+    if (e < MOST) return w;
+    const uint32_t apart = (w & 0x7f7f7f7fu) ^ 0x78787878u;
+    return w - ((~(apart + 0x7f7f7f7fu) & 0x80808080u) >> 7);
+}
 
 // What four bytes stand for, before the scale.
 __device__ __forceinline__ void from_e4m3x4(uint32_t b, float (&out)[4]) {

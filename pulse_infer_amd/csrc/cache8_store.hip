@@ -347,8 +347,8 @@ __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T*
                 hi = cache8::to_e4m3x4(kx[n][2] * by_k, ky[n][2] * by_k, kx[n][3] * by_k, ky[n][3] * by_k);
             }
             uint8_t* to = j.keys + (j.at + i) * d;
-            *reinterpret_cast<uint32_t*>(to + first) = lo;
-            *reinterpret_cast<uint32_t*>(to + second) = hi;
+            *reinterpret_cast<uint32_t*>(to + first) = cache8::at_exponent(ek, lo);
+            *reinterpret_cast<uint32_t*>(to + second) = cache8::at_exponent(ek, hi);
         }
         const int qd = quad + n * quads_at_once;
         if (quad < quads_at_once && qd < 4) {
@@ -360,8 +360,8 @@ __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T*
                 if (grew_v) x = cache8::moved(x, down_v), y = cache8::moved(y, down_v);
                 x = (x & ~fill) | (cache8::to_e4m3x4(vx[n][0] * by_v, vx[n][1] * by_v, vx[n][2] * by_v, vx[n][3] * by_v) & fill);
                 y = (y & ~fill) | (cache8::to_e4m3x4(vy[n][0] * by_v, vy[n][1] * by_v, vy[n][2] * by_v, vy[n][3] * by_v) & fill);
-                *reinterpret_cast<uint32_t*>(j.values + vc * 16 + qd * 4) = x;
-                *reinterpret_cast<uint32_t*>(j.values + vc * 16 + 16 + qd * 4) = y;
+                *reinterpret_cast<uint32_t*>(j.values + vc * 16 + qd * 4) = cache8::at_exponent(ev, x);
+                *reinterpret_cast<uint32_t*>(j.values + vc * 16 + 16 + qd * 4) = cache8::at_exponent(ev, y);
             }
         }
     }
@@ -442,14 +442,14 @@ __global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out,
             int ia, ib;
             channels_of(a, 4 * c + e, ia, ib);
             if (2 * (4 * c + e) < d) {
-                const uint32_t both = cache8::to_e4m3x2(x[e] * by_k, y[e] * by_k);
+                const uint32_t both = cache8::at_exponent(ek, cache8::to_e4m3x2(x[e] * by_k, y[e] * by_k));
                 to[ia] = static_cast<uint8_t>(both);
                 to[ib] = static_cast<uint8_t>(both >> 8);
             }
         }
     }
     for (int i = vg; i < j.rows && vg < groups; i += groups) {
-        const uint32_t both = cache8::to_e4m3x2(to_f32<T>(vrow[i * a.row_stride]) * by_v, to_f32<T>(vrow[i * a.row_stride + 1]) * by_v);
+        const uint32_t both = cache8::at_exponent(ev, cache8::to_e4m3x2(to_f32<T>(vrow[i * a.row_stride]) * by_v, to_f32<T>(vrow[i * a.row_stride + 1]) * by_v));
         uint8_t* to = j.values + static_cast<int64_t>(vc) * a.block + j.at + i;
         to[0] = static_cast<uint8_t>(both);
         to[a.block] = static_cast<uint8_t>(both >> 8);

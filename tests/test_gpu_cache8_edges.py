@@ -1,0 +1,83 @@
+"""A cache of keys and values in 8 bits at its edges: the largest numbers, the last positions, calls without rows, rows that overlap, other
+streams.  Tolerances are those of test_gpu_cache8.py, from whose plain forms the expected values come."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import require_gpu
+from plain import cache8_plain as plain
+from test_gpu_cache8 import DEV, F64, bound_of, ints, metas, view_of
+
+pytestmark = pytest.mark.gpu
+
+
+def held(view, page):
+    """The plain cache that holds what the kernels' cache holds."""
+    pages, nkv, _, d = view.keys.shape
+    cache = plain.Cache(pages, nkv, page, d)
+    cache.x[0].copy_(plain.decode(view.keys).view(cache.x[0].shape))
+    cache.x[1].copy_(plain.decode(view.values).transpose(3, 4))
+    cache.e.copy_(torch.log2(view.scales.cpu().to(F64).abs()))
+    return cache
+
+
+# --------------------------------------------------------------------------------------------------- the largest numbers
+LARGE = [torch.finfo(torch.bfloat16).max, 248.0 * 2.0 ** 120, 247.0 * 2.0 ** 120, -255.0 * 2.0 ** 120, 225.0 * 2.0 ** 120]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page", [16, 20])
+def test_store_of_the_largest_numbers(dtype, page):
+    """At the greatest exponent the largest byte is 240's, in a block that is begun and in one whose earlier bytes move: nothing stands for more
+    than a float32 number, and everything is within 2^-4 of what came."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    d = 32
+    view = view_of(plain.Cache(2, 1, page, d))
+    x = torch.randn((page + 3, 3 * d), generator=torch.Generator().manual_seed(0)).to(dtype)
+    for i, v in enumerate(LARGE):
+        x[i, d + i], x[i + 4, 2 * d + 7 + i], x[page + 2, d + 3 * i], x[page + 2, 2 * d + 5 * i] = v, v, -v, v
+    if dtype == torch.float32:
+        x[page + 1, d + 20] = torch.finfo(torch.float32).max
+    dev = x.to(DEV)
+    for first, rows, block, at in ((0, page, 1, 0), (page, 2, 0, 0), (page + 2, 1, 0, 2)):
+        cache8.store(dev[first:first + rows], torch.empty((rows, d), dtype=dtype, device=DEV), 1, 1, d, view, ints([0] * rows), ints([[0, rows, block, at]]))
+    cache = held(view, page)
+    assert (view.scales == 2.0 ** 120).all()      # (every block holds one of them, and none that is not finite)
+    keys, values = (c[:, 0, :].to(F64) for c in (cache.x[0][:, :, 0] * 2.0 ** 120, cache.x[1][:, :, 0] * 2.0 ** 120))
+    for got, first in ((keys, d), (values, 2 * d)):
+        want = x[:, first:first + d].to(F64)
+        got = torch.cat([got[1], got[0, :3]])
+        assert (got.abs() <= 240 * 2.0 ** 120).all() and (got.abs() == 240 * 2.0 ** 120).any()
+        assert ((got - want).abs() <= 2.0 ** -4 * want.abs())[want.abs() > 1.0e38].all()
+
+
+@pytest.mark.parametrize("d,page", [(32, 16), (64, 32), (128, 16), (192, 16)])
+@pytest.mark.parametrize("few", [True, False])
+def test_the_largest_numbers_stay_with_those_who_see_them(d, page, few, monkeypatch):
+    """bfloat16's largest number as a value and as a key: rows before it are what they are without it."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    nq, nkv, rows, at = 4, 2, 45, 30
+    if not few:
+        monkeypatch.setattr(cache8.AttentionPlan, "FEW_WALKS", 0)
+    view = view_of(plain.Cache(4, nkv, page, d))
+    g = torch.Generator().manual_seed(d)
+    qkv = torch.randn((rows, (nq + 2 * nkv) * d), generator=g)
+    qkv[at, (nq + nkv) * d + 3] = qkv[at + 2, nq * d + d + 5] = torch.finfo(torch.bfloat16).max
+    qkv[at, nq * d + 1] = -torch.finfo(torch.bfloat16).max
+    qkv = qkv.to(torch.bfloat16).to(DEV)
+    positions = ints(list(range(rows)))
+    pages = [3, 1, 0][:-(-rows // page)]
+    want = plain.maps([(0, rows)], pages, page, 4, 3)
+    q, out = (torch.zeros((rows, nq * d), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    cache8.store(qkv, q, nq, nkv, d, view, positions, ints(want["blocks"]))
+    made = cache8.plan(metas([(0, rows)]), nq, nkv, d, positions, page_size=page, dtype=torch.bfloat16)
+    cache8.attention(q, out, made, view, positions, ints([0] * rows), ints(want["table"]), d ** -0.5)
+    ref, mass, size = plain.attention(q[:at].cpu().to(F64).view(at, nq, d), held(view, page), [(0, at)], want["table"], d ** -0.5)
+    got = out[:at].cpu().to(F64).view(at, nq, d)
+    assert torch.isfinite(got).all()
+    assert ((got - ref).abs() <= bound_of(torch.bfloat16, d, ref, mass, size) + 1e-12).all()
