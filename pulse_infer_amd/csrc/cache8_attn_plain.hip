@@ -41,7 +41,7 @@ __global__ __launch_bounds__(WAVES * PULSE_WAVE) void attn8_plain_kernel(PulseAt
     for (int c = tid; c < MAX_DIM; c += THREADS) s_q[c] = c < d ? to_f32<T>(q[c]) : 0.f;
     __syncthreads();
     const int block = cache8::block_tokens(a.page_size), nb = a.page_size / block;
-    const int lo = cache8::low_key(a.window, a.chunk, a.positions[row]);
+    const int lo = max(0, min(cache8::low_key(a.window, a.chunk, a.positions[row]), pos + 1));      // (so that no wavefront's first key leaves 32 bits)
     const int* bt = a.table + static_cast<int64_t>(entry) * a.table_width;
     float m = -INFINITY, l = 0.f, acc[CH];
 #pragma unroll

@@ -81,3 +81,34 @@ def test_the_largest_numbers_stay_with_those_who_see_them(d, page, few, monkeypa
     got = out[:at].cpu().to(F64).view(at, nq, d)
     assert torch.isfinite(got).all()
     assert ((got - ref).abs() <= bound_of(torch.bfloat16, d, ref, mass, size) + 1e-12).all()
+
+
+# ------------------------------------------------------------------------------------------------------ the last positions
+@pytest.mark.parametrize("d,page,dtype", [(32, 20, torch.bfloat16), (64, 16, torch.float32), (300, 16, torch.bfloat16), (32, 16, torch.bfloat16), (128, 32, torch.bfloat16)])
+@pytest.mark.parametrize("window,chunk", [(5, 0), (700, 0), (0, 48), (2 ** 31 - 1, 0), (2 ** 31 - 100, 0), (0, 2 ** 30)])
+@pytest.mark.parametrize("rows,back", [(1, 0), (40, 0), (600, 300), (1, 3000)])
+def test_attention_of_the_last_positions_behind_a_mask(d, page, dtype, window, chunk, rows, back):
+    """Rows at the last positions that 32 bits have, whose window or chunk begins behind the table (rows of zeros) or reaches into it."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    pages, start = 9, 2 ** 31 - rows - back
+    cache = plain.Cache(pages, 2, page, d)
+    x = torch.randn((pages * page, 2, d), generator=torch.Generator().manual_seed(5), dtype=F64)
+    cache.store(x, x.flip(0), [[i * cache.block, cache.block, i, 0] for i in range(pages * cache.nb)])
+    q = torch.randn((rows, 4 * d), generator=torch.Generator().manual_seed(6)).to(dtype).to(DEV)
+    positions = torch.arange(start, start + rows, dtype=torch.int64)
+    low = positions // chunk * chunk if chunk else (positions - window + 1).clamp_min(0)
+    made = cache8.plan(metas([(start, rows)]), 4, 2, d, positions.to(torch.int32).to(DEV), page_size=page, dtype=dtype, window=window, chunk=chunk)
+    out = torch.full_like(q, 7.0)
+    cache8.attention(q, out, made, view_of(cache), positions.to(torch.int32).to(DEV), ints([0] * rows), ints([list(range(pages))]), d ** -0.5)
+    got = out.cpu().to(F64).reshape(rows, 4, d)
+    keys, values = cache.rows(list(range(pages)))
+    seen = torch.arange(pages * page) >= low[:, None]
+    for h in range(4):
+        qh = q[:, h * d:(h + 1) * d].cpu().to(F64)
+        s = torch.where(seen, qh @ keys[h // 2].T * d ** -0.5, torch.full((), -float("inf"), dtype=F64))
+        p = torch.where(seen.any(-1, keepdim=True), torch.softmax(s, -1), torch.zeros((), dtype=F64))
+        want, mass, size = p @ values[h // 2], p @ values[h // 2].abs(), (qh.abs() @ keys[h // 2].abs().T).amax(-1, keepdim=True) * d ** -0.5
+        assert ((got[:, h] - want).abs() <= bound_of(dtype, d, want, mass, size) + 1e-12).all()
+        assert (got[:, h][~seen.any(-1)] == 0).all()
