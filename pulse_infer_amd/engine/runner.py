@@ -203,7 +203,9 @@ class ModelRunner:
         cache, groups = self.cache, self.cache.groups
         total, batch = metas[-1].first_row + metas[-1].count, len(metas)
         widths = [max(1, max(g.pages_for(m.start + m.count) for m in metas)) for g in groups]
-        if self.device.type != "cuda" or not self.MAPS_FROM <= batch <= cache8.MAX_REQUESTS:      # all of it on the host
+        # (all of it on the host, also where a pool has more slots than step_maps has numbers for)
+        if (self.device.type != "cuda" or not self.MAPS_FROM <= batch <= cache8.MAX_REQUESTS
+                or any(g.page_size * g.pool.num_pages >= 2 ** 31 for g in groups)):
             offsets = self._layout(total, batch, len(want_rows), widths)
             flat = np.zeros(int(offsets[-1]), dtype=np.int32)
             self._fill(flat, offsets, entries, metas, want_rows, widths)
