@@ -67,3 +67,52 @@ def test_pools_of_more_slots_than_32_bits_number():
         runner.add_request(r)
         runner.reserve(r, 40)
     same(runner, [StepEntry(r, [r + 1] * (r + 1), [0]) for r in range(9)])
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_host_and_device_agree(seed):
+    """Groups with and without windows and chunks, pages that were given back, portions of uneven lengths, pages reserved ahead, ids that
+    come from the device."""
+    require_gpu()
+    from pulse_infer_amd.cache import Paged8KVSpec, PagedKVSpec
+    from pulse_infer_amd.engine.runner import StepEntry
+
+    r = random.Random(seed)
+    page = r.choice([1, 4, 16, 24])
+    specs = [PagedKVSpec(2, 32), PagedKVSpec(2, 32, window=r.randint(1, 40)), PagedKVSpec(1, 64, chunk=r.randint(2, 50)), PagedKVSpec(2, 32),
+             Paged8KVSpec(2, 32, window=r.randint(1, 40))]
+    runner = runner_over(specs, page, 12_000)
+    live, gone = [], False
+    for step in range(12):
+        for _ in range(r.randint(0, 6) if step else 9):
+            live.append((seed, step, len(live)))
+            runner.add_request(live[-1])
+        if step > 4 and len(live) > 9:
+            runner.free_request(live.pop(r.randrange(len(live))))
+        entries = []
+        for name in r.sample(live, r.randint(1, len(live))):
+            n = r.choice([1, 1, 1, r.randint(1, 100)])
+            runner.reserve(name, runner.cache.computed(name) + n + r.choice([0, 0, 70]))
+            entries.append(StepEntry(name, [r.randrange(1000) for _ in range(n)], sorted(r.sample(range(n), r.randint(0, min(n, 3))))))
+        total = sum(len(e.tokens) for e in entries)
+        feed = None
+        if step % 3 == 1:
+            places = r.sample(range(total), r.randint(1, total))
+            source = torch.tensor([r.randrange(1000) for _ in range(total + 2)], dtype=torch.int32, device="cuda:0")
+            feed = (source, places, [r.randrange(total + 2) for _ in places])
+        same(runner, entries, feed)
+        gone = gone or any(-1 in t for g in runner.cache.groups for t in g.tables.values())
+    assert gone and len(runner.cache.groups) == 4
+
+
+def test_a_model_that_pages_nothing():
+    require_gpu()
+    from pulse_infer_amd.cache import StateSpec
+    from pulse_infer_amd.engine.runner import StepEntry
+
+    runner = runner_over([StateSpec((4, 4), "float32"), None], 16, 8)
+    for r in range(10):
+        runner.add_request(r)
+        runner.reserve(r, 50)
+    same(runner, [StepEntry(r, list(range(1, 2 + 3 * r)), [0] if r % 2 else []) for r in (9, 0, 3, 4, 5, 6, 7, 8, 1)])
+    same(runner, [StepEntry(r, [5], [0]) for r in range(10)])
