@@ -211,6 +211,8 @@ def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, vie
         shares, part_stride, part_row = parts.shape[0], parts.stride(0), parts.shape[2]
         if not store_takes_parts(qkv, d, rotated, page, parts, q_out, q_weight, k_weight, cos, sin) or part_row % 4 or q_stride % 4 or shares < 1:
             _refuse(what, "shares need bfloat16 rows, aligned, in chunks of eight channels, and pages of a multiple of 16 tokens")
+    if tokens == 0:       # (whose tensors have no addresses)
+        return
     call("pulse_store8", _STORE.pack(
         qkv.data_ptr(), stride, q_out.data_ptr(), q_stride, _at(q_weight), _at(k_weight), _at(cos), _at(sin), view.keys.data_ptr(),
         view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(), blocks.data_ptr(), _tag(qkv, what), w_tag, rotated, pairing,

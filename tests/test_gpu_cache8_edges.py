@@ -112,3 +112,30 @@ def test_attention_of_the_last_positions_behind_a_mask(d, page, dtype, window, c
         want, mass, size = p @ values[h // 2], p @ values[h // 2].abs(), (qh.abs() @ keys[h // 2].abs().T).amax(-1, keepdim=True) * d ** -0.5
         assert ((got[:, h] - want).abs() <= bound_of(dtype, d, want, mass, size) + 1e-12).all()
         assert (got[:, h][~seen.any(-1)] == 0).all()
+
+
+# -------------------------------------------------------------------------------------------------------- no rows at all
+@pytest.mark.parametrize("dtype,page", [(torch.bfloat16, 16), (torch.float32, 20)])
+def test_steps_without_rows(dtype, page):
+    """Requests that bring no tokens: nothing is stored, attended or listed, and nothing is refused."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    nkv, d, entries = 2, 32, [(3, 0), (0, 0)]
+    view = view_of(plain.Cache(2, nkv, page, d))
+    before = [t.clone().view(torch.uint8) for t in (view.keys, view.values, view.scales)]
+    empty, none = torch.zeros((0, 3 * nkv * d), dtype=dtype, device=DEV), ints([])
+    blocks = torch.full((2, 4), 9, dtype=torch.int32, device=DEV)
+    cache8.step_maps(ints([s for s, _ in entries]), ints([c for _, c in entries]), page_size=page, num_pages=2, table=ints([[1], [-1]]), blocks=blocks,
+                     positions=none, token_entry=none, slots=none)
+    assert blocks.tolist() == [[0, 0, -1, 0]] * 2
+    for listed in (blocks, blocks[:0]):
+        cache8.store(empty, empty[:, :nkv * d], nkv, nkv, d, view, none, listed)
+    cache8.store(empty, empty[:, :nkv * d], nkv, nkv, d, view, none, blocks, cos=torch.zeros((0, 16), device=DEV), sin=torch.zeros((0, 16), device=DEV),
+                 rotary_dim=32, plain_norm=True, q_temperature=(0.1, 3))
+    made = cache8.plan(metas(entries), nkv, nkv, d, none, page_size=page, dtype=dtype)
+    cache8.attention(empty, empty.clone(), made, view, none, none, ints([[1], [-1]]), 1.0)
+    out = torch.full((3, nkv * d), 7.0, dtype=dtype, device=DEV)      # (rows that no entry has)
+    cache8.attention(torch.zeros_like(out), out, made, view, ints([0] * 3), ints([-1] * 3), ints([[1], [-1]]), 1.0)
+    assert (out == 7.0).all()
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, (view.keys, view.values, view.scales)))
