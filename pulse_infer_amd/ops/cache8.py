@@ -274,6 +274,8 @@ class AttentionPlan:
             self.rows += e.count
         self.matrix = not plain and matrix_cores(d, page_size, dtype)
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:      # (the one that its lists lie on, whichever is the current one later)
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.ready = not self.matrix      # whether the keys have been shared out
         self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, counters an item, hundredths of the mean, longer pieces, cut)
         self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces, joined by the last)
