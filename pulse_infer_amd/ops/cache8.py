@@ -279,9 +279,12 @@ class AttentionPlan:
         self.ready = not self.matrix      # whether the keys have been shared out
         self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, counters an item, hundredths of the mean, longer pieces, cut)
         self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces, joined by the last)
+        self.streams: set = set()         # whose work the lists' memory waits for when the plan goes
         if not self.matrix:
             self.calls.append(("pulse_attn8_plain", 0, 0, 0, 0, 0, 0))
             return
+        if self.device.type == "cuda":
+            self.streams.add(_stream().value)
         units, group = compute_units(), nq // nkv
         few, many = [], []
         each, wide, groups = max(1, FEW // group), MANY // group, nkv * ((group + FEW - 1) // FEW)
@@ -330,6 +333,16 @@ class AttentionPlan:
             many[first:] = many[:first - 1:-1]
         add("pulse_attn8_many", MANY, many, nkv, self.MANY_NARROW_SLOTS if d in (32, 64) else self.MANY_SLOTS, self.MANY_LEAST, self.MANY_ROUNDS, self.MANY_EVEN)
 
+    def on(self, stream: Any) -> Any:
+        """``stream``, the current one, which reads the lists from now on: they may have been made on another, and the plan be dropped
+        before it has come to them."""
+        if stream.value not in self.streams:
+            self.streams.add(stream.value)
+            for work in self.works:
+                for t in (work[0], work[-1]):
+                    t.record_stream(torch.cuda.current_stream())
+        return stream
+
     def _tiles(self, start: int, count: int) -> int:
         """Tiles that hold keys of ``count`` tokens from position ``start`` on."""
         low = start - start % self.chunk if self.chunk else max(0, start - self.window + 1) if self.window else 0
@@ -342,9 +355,10 @@ class AttentionPlan:
         if self.device.index is not None and positions.device != self.device:
             _refuse("plan", f"it was made for {self.device}, the positions lie on {positions.device}")
         self.ready = True
+        stream = self.on(_stream())
         for items, n, slots, least, room, groups, even, shrink, cut in self.works:
             call("pulse_attn8_cut", _ptr(items), _i32(n), _ptr(positions), _i32(self.window), _i32(self.chunk), _i32(slots), _i32(least),
-                 _i32(room), _i32(groups), _i32(even), _i32(shrink), _ptr(cut), _stream())
+                 _i32(room), _i32(groups), _i32(even), _i32(shrink), _ptr(cut), stream)
         return self
 
 
@@ -352,7 +366,7 @@ def plan(entries: Sequence[Any], nq: int, nkv: int, d: int, positions: torch.Ten
          window: int = 0, chunk: int = 0, workspace: Any = None, to_device: Optional[Callable] = None) -> AttentionPlan:
     """The attention of a step of ``entries`` (``EntryMeta``: start, count, first_row; one's rows behind the other's from row 0 on, at
     positions that follow each other) whose rows stand at ``positions``, for layers of these heads.  It is made outside a recording; a step of the same shape takes the same plan, cut anew (``AttentionPlan.cut``, which may be
-    recorded).  A plan, its counters among it, serves the calls of one stream, one after the other.  ``workspace`` (a ``Workspace``):
+    recorded).  A plan, its counters among it, serves calls that follow each other, on whichever stream.  ``workspace`` (a ``Workspace``):
     where the room for joined pieces comes from, for the calls of one stream and not for two recordings at once; without one every
     call takes it from torch's pool."""
     return AttentionPlan(entries, nq, nkv, d, page_size=page_size, dtype=dtype, window=window, chunk=chunk, device=positions.device,
@@ -411,7 +425,7 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     if tokens == 0:
         return
     workspace = workspace if workspace is not None else plan.workspace
-    q_at, out_at = q.data_ptr(), out.data_ptr()
+    q_at, out_at, stream = q.data_ptr(), out.data_ptr(), plan.on(_stream())
     if plan.matrix and (q_at % 16 or q_stride % 8 or out_at % 8 or o_stride % 4):
         _refuse(what, "rows must be aligned to 16 bytes")
     for name, items, cut, n_items, room, rows, here in plan.calls:
@@ -428,4 +442,4 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
             q_at, q_stride, out_at, o_stride, view.keys.data_ptr(), view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(),
             token_entry.data_ptr(), table.data_ptr(), _at(gate), gate_stride, _at(sink), items, cut, part_o, part_ml, plan.tag, plan.rows,
             shape[0], shape[1], nq, nkv, d, page, pages, plan.window, plan.chunk, gate_width, n_items, room, here, 0, scale, softcap),
-            _stream())
+            stream)

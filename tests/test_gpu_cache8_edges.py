@@ -139,3 +139,50 @@ def test_steps_without_rows(dtype, page):
     cache8.attention(torch.zeros_like(out), out, made, view, ints([0] * 3), ints([-1] * 3), ints([[1], [-1]]), 1.0)
     assert (out == 7.0).all()
     assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, (view.keys, view.values, view.scales)))
+
+
+# ------------------------------------------------------------------------------------------------------------- streams
+@pytest.mark.parametrize("recut", [False, True])
+def test_a_plan_that_is_dropped_before_its_stream_has_come_to_it(recut):
+    """Made on one stream, used on another that is busy, dropped at once: nobody gets its lists' memory before they have been read."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    nq, nkv, d, page, entries = 8, 2, 64, 16, [(700, 1), (0, 150), (300, 40), (1200, 1)]
+    view = view_of(plain.Cache(200, nkv, page, d))
+    view.keys.copy_(torch.randn(view.keys.shape, device=DEV).to(view.keys.dtype))
+    view.values.copy_(torch.randn(view.values.shape, device=DEV).to(view.values.dtype))
+    view.scales.fill_(1.0)
+    total = sum(c for _, c in entries)
+    table = torch.randperm(200, generator=torch.Generator().manual_seed(1))[:4 * 50].to(torch.int32).view(4, 50).contiguous().to(DEV)
+    positions = ints([p for s, c in entries for p in range(s, s + c)])
+    token_entry = ints([b for b, (_, c) in enumerate(entries) for _ in range(c)])
+    table[3, 40:] = -1
+    q = torch.randn((total, nq * d), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(DEV)
+    want, out = torch.zeros_like(q), torch.zeros_like(q)
+    work, busy = torch.randn((8192, 8192), device=DEV).to(torch.bfloat16), torch.cuda.Stream()
+
+    def plan():
+        return cache8.plan(metas(entries), nq, nkv, d, positions, page_size=page, dtype=torch.bfloat16)
+
+    cache8.attention(q, want, plan(), view, positions, token_entry, table, d ** -0.5)
+    with torch.cuda.stream(busy):
+        product = work @ work      # (the library is loaded and its scratch there)
+    torch.cuda.synchronize()
+    made = plan()
+    lists = [(t.data_ptr(), t.numel()) for w in made.works for t in (w[0], w[-1])]
+    done = torch.cuda.Event()
+    busy.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(busy):
+        for _ in range(100):
+            torch.mm(work, work, out=product)
+        if recut:
+            made.cut(positions)
+        cache8.attention(q, out, made, view, positions, token_entry, table, d ** -0.5)
+        done.record()
+    del made
+    others = [torch.empty(n, dtype=torch.int32, device=DEV) for _ in range(8) for _, n in lists]      # (nothing is written to them)
+    assert not done.query()
+    assert not {t.data_ptr() for t in others} & {at for at, _ in lists}
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
