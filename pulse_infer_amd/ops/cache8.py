@@ -70,6 +70,16 @@ def _pages(what: str, view: Paged8CacheView, nkv: int, d: int) -> Tuple[int, int
     return pages, page
 
 
+def _apart(a: torch.Tensor, a_columns: int, b: torch.Tensor, b_columns: int) -> bool:
+    """Whether the first columns of ``a``'s rows and of ``b``'s, which are as many and of one type, have no byte in common."""
+    rows, size = a.shape[0], a.element_size()
+    at_a, at_b, step_a, step_b = a.data_ptr(), b.data_ptr(), a.stride(0) * size, b.stride(0) * size
+    if at_b >= at_a + (rows - 1) * step_a + a_columns * size or at_a >= at_b + (rows - 1) * step_b + b_columns * size:
+        return True
+    between = (at_b - at_a) % step_a if step_a else 0      # (rows of one buffer beside each other)
+    return rows > 1 and step_a == step_b and between >= a_columns * size and between + b_columns * size <= step_a
+
+
 # The arguments of the entry points as the structures of csrc/cache8_maps.hip, cache8_store.hip and cache8_attn.h, put together at once.
 _MAPS = struct.Struct("@9Q8i")
 _STORE = struct.Struct("@QqQq9Q14i2fQ3q")
@@ -179,6 +189,12 @@ def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, vie
     stride, q_stride = qkv.stride(0), q_out.stride(0)
     if tokens > 1 and (stride < columns or q_stride < nq * d):
         _refuse(what, "rows that overlap")
+    if tokens and parts is None:
+        if qkv.data_ptr() == q_out.data_ptr() and (tokens == 1 or stride == q_stride):
+            if v_head0 < nq:
+                _refuse(what, f"values from head {v_head0} on lie among the {nq} heads of q that q_out takes the place of")
+        elif not _apart(qkv, columns, q_out, nq * d):
+            _refuse(what, "q_out overlaps rows of qkv (it may be their front, or lie apart)")
     _ints(what, "positions", positions, tokens)
     places = _block_list(what, blocks)
     if (q_weight is None) != (k_weight is None) or (plain_norm and q_weight is not None):
@@ -377,7 +393,7 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
               token_entry: torch.Tensor, table: torch.Tensor, scale: float, *, gate: Optional[torch.Tensor] = None, gate_width: int = 0,
               sink: Optional[torch.Tensor] = None, softcap: float = 0.0, workspace: Any = None) -> None:
     """Causal attention of a step's rows over a cache in 8 bits, as ``plan`` has it: ``q``, ``out`` [T, >= nq * d] of one storage type (bfloat16
-    or float32; rows may be strided), ``positions`` (those that the plan was cut for) and ``token_entry`` int32 [T], ``table`` int32
+    or float32; rows may be strided, ``out`` may be ``q``), ``positions`` (those that the plan was cut for) and ``token_entry`` int32 [T], ``table`` int32
     [entries, width].
 
     A row sees the keys of its request from its window's (chunk's) first to its own position, in pages that are there: a table entry
@@ -401,6 +417,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     q_stride, o_stride = (q.stride(0), out.stride(0)) if tokens > 1 else (nq * d, nq * d)
     if q_stride < nq * d or o_stride < nq * d:
         _refuse(what, "rows that overlap")
+    if tokens and not (q.data_ptr() == out.data_ptr() and q_stride == o_stride) and not _apart(q, nq * d, out, nq * d):
+        _refuse(what, "out overlaps rows of q (it may be the same, or lie apart)")
     if plan.rows > tokens:
         _refuse(what, f"the plan has {plan.rows} rows, q {tokens}")
     if not plan.ready:

@@ -1,6 +1,7 @@
 """Plans of the attention over a cache in 8 bits, what of them no GPU is needed for."""
 from __future__ import annotations
 
+import pytest
 import torch
 
 from test_cache8_host import metas
@@ -14,3 +15,24 @@ def test_a_plan_is_one_devices(monkeypatch):
     plan = cache8.AttentionPlan(metas([(0, 3)]), 1, 1, 32, page_size=16, dtype=torch.float32)      # (one that has no lists)
     assert plan.device == torch.device("cuda", 3)
     assert cache8.AttentionPlan(metas([(0, 3)]), 1, 1, 32, page_size=16, dtype=torch.float32, device="cuda:1").device.index == 1
+
+
+@pytest.mark.parametrize("seed", range(300))
+def test_rows_that_lie_apart(seed):
+    """Against the bytes themselves, marked one by one."""
+    import random
+
+    r = random.Random(seed)
+    buffer = torch.zeros(4000, dtype=torch.bfloat16)
+    rows, a_columns, b_columns = r.randint(1, 6), r.randint(1, 40), r.randint(1, 40)
+    a_step = a_columns + r.randint(0, 60)
+    b_step = a_step if r.random() < 0.6 and a_step >= b_columns else b_columns + r.randint(0, 60)
+    a = buffer.as_strided((rows, a_columns), (a_step, 1), r.randint(0, 300))
+    b = buffer.as_strided((rows, b_columns), (b_step, 1), r.randint(0, 300))
+    a.fill_(1.0)
+    share = bool((b == 1.0).any())
+    got = cache8._apart(a, a_columns, b, b_columns)
+    if rows == 1 or a_step == b_step:
+        assert got == (not share)
+    else:                        # (rows of two steps that interleave are taken to overlap)
+        assert not (got and share)

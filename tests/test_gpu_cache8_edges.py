@@ -186,3 +186,76 @@ def test_a_plan_that_is_dropped_before_its_stream_has_come_to_it(recut):
     assert not {t.data_ptr() for t in others} & {at for at, _ in lists}
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------------------------------------ rows that overlap
+def test_rows_that_overlap_what_is_still_read_are_refused():
+    """q_out among k and v, out among other rows of q; beside each other in one buffer and in place they are served."""
+    require_gpu()
+    from pulse_infer_amd.ops import KernelError, cache8
+
+    nq, nkv, d, rows = 4, 2, 32, 5
+    view = view_of(plain.Cache(1, nkv, 16, d))
+    columns = (nq + 2 * nkv) * d
+    positions, blocks = ints(list(range(rows))), ints([[0, rows, 0, 0]])
+    buffer = torch.randn((rows, columns + nq * d), generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(DEV)
+
+    def store(qkv, q_out, **k):
+        cache8.store(qkv, q_out, nq, nkv, d, view, positions[:qkv.shape[0]], ints([[0, qkv.shape[0], 0, 0]]), **k)
+
+    for n in (1, rows):
+        with pytest.raises(KernelError, match="overlaps"):
+            store(buffer[:n], buffer[:n, d:])
+        with pytest.raises(KernelError, match="overlaps"):
+            store(buffer[:n], buffer[:n, columns - d:])
+        with pytest.raises(KernelError, match="among"):
+            store(buffer[:n], buffer[:n], v_head0=nq - 1)
+        store(buffer[:n], torch.empty_like(buffer[:n]), v_head0=0)      # (from rows of their own values may be any columns)
+    with pytest.raises(KernelError, match="overlaps"):
+        store(buffer[1:], buffer[:rows - 1])
+    with pytest.raises(KernelError, match="overlaps"):
+        store(buffer[:, :columns], buffer.view(-1)[:rows * nq * d].view(rows, nq * d))
+    q, out, token_entry, table = buffer[:, :nq * d].clone(), torch.empty((rows, nq * d), dtype=torch.bfloat16, device=DEV), ints([0] * rows), ints([[0]])
+    store(buffer[:, :columns], buffer[:, columns:])
+    assert torch.equal(buffer[:, columns:], q)      # (no norm, no rotation: q as it came)
+    store(buffer, buffer)
+    made = cache8.plan(metas([(0, rows)]), nq, nkv, d, positions, page_size=16, dtype=torch.bfloat16)
+
+    def attend(q, out):
+        cache8.attention(q, out, made, view, positions, token_entry, table, 0.2)
+
+    for bad in (buffer[:, d:], buffer[:, 8:]):
+        with pytest.raises(KernelError, match="overlaps"):
+            attend(buffer, bad)
+    longer = torch.zeros((rows + 1, nq * d), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(KernelError, match="overlaps"):
+        attend(longer[:rows], longer[1:])
+    attend(buffer, out)
+    attend(buffer, buffer[:, nq * d:])
+    assert torch.equal(buffer[:, nq * d:2 * nq * d], out)
+
+
+@pytest.mark.parametrize("d,page,dtype,entries", [(64, 16, torch.bfloat16, [(2000, 1), (3, 1), (700, 1)]), (64, 16, torch.bfloat16, [(2500, 300), (0, 90), (40, 1)]),
+                                                  (64, 8, torch.bfloat16, [(100, 40)]), (128, 16, torch.float32, [(300, 9)])])
+def test_attention_in_place(d, page, dtype, entries):
+    """out = q, through every kernel and join."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    nq, nkv = 8, 2
+    held = [-(-(s + c) // page) for s, c in entries]
+    pool = sum(held)
+    view = view_of(plain.Cache(pool, nkv, page, d))
+    view.keys.copy_(torch.randn(view.keys.shape, device=DEV).to(view.keys.dtype))
+    view.values.copy_(torch.randn(view.values.shape, device=DEV).to(view.values.dtype))
+    view.scales.fill_(1.0)
+    at = [sum(held[:i]) for i in range(len(held))]
+    table = ints([list(range(a, a + n)) + [-1] * (max(held) - n) for a, n in zip(at, held)])
+    positions = ints([p for s, c in entries for p in range(s, s + c)])
+    token_entry = ints([b for b, (_, c) in enumerate(entries) for _ in range(c)])
+    q = torch.randn((positions.numel(), nq * d + 8), device=DEV).to(dtype)
+    made = cache8.plan(metas(entries), nq, nkv, d, positions, page_size=page, dtype=dtype)
+    out = torch.empty_like(q)
+    cache8.attention(q, out, made, view, positions, token_entry, table, d ** -0.5)
+    cache8.attention(q, q, made, view, positions, token_entry, table, d ** -0.5)
+    assert torch.isfinite(out[:, :nq * d]).all() and torch.equal(q[:, :nq * d], out[:, :nq * d])
