@@ -11,6 +11,7 @@ falls back to another implementation.
 """
 from __future__ import annotations
 
+import math
 import struct
 from typing import Any, Callable, List, Optional, Sequence, Tuple
 
@@ -25,6 +26,7 @@ MAX_REQUESTS = 4096          # of step_maps
 MAX_HEAD_DIM = 512           # of store and of attention
 PIECE_INTS = 12              # of a piece of work (csrc/cache8_attn.h)
 TILE = 64                    # keys of a step of the matrix-core kernels
+MATRIX_CAP = 256.0           # the largest cap of those kernels, which have a capped score to 2^-22 of the cap: of 256 6e-5, where a weight is rounded by 2^-8
 FEW, MANY = 16, 128          # columns (rows times the heads that share a kv head) of an item of the two matrix-core kernels
 
 
@@ -248,6 +250,9 @@ def matrix_cores(d: int, page_size: int, dtype: torch.dtype) -> bool:
     return dtype == torch.bfloat16 and d % 16 == 0 and 32 <= d <= 256 and (d % 32 == 0 or d < 128) and page_size % 16 == 0
 
 
+PLAIN_CALLS = [("pulse_attn8_plain", 0, 0, 0, 0, 0, 0)]      # (of AttentionPlan.calls)
+
+
 class AttentionPlan:
     """A step's attention: which rows go together, and how the keys are shared out over the GPU.  The first depends on the step's shape
     alone (how many tokens each request brings); the second is made on the GPU from the positions, by ``cut``, once a step for all
@@ -297,7 +302,7 @@ class AttentionPlan:
         self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces, joined by the last)
         self.streams: set = set()         # whose work the lists' memory waits for when the plan goes
         if not self.matrix:
-            self.calls.append(("pulse_attn8_plain", 0, 0, 0, 0, 0, 0))
+            self.calls = PLAIN_CALLS
             return
         if self.device.type == "cuda":
             self.streams.add(_stream().value)
@@ -397,7 +402,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     [entries, width].
 
     A row sees the keys of its request from its window's (chunk's) first to its own position, in pages that are there: a table entry
-    outside the pool hides its keys.  A row that sees none is zeros.  ``scale`` > 0; ``softcap``: scores become cap * tanh(score / cap);
+    outside the pool hides its keys.  A row that sees none is zeros.  ``scale`` > 0; ``softcap``: scores become cap * tanh(score / cap)
+    (of caps above ``MATRIX_CAP`` by the kernel that serves every size);
     ``sink`` float32 [nq]: exp(sink) is one more term of the denominator; ``gate`` [T, nq] of q's storage type: head h is multiplied by
     sigmoid(gate[:, h]), or with ``gate_width`` [T, nq * gate_width] its first channels each by one of its own.  What is not finite
     reaches the rows that see it and no others.  Rows that no entry of the plan has are left as they were."""
@@ -423,8 +429,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
         _refuse(what, f"the plan has {plan.rows} rows, q {tokens}")
     if not plan.ready:
         _refuse(what, "the plan has not been cut for any positions")
-    if not scale > 0.0 or not softcap >= 0.0:
-        _refuse(what, "the scale must be positive and the cap not negative")
+    if not 0.0 < scale < math.inf or not 0.0 <= softcap < math.inf:
+        _refuse(what, "the scale must be positive and the cap not negative, and both finite")
     _ints(what, "positions", positions, tokens)
     _ints(what, "token_entry", token_entry, tokens)
     shape = table.shape
@@ -444,9 +450,10 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
         return
     workspace = workspace if workspace is not None else plan.workspace
     q_at, out_at, stream = q.data_ptr(), out.data_ptr(), plan.on(_stream())
-    if plan.matrix and (q_at % 16 or q_stride % 8 or out_at % 8 or o_stride % 4):
+    calls = plan.calls if softcap <= MATRIX_CAP else PLAIN_CALLS
+    if calls is not PLAIN_CALLS and (q_at % 16 or q_stride % 8 or out_at % 8 or o_stride % 4):
         _refuse(what, "rows must be aligned to 16 bytes")
-    for name, items, cut, n_items, room, rows, here in plan.calls:
+    for name, items, cut, n_items, room, rows, here in calls:
         part_o = part_ml = 0
         if rows:
             if workspace is not None:

@@ -7,7 +7,7 @@ import torch
 
 from conftest import require_gpu
 from plain import cache8_plain as plain
-from test_gpu_cache8 import DEV, F64, bound_of, ints, metas, view_of
+from test_gpu_cache8 import DEV, F64, MIX, attend, bound_of, ints, metas, view_of
 
 pytestmark = pytest.mark.gpu
 
@@ -259,3 +259,24 @@ def test_attention_in_place(d, page, dtype, entries):
     cache8.attention(q, out, made, view, positions, token_entry, table, d ** -0.5)
     cache8.attention(q, q, made, view, positions, token_entry, table, d ** -0.5)
     assert torch.isfinite(out[:, :nq * d]).all() and torch.equal(q[:, :nq * d], out[:, :nq * d])
+
+
+# ---------------------------------------------------------------------------------------------------------------- caps
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cap", [0.01, 30.0, 256.0, 256.1, 1e4, 1e6, 1e30])
+def test_attention_of_every_cap(dtype, cap):
+    """Scores under a cap far above them are the scores themselves."""
+    attend(MIX + [(600, 1)], 4, 2, 64, 16, dtype, seed=31, softcap=cap, sink=True, gate=0)
+    attend(MIX, 4, 2, 128, 16, dtype, seed=32, softcap=cap, window=33)
+
+
+@pytest.mark.parametrize("bad", [dict(softcap=float("inf")), dict(softcap=float("nan")), dict(scale=float("inf")), dict(scale=float("nan"))])
+def test_caps_and_scales_that_are_no_numbers_are_refused(bad):
+    require_gpu()
+    from pulse_infer_amd.ops import KernelError, cache8
+
+    view, pos = view_of(plain.Cache(1, 1, 16, 32)), ints([0])
+    q = torch.zeros((1, 32), dtype=torch.bfloat16, device=DEV)
+    made = cache8.plan(metas([(0, 1)]), 1, 1, 32, pos, page_size=16, dtype=torch.bfloat16)
+    with pytest.raises(KernelError, match="finite"):
+        cache8.attention(q, q.clone(), made, view, pos, pos, ints([[0]]), bad.get("scale", 1.0), softcap=bad.get("softcap", 0.0))
