@@ -24,6 +24,7 @@ from .library import KernelError, call
 
 MAX_REQUESTS = 4096          # of step_maps
 MAX_HEAD_DIM = 512           # of store and of attention
+MAX_PIECES = 65535           # of a launch's grid
 PIECE_INTS = 12              # of a piece of work (csrc/cache8_attn.h)
 TILE = 64                    # keys of a step of the matrix-core kernels
 MATRIX_CAP = 256.0           # the largest cap of those kernels, which have a capped score to 2^-22 of the cap: of 256 6e-5, where a weight is rounded by 2^-8
@@ -323,9 +324,10 @@ class AttentionPlan:
                 return
             tiles = [self._tiles(start, rows) for start, _, rows, _ in items]
             whole = n * groups >= slots * units and max(tiles) * slots * units <= even * sum(tiles) * groups
-            slots = max(1, slots * units // groups, rounds * n)
+            _need(n <= MAX_PIECES, f"plan: {n} items are too many")
+            whole = whole or n == MAX_PIECES
+            slots = max(1, min(max(slots * units // groups, rounds * n), MAX_PIECES - n))      # (fewer than the items: nothing is cut)
             room = n if whole else n + slots
-            _need(room <= 65535, f"plan: {n} items are too many")
             if not whole and columns == MANY:      # the longest pieces first, as far as can be told from the starts
                 low = max(least, -(-sum(tiles) // slots))
                 high = max(low, max(tiles))

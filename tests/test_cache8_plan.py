@@ -36,3 +36,12 @@ def test_rows_that_lie_apart(seed):
         assert got == (not share)
     else:                        # (rows of two steps that interleave are taken to overlap)
         assert not (got and share)
+
+
+@pytest.mark.parametrize("n", [21844, 21846, 30000, 65533, 65534])
+def test_many_requests_and_one_long(n):
+    """Items that are too many for each to have two pieces more are cut into fewer, or not at all."""
+    plan = cache8.AttentionPlan(metas([(100_000, 1)] + [(5, 1)] * n), 4, 2, 32, page_size=16, dtype=torch.bfloat16, device="cpu")
+    (_, _, _, items, room, columns, _), (_, _, slots, *_) = plan.calls[0], plan.works[0]
+    assert items == n + 1 <= room <= 65535 and (columns == 0) == (room == items)
+    assert slots >= 1 and (room == items or room >= items + slots)

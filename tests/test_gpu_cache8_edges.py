@@ -280,3 +280,32 @@ def test_caps_and_scales_that_are_no_numbers_are_refused(bad):
     made = cache8.plan(metas([(0, 1)]), 1, 1, 32, pos, page_size=16, dtype=torch.bfloat16)
     with pytest.raises(KernelError, match="finite"):
         cache8.attention(q, q.clone(), made, view, pos, pos, ints([[0]]), bad.get("scale", 1.0), softcap=bad.get("softcap", 0.0))
+
+
+# ------------------------------------------------------------------------------------------------------- many requests
+def test_attention_of_many_requests_and_one_long():
+    """A long context beside 30,000 short ones, or as many as a launch has room for, that are alike: the same rows as of the long one beside three."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    nq, nkv, d, pages = 4, 2, 32, 1251
+    view = view_of(plain.Cache(pages, nkv, 16, d))
+    view.keys.copy_(torch.randn(view.keys.shape, device=DEV).to(view.keys.dtype))
+    view.values.copy_(torch.randn(view.values.shape, device=DEV).to(view.values.dtype))
+    view.scales.fill_(1.0)
+    outs = []
+    for n in (3, 30_000, 65_534):
+        entries = [(20_000, 1)] + [(9, 1)] * n
+        table = torch.full((n + 1, pages), -1, dtype=torch.int32, device=DEV)
+        table[0], table[1:, 0] = torch.arange(pages, dtype=torch.int32, device=DEV), 7
+        q = torch.randn((2, nq * d), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+        q = torch.cat([q[:1], q[1:].expand(n, -1)])
+        positions = ints([s for s, _ in entries])
+        made = cache8.plan(metas(entries), nq, nkv, d, positions, page_size=16, dtype=torch.bfloat16)
+        out = torch.zeros_like(q)
+        cache8.attention(q, out, made, view, positions, ints(list(range(n + 1))), table, d ** -0.5)
+        assert torch.equal(out[1:], out[1:2].expand(n, -1))
+        outs.append(out[:2].double())
+    assert torch.equal(outs[0][1], outs[1][1]) and torch.equal(outs[0][1], outs[2][1]) and torch.isfinite(torch.stack(outs)).all()
+    # (the long one is cut differently: one rounding of the weights and one of the result on either side, of no more than the largest value)
+    assert ((outs[0][0] - torch.stack(outs)[:, 0]).abs() <= 4 * 2.0 ** -8 * view.values.float().abs().max().double()).all()
