@@ -118,11 +118,13 @@ __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restri
     cache8::Piece* work = reinterpret_cast<cache8::Piece*>(cut);
     int2* info = reinterpret_cast<int2*>(cut + cache8::PIECE_INTS * max_work);
     int* arrived = cut + cache8::PIECE_INTS * max_work + 2 * n;
-    const int at_most = 0x7fffffff / n;       // (so that no sum leaves 32 bits, whatever the positions are: 2 million tokens for 65,535 items)
+    // A thread's part of a sum ends here, so that no sum and none with the slots in it leaves 32 bits: of lengths it only says where the search
+    // begins and whether items are alike, and as a number of pieces it is more than the slots in any case.
+    constexpr int FULL = 0x7fff0000 / THREADS;
     auto walk = [&](int i) {
         const int4 it = items[i];
         const int hi = positions[it.x + it.y - 1], pos0 = positions[it.x], first = cache8::low_key(window, chunk, pos0) / TILE;
-        const int count = min(max(hi / TILE + 1 - first, 1), at_most);
+        const int count = max(hi / TILE + 1 - first, 1);
         return cache8::Piece{it.x, it.y, it.z, i, first, first + count, 0, 0, hi, pos0, {0, 0}};
     };
     // over all threads
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restri
     int total = 0, most = 0;
     for (int i = tid; i < n; i += THREADS) {
         const int t = tiles(i);
-        total += t;
+        total = min(total + t, FULL);
         most = max(most, t);
     }
     both(total, most);
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(THREADS) void attn8_cut_kernel(const int4* __restri
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
         int pieces = 0, unused = 0;
-        for (int i = tid; i < n; i += THREADS) pieces += (tiles(i) + mid - 1) / mid;
+        for (int i = tid; i < n; i += THREADS) pieces = min(pieces + (tiles(i) + mid - 1) / mid, FULL);
         both(pieces, unused);
         if (pieces <= slots) hi = mid;
         else lo = mid + 1;

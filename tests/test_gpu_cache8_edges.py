@@ -309,3 +309,38 @@ def test_attention_of_many_requests_and_one_long():
     assert torch.equal(outs[0][1], outs[1][1]) and torch.equal(outs[0][1], outs[2][1]) and torch.isfinite(torch.stack(outs)).all()
     # (the long one is cut differently: one rounding of the weights and one of the result on either side, of no more than the largest value)
     assert ((outs[0][0] - torch.stack(outs)[:, 0]).abs() <= 4 * 2.0 ** -8 * view.values.float().abs().max().double()).all()
+
+
+@pytest.mark.parametrize("n,tokens", [(65_535, 2_500_001), (40_000, 4_000_000)])
+def test_attention_of_a_context_of_millions_beside_many(n, tokens):
+    """The last keys of a context of millions of tokens count, however many requests are beside it."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    d, page = 32, 4096
+    view = view_of(plain.Cache(2, 1, page, d))
+    g = torch.Generator().manual_seed(n)
+    view.keys.copy_((torch.randn(view.keys.shape, generator=g) * 0.1).to(DEV).to(view.keys.dtype))
+    view.values.copy_(torch.randn(view.values.shape, generator=g).to(DEV).to(view.values.dtype))
+    view.scales.fill_(1.0)
+    q = torch.randn((1, d), generator=g).to(torch.bfloat16)
+    view.keys[1, 0, :9] = (torch.sign(q) * 4).to(DEV).to(view.keys.dtype)      # (a few keys of the last page outweigh all that is before them)
+    last = (tokens - 1) // page
+    table = torch.full((n, last + 1), -1, dtype=torch.int32, device=DEV)
+    table[:, 0], table[0] = 0, 0
+    table[0, last] = 1
+    positions = ints([tokens - 1] + [20] * (n - 1))
+    made = cache8.plan(metas([(tokens - 1, 1)] + [(20, 1)] * (n - 1)), 1, 1, d, positions, page_size=page, dtype=torch.bfloat16)
+    rows = q.to(DEV).expand(n, -1).contiguous()
+    out = torch.zeros_like(rows)
+    cache8.attention(rows, out, made, view, positions, ints(list(range(n))), table, 1.0)
+    keys, values = (x[:, 0] for x in (plain.decode(view.keys), plain.decode(view.values).transpose(3, 4).reshape(2, 1, page, d)))
+    s = [keys[i] @ q[0].to(F64) for i in (0, 1)]
+    s[1] = s[1][:(tokens - 1) % page + 1]
+    top = max(float(x.max()) for x in s)
+    p = [torch.exp(x - top) * w for x, w in zip(s, (last, 1))]
+    total = sum(x.sum() for x in p)
+    want, mass = (sum(x @ f(v[:x.numel()]) for x, v in zip(p, values)) / total for f in (lambda v: v, torch.abs))
+    size = max(float((keys[i].abs() @ q[0].abs().to(F64)).max()) for i in (0, 1))
+    assert ((out[0].cpu().to(F64) - want).abs() <= bound_of(torch.bfloat16, d, want, mass, size)).all()
+    assert float(p[1][:9].sum() / total) > 0.5
