@@ -287,7 +287,9 @@ class AttentionPlan:
         _need(window >= 0 and chunk >= 0 and not (window and chunk), "plan: a window and chunks at once, or a negative one")
         _need(dtype in (torch.bfloat16, torch.float32), f"plan: storage type {dtype} is not supported (float32 or bfloat16)")
         self.nq, self.nkv, self.d, self.page_size, self.dtype = nq, nkv, d, int(page_size), dtype
-        self.window, self.chunk, self.workspace = int(window), int(chunk), workspace
+        # (one that no position of 32 bits reaches beyond hides nothing)
+        self.window, self.chunk = (0 if v >= 2 ** 31 else int(v) for v in (window, chunk))
+        self.workspace = workspace
         self.tag = _TAG[dtype]
         self.rows, self.entries = 0, len(entries)
         for e in entries:

@@ -45,3 +45,11 @@ def test_many_requests_and_one_long(n):
     (_, _, _, items, room, columns, _), (_, _, slots, *_) = plan.calls[0], plan.works[0]
     assert items == n + 1 <= room <= 65535 and (columns == 0) == (room == items)
     assert slots >= 1 and (room == items or room >= items + slots)
+
+
+def test_windows_and_chunks_beyond_32_bits_hide_nothing():
+    for given in (dict(window=2 ** 31), dict(chunk=2 ** 31), dict(window=2 ** 40), dict(chunk=10 ** 12)):
+        plan = cache8.AttentionPlan(metas([(70, 1), (2 ** 31 - 3, 2)]), 2, 1, 32, page_size=16, dtype=torch.bfloat16, device="cpu", **given)
+        assert (plan.window, plan.chunk) == (0, 0) and plan._tiles(70, 1) == 2
+    plan = cache8.AttentionPlan(metas([(70, 1)]), 2, 1, 32, page_size=16, dtype=torch.bfloat16, device="cpu", window=2 ** 31 - 1)
+    assert plan.window == 2 ** 31 - 1
