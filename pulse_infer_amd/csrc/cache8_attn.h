@@ -31,7 +31,6 @@ __device__ __forceinline__ int low_key(int window, int chunk, int pos) {
     if (chunk > 0) return pos > 0 ? pos / chunk * chunk : 0;
     return window > 0 ? max(0, pos - window + 1) : 0;
 }
-__device__ __forceinline__ float tanh_of(float x) { return 1.f - 2.f / (__expf(2.f * x) + 1.f); }
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + __expf(-x)); }
 
 // What a cut is: for every workgroup a piece (no rows: nothing to do), for every item its first piece and how many it has, then
