@@ -173,8 +173,11 @@ class CacheManager:
         return spec.view(self.state[key], 0, -1, self.page_size, writable)
 
     def storage_bytes(self, element_size: int) -> int:
-        return sum(len(g.runs) * g.pool.num_pages * g.page_size * g.spec.bytes_per_token(element_size)
-                   for g in self.groups)
+        def page(g: CacheGroup) -> int:
+            whole = getattr(g.spec, "bytes_per_page", None)
+            return whole(element_size, g.page_size) if whole else g.page_size * g.spec.bytes_per_token(element_size)
+
+        return sum(len(g.runs) * g.pool.num_pages * page(g) for g in self.groups)
 
     # ----------------------------------------------------------------- requests
     def add_request(self, request: Hashable) -> int:

@@ -14,7 +14,8 @@ A spec is a small hashable object that the cache manager asks, never inspects:
   chunks of that many, counted from 0, and a token reads keys of its own chunk
   only, so pages wholly in chunks that are over go back.
 * ``bytes_per_token(element_size)`` (per-token specs) — what one token costs one
-  run, for sizing pools and pricing steps.
+  run, for sizing pools and pricing steps.  ``bytes_per_page(element_size,
+  page_size)`` (optional) — what a page does, where that is not its tokens' sum.
 * ``allocate(runs, units, page_size, device, dtype)`` — the storage of all runs of
   a group (``units`` pages of ``page_size`` tokens each) or of one run's state
   (``units`` slots; ``runs`` is 1).  Whatever it returns is kept as it is.
@@ -126,6 +127,9 @@ class Paged8KVSpec:
 
     def bytes_per_token(self, element_size: int) -> int:
         return 2 * self.num_kv_heads * self.head_dim + (8 * self.num_kv_heads + 15) // 16
+
+    def bytes_per_page(self, element_size: int, page_size: int) -> int:
+        return self.num_kv_heads * (2 * self.head_dim * page_size + 8 * (page_size // block_tokens(page_size)))
 
     def allocate(self, runs: int, units: int, page_size: int, device: Any, dtype: Any) -> Tuple[Any, Any, Any]:
         import torch

@@ -6,6 +6,7 @@ import torch
 
 from test_cache8_host import metas
 
+from pulse_infer_amd.cache import CacheManager, Paged8KVSpec, PagedKVSpec
 from pulse_infer_amd.ops import cache8
 
 
@@ -53,3 +54,12 @@ def test_windows_and_chunks_beyond_32_bits_hide_nothing():
         assert (plan.window, plan.chunk) == (0, 0) and plan._tiles(70, 1) == 2
     plan = cache8.AttentionPlan(metas([(70, 1)]), 2, 1, 32, page_size=16, dtype=torch.bfloat16, device="cpu", window=2 ** 31 - 1)
     assert plan.window == 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("page", [1, 4, 8, 16, 24, 48, 64])
+@pytest.mark.parametrize("heads", [1, 3, 8])
+def test_bytes_of_the_storage(page, heads):
+    """What the manager says of its pools is what their tensors take: of 8 bits with scales for every block, whatever the page."""
+    manager = CacheManager([Paged8KVSpec(heads, 32), PagedKVSpec(2, 16), Paged8KVSpec(heads, 32)], page_size=page, num_pages=5, max_requests=2)
+    manager.allocate_storage("cpu", torch.bfloat16)
+    assert manager.storage_bytes(2) == sum(t.numel() * t.element_size() for g in manager.groups for t in g.spec.tensors(g.storage))
