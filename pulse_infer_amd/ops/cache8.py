@@ -259,21 +259,31 @@ class AttentionPlan:
     alone (how many tokens each request brings); the second is made on the GPU from the positions, by ``cut``, once a step for all
     layers that are alike in heads, window and chunk.  ``plain``: everything goes to the kernel that serves every size."""
 
-    # Workgroups a compute unit that a kernel's keys are shared out over, the fewest tiles of 64 keys of a piece, and how many times the
-    # items there may be pieces in any case.  Of attn8_many's a unit's registers hold three where heads have 32 or 64 channels (two / three,
-    # us: 2,048 tokens 42 / 34.5, 2 portions of 509 behind 7,000 at 40 heads 133 / 107); pieces for as many in
-    # attn8_few read no faster (64 contexts of 4,096 95 / 104).
-    FEW_SLOTS, FEW_LEAST, FEW_ROUNDS = 2, 8, 2
-    MANY_SLOTS, MANY_NARROW_SLOTS, MANY_LEAST, MANY_ROUNDS = 2, 3, 8, 1
+    # Workgroups a compute unit that a kernel's keys are shared out over ("slots") and the fewest tiles of 64 keys of a piece.  Of attn8_many's a
+    # unit's registers hold three where heads have 32 or 64 channels (two / three, us: 2,048 tokens 42 / 34.5, 2 portions of 509 behind 7,000
+    # at 40 heads 133 / 107); pieces for as many in attn8_few read no faster (64 contexts of 4,096 95 / 104).
+    FEW_SLOTS, FEW_LEAST = 2, 8
+    MANY_SLOTS, MANY_NARROW_SLOTS, MANY_LEAST = 2, 3, 8
+    # How many times the items there may be pieces in any case, where the items have not and where they have a slot each by themselves (32 heads on
+    # 8 of 128, us).  attn8_few, once / twice / three times: contexts of 3,000 on the average, the longest 15,000, 40 of them 53 / 60 / 59, 64
+    # 139 / 89 / 86, 100 of 2,000 106 / 90 / 91; 40 of 6,000 that are alike 110 / 101.  attn8_many: 1,500 tokens 36.6 / 42.8, 3 portions of 500
+    # behind 1,000 49.7 / 60 / 63; 300 behind 8,000 beside 2,000 229 / 106 / 117, 600 behind 12,000 beside six of 500 343 / 192 / 196.  (Of 256
+    # channels a unit holds one workgroup of attn8_many: five portions up to 2,009 132 / 160.)
+    FEW_ROUNDS, MANY_ROUNDS = (2, 2), (1, 2)
     # Up to so many pieces an item on the average the last one joins them (in a launch of its own / by the last, us: 1,024 tokens 39 / 28, 3
     # portions of 300 behind 2,000 59 / 48, 512 behind 8,192 98 / 96; at 10 an item 74 / 109).
     MANY_HERE = 6
-    # Nothing is cut (and nothing joined) where the items fill the GPU by themselves and the longest is at most that many times what a
-    # workgroup's share of them would be.
-    FEW_EVEN, MANY_EVEN = 1.15, 2.2
-    # Of attn8_few, where every unit has an item, neither are those whose lengths are (on the GPU, in a step's own positions) within so many
-    # hundredths of their mean, unless some units had two and most one: 32 / 48 / 56 contexts of 4,000, 32 heads on 8 of 128, cut / whole, us: 45.9 /
-    # 42.9, 76.7 / 78.9, 94 / 83 (of 1,000 17.7 / 14.8, 22.3 / 20.7, 27.7 / 21.8); 40 66 / 72; 40 of 64 channels 33.6 / 30.4.
+    # Nothing is cut (and nothing joined) where the items have a slot each by themselves and the longest is not much more than a slot's share of all:
+    # so many times of attn8_few's, at most so many tiles more of attn8_many's.  Whole / cut, us, 32 heads on 8 of 128: 64 contexts of 4,000 on the
+    # average 94 / 107 (1.05 times), 96 / 110 (1.15), 101 / 111 (1.3), 106 / 110 (1.5), 114 / 112 (1.8), but 96 of 3,000 118 / 122 (1.0), 124 / 122 (1.2),
+    # 129 / 123 (1.5) and 128 of 2,000 113 / 111 (0.9), 117 / 112 (1.15), 121 / 112 (1.3).  Portions: 1,044 and 1,668 tokens 54 / 62 (11 tiles more), 2,600
+    # 79 / 84 (14), 2,048 63 / 59 to 71 (16), 600 behind 3,000 beside 2,000 107 / 95 (26), 1,200 behind 4,000 beside 1,500 158 / 136 (30), 600 behind
+    # 6,000 beside 2,000 183 / 132 (59).
+    FEW_EVEN, MANY_LONGER = 1.15, 24
+    # Of attn8_few, where every unit has an item, neither are those cut whose lengths are (on the GPU, in a step's own positions) within so many
+    # hundredths of their mean, unless some units had two and most one.  Cut / whole, us, 32 heads on 8 of 128, contexts of 1,000 / 4,000 / 8,000: 32 of
+    # them 19.6 / 16.6, 52.9 / 49.2, 98 / 93; 40 24.6 / 26, 71 / 76, 129 / 147; 48, where it changes with the length, 25.7 / 24.7, 77.8 / 79.9, 143 / 152; 56 33 / 25.7,
+    # 94 / 84, 175 / 160.  Of 64 channels 40 14.2 / 11.6, 39 / 36, 71 / 68.
     FEW_ALIKE = 110
     # Portions go through attn8_few up to so many columns, and altogether while they walk no more tiles a compute unit for it.  One portion
     # of 128 rows, 32 heads on 8, many / few, us: from the start 14.5 / 11.6, behind 1,000 tokens 22.1 / 12.7, behind 8,000 42.5 / 47; of 200
@@ -320,15 +330,16 @@ class AttentionPlan:
             to += [(e.start + at, e.first_row + at, min(step, e.count - at), i) for at in range(0, e.count, step)]
         to_device = to_device or (lambda flat: torch.tensor(flat, dtype=torch.int32, device=self.device))
 
-        def add(name: str, columns: int, items: List[Tuple], groups: int, slots: int, least: int, rounds: int, even: float) -> None:
+        def add(name: str, columns: int, items: List[Tuple], groups: int, slots: int, least: int, rounds: Tuple[int, int]) -> None:
             n = len(items)
             if not n:
                 return
             tiles = [self._tiles(start, rows) for start, _, rows, _ in items]
-            whole = n * groups >= slots * units and max(tiles) * slots * units <= even * sum(tiles) * groups
             _need(n <= MAX_PIECES, f"plan: {n} items are too many")
-            whole = whole or n == MAX_PIECES
-            slots = max(1, min(max(slots * units // groups, rounds * n), MAX_PIECES - n))      # (fewer than the items: nothing is cut)
+            filled = n * groups >= slots * units
+            share = sum(tiles) * groups / (slots * units)
+            whole = n == MAX_PIECES or filled and max(tiles) <= (share + self.MANY_LONGER if columns == MANY else self.FEW_EVEN * share)
+            slots = max(1, min(max(slots * units // groups, rounds[filled] * n), MAX_PIECES - n))      # (fewer than the items: nothing is cut)
             room = n if whole else n + slots
             if not whole and columns == MANY:      # the longest pieces first, as far as can be told from the starts
                 low = max(least, -(-sum(tiles) // slots))
@@ -350,13 +361,14 @@ class AttentionPlan:
             self.works.append((on_gpu, n, slots, least, room, counters // n, alike, int(columns == FEW), cut))
             self.calls.append((name, on_gpu.data_ptr(), cut.data_ptr(), n, room, 0 if whole else room * groups * columns, here))
 
-        add("pulse_attn8_few", FEW, few, groups, self.FEW_SLOTS, self.FEW_LEAST, self.FEW_ROUNDS, self.FEW_EVEN)
+        add("pulse_attn8_few", FEW, few, groups, self.FEW_SLOTS, self.FEW_LEAST, self.FEW_ROUNDS)
         # The longest walks first; where two workgroups share a unit, the second ones' from the other end, the shortest beside the longest.
         many.sort(key=lambda it: -it[0])
         first = max(1, units // nkv)
         if first < len(many) <= 2 * first:
             many[first:] = many[:first - 1:-1]
-        add("pulse_attn8_many", MANY, many, nkv, self.MANY_NARROW_SLOTS if d in (32, 64) else self.MANY_SLOTS, self.MANY_LEAST, self.MANY_ROUNDS, self.MANY_EVEN)
+        add("pulse_attn8_many", MANY, many, nkv, self.MANY_NARROW_SLOTS if d in (32, 64) else self.MANY_SLOTS, self.MANY_LEAST,
+            self.MANY_ROUNDS if d < 256 else (1, 1))
 
     def on(self, stream: Any) -> Any:
         """``stream``, the current one, which reads the lists from now on: they may have been made on another, and the plan be dropped

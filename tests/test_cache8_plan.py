@@ -63,3 +63,19 @@ def test_bytes_of_the_storage(page, heads):
     manager = CacheManager([Paged8KVSpec(heads, 32), PagedKVSpec(2, 16), Paged8KVSpec(heads, 32)], page_size=page, num_pages=5, max_requests=2)
     manager.allocate_storage("cpu", torch.bfloat16)
     assert manager.storage_bytes(2) == sum(t.numel() * t.element_size() for g in manager.groups for t in g.spec.tensors(g.storage))
+
+
+def test_portions_of_uneven_walks_are_cut_where_they_fill_the_gpu(monkeypatch):
+    """A slot each by themselves: two pieces an item where one walk is far longer than a slot's share of all, else whole; of 256 channels, of which a
+    compute unit holds one workgroup, no more pieces than items."""
+    monkeypatch.setattr(cache8, "compute_units", lambda: 256)
+
+    def room(entries, d=128):
+        plan = cache8.AttentionPlan(metas(entries), 32, 8, d, page_size=16, dtype=torch.bfloat16, device="cpu")
+        (name, _, _, items, pieces, _, _), = plan.calls
+        assert name == "pulse_attn8_many" and items * 8 >= 512
+        return pieces / items
+
+    assert room([(8000, 300), (0, 2000)]) == room([(6000, 600), (0, 2000)]) == 3      # (the items and twice as many)
+    assert room([(0, 2048)]) == room([(0, 2600)]) == room([(0, 1044), (0, 1668)]) == room([(8000, 2048)]) == 1
+    assert room([(8000, 300), (0, 2000)], d=256) == 2

@@ -344,3 +344,15 @@ def test_attention_of_a_context_of_millions_beside_many(n, tokens):
     size = max(float((keys[i].abs() @ q[0].abs().to(F64)).max()) for i in (0, 1))
     assert ((out[0].cpu().to(F64) - want).abs() <= bound_of(torch.bfloat16, d, want, mass, size)).all()
     assert float(p[1][:9].sum() / total) > 0.5
+
+
+@pytest.mark.parametrize("window", [0, 900])
+def test_attention_of_portions_that_fill_the_gpu_and_are_cut(window):
+    """A short portion far behind beside a longer one from the start, whose items have a place each by themselves."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    entries = [(4000, 40), (0, 500)]
+    plan = cache8.AttentionPlan(metas(entries), 128, 32, 96, page_size=16, dtype=torch.bfloat16)
+    assert plan.calls[0][3] * 32 >= 512 and plan.calls[0][4] == 3 * plan.calls[0][3]
+    attend(entries, 128, 32, 96, 16, seed=40, window=window)
