@@ -313,6 +313,7 @@ class AttentionPlan:
         self.ready = not self.matrix      # whether the keys have been shared out
         self.works: List[Tuple] = []      # (items on the GPU, their number, slots, least, room for pieces, counters an item, hundredths of the mean, longer pieces, cut)
         self.calls: List[Tuple] = []      # (entry point, items, cut, number of items, room for pieces, columns of the room for joined pieces, joined by the last)
+        self.rooms: dict = {}             # what its calls had of the workspace: a recording goes on writing there when the workspace has grown
         self.streams: set = set()         # whose work the lists' memory waits for when the plan goes
         if not self.matrix:
             self.calls = PLAIN_CALLS
@@ -404,8 +405,8 @@ def plan(entries: Sequence[Any], nq: int, nkv: int, d: int, positions: torch.Ten
     """The attention of a step of ``entries`` (``EntryMeta``: start, count, first_row; one's rows behind the other's from row 0 on, at
     positions that follow each other) whose rows stand at ``positions``, for layers of these heads.  It is made outside a recording; a step of the same shape takes the same plan, cut anew (``AttentionPlan.cut``, which may be
     recorded).  A plan, its counters among it, serves calls that follow each other, on whichever stream.  ``workspace`` (a ``Workspace``):
-    where the room for joined pieces comes from, for the calls of one stream and not for two recordings at once; without one every
-    call takes it from torch's pool."""
+    where the room for joined pieces comes from, for calls and replays that follow each other; without one every call takes it from
+    torch's pool.  A recording needs its plan (the lists, and the room that it was recorded with) for as long as it is replayed."""
     return AttentionPlan(entries, nq, nkv, d, page_size=page_size, dtype=dtype, window=window, chunk=chunk, device=positions.device,
                          workspace=workspace, to_device=to_device).cut(positions)
 
@@ -475,6 +476,11 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
             if workspace is not None:
                 o = workspace.buffer("attention8.part_o", rows, d, torch.float32)
                 ml = workspace.buffer("attention8.part_ml", rows, 2, torch.float32)
+                place = o.data_ptr(), ml.data_ptr(), stream.value
+                if place not in plan.rooms:
+                    plan.rooms[place] = o, ml
+                    for t in (o, ml):          # (made on another stream, perhaps)
+                        t.record_stream(torch.cuda.current_stream())
             else:
                 o = torch.empty((rows, d), dtype=torch.float32, device=q.device)
                 ml = torch.empty((rows, 2), dtype=torch.float32, device=q.device)

@@ -142,11 +142,13 @@ def test_steps_without_rows(dtype, page):
 
 
 # ------------------------------------------------------------------------------------------------------------- streams
-@pytest.mark.parametrize("recut", [False, True])
-def test_a_plan_that_is_dropped_before_its_stream_has_come_to_it(recut):
-    """Made on one stream, used on another that is busy, dropped at once: nobody gets its lists' memory before they have been read."""
+@pytest.mark.parametrize("recut,room", [(False, False), (True, False), (False, True)])
+def test_a_plan_that_is_dropped_before_its_stream_has_come_to_it(recut, room):
+    """Made on one stream, used on another that is busy, dropped at once (with its workspace): nobody gets its lists' memory, or the workspace's, before
+    they have been read."""
     require_gpu()
     from pulse_infer_amd.ops import cache8
+    from pulse_infer_amd.parts.base import Workspace
 
     nq, nkv, d, page, entries = 8, 2, 64, 16, [(700, 1), (0, 150), (300, 40), (1200, 1)]
     view = view_of(plain.Cache(200, nkv, page, d))
@@ -162,15 +164,21 @@ def test_a_plan_that_is_dropped_before_its_stream_has_come_to_it(recut):
     want, out = torch.zeros_like(q), torch.zeros_like(q)
     work, busy = torch.randn((8192, 8192), device=DEV).to(torch.bfloat16), torch.cuda.Stream()
 
-    def plan():
-        return cache8.plan(metas(entries), nq, nkv, d, positions, page_size=page, dtype=torch.bfloat16)
+    def plan(ws=None):
+        return cache8.plan(metas(entries), nq, nkv, d, positions, page_size=page, dtype=torch.bfloat16, workspace=ws)
 
     cache8.attention(q, want, plan(), view, positions, token_entry, table, d ** -0.5)
     with torch.cuda.stream(busy):
         product = work @ work      # (the library is loaded and its scratch there)
     torch.cuda.synchronize()
-    made = plan()
+    ws = Workspace(torch.device(DEV)) if room else None
+    made = plan(ws)
     lists = [(t.data_ptr(), t.numel()) for w in made.works for t in (w[0], w[-1])]
+    if room:      # (the workspace's buffers are the first stream's)
+        cache8.attention(q, out, made, view, positions, token_entry, table, d ** -0.5)
+        lists += [(t.data_ptr(), t.numel()) for r in made.rooms.values() for t in r]
+        assert len(lists) >= 4
+        out.zero_()
     done = torch.cuda.Event()
     busy.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(busy):
@@ -180,7 +188,7 @@ def test_a_plan_that_is_dropped_before_its_stream_has_come_to_it(recut):
             made.cut(positions)
         cache8.attention(q, out, made, view, positions, token_entry, table, d ** -0.5)
         done.record()
-    del made
+    del made, ws
     others = [torch.empty(n, dtype=torch.int32, device=DEV) for _ in range(8) for _, n in lists]      # (nothing is written to them)
     assert not done.query()
     assert not {t.data_ptr() for t in others} & {at for at, _ in lists}
@@ -356,3 +364,49 @@ def test_attention_of_portions_that_fill_the_gpu_and_are_cut(window):
     plan = cache8.AttentionPlan(metas(entries), 128, 32, 96, page_size=16, dtype=torch.bfloat16)
     assert plan.calls[0][3] * 32 >= 512 and plan.calls[0][4] == 3 * plan.calls[0][3]
     attend(entries, 128, 32, 96, 16, seed=40, window=window)
+
+
+# ---------------------------------------------------------------------------------------------------------- recordings
+def test_a_recording_outlives_the_workspace_it_was_recorded_with():
+    """A workspace that grows behind a recording, for another recording and for eager calls: each replay is the eager call, in whatever order."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+    from pulse_infer_amd.parts.base import Workspace
+
+    nq, nkv, d, page = 8, 2, 64, 16
+    view = view_of(plain.Cache(300, nkv, page, d))
+    view.keys.copy_(torch.randn(view.keys.shape, device=DEV).to(view.keys.dtype))
+    view.values.copy_(torch.randn(view.values.shape, device=DEV).to(view.values.dtype))
+    view.scales.fill_(1.0)
+    table = torch.randperm(300, generator=torch.Generator().manual_seed(1))[:4 * 75].to(torch.int32).view(4, 75).contiguous().to(DEV)
+    shared, programs = Workspace(torch.device(DEV)), []
+    for entries in ([(900, 1), (1100, 1)], [(1000, 1)] * 3, [(700, 300), (0, 90), (1000, 1)], [(900, 200), (800, 100), (900, 200), (1000, 1)]):
+        total = sum(c for _, c in entries)
+        positions = ints([p for s, c in entries for p in range(s, s + c)])
+        token_entry = ints([b for b, (_, c) in enumerate(entries) for _ in range(c)])
+        q = torch.randn((total, nq * d), generator=torch.Generator().manual_seed(total)).to(torch.bfloat16).to(DEV)
+        out = torch.zeros_like(q)
+
+        def call(plan, out=out, q=q, positions=positions, token_entry=token_entry):
+            cache8.attention(q, out, plan, view, positions, token_entry, table, d ** -0.5)
+
+        make = lambda ws: cache8.plan(metas(entries), nq, nkv, d, positions, page_size=page, dtype=torch.bfloat16, workspace=ws)  # noqa: E731
+        call(make(None))
+        want, plan = out.clone(), make(shared)
+        call(plan)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):      # (which gives the pool's free memory back to the device)
+            call(plan)
+        programs.append((plan, call, graph, out, want))
+    current = {shared.buffer("attention8.part_o", 1, 1, torch.float32).data_ptr()}
+    rooms = [{at for at, _, _ in plan.rooms} for plan, *_ in programs]
+    assert all(rooms) and len(set().union(*rooms)) > 1 and any(not r & current for r in rooms)      # (some were recorded with what has been replaced)
+    assert all(o.data_ptr() == at for plan, *_ in programs for (at, _, _), (o, _) in plan.rooms.items())
+    torch.cuda.empty_cache()
+    for i in (0, 3, 1, 2, 0, 0, 3):
+        plan, call, graph, out, want = programs[i]
+        for run in (graph.replay, lambda: call(plan), graph.replay):
+            out.zero_()
+            run()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), i
