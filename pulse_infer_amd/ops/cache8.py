@@ -11,7 +11,6 @@ falls back to another implementation.
 """
 from __future__ import annotations
 
-import math
 import struct
 from typing import Any, Callable, List, Optional, Sequence, Tuple
 
@@ -24,6 +23,7 @@ from .library import KernelError, call
 
 MAX_REQUESTS = 4096          # of step_maps
 MAX_HEAD_DIM = 512           # of store and of attention
+INF = float("inf")
 MAX_PIECES = 65535           # of a launch's grid
 PIECE_INTS = 12              # of a piece of work (csrc/cache8_attn.h)
 TILE = 64                    # keys of a step of the matrix-core kernels
@@ -73,14 +73,13 @@ def _pages(what: str, view: Paged8CacheView, nkv: int, d: int) -> Tuple[int, int
     return pages, page
 
 
-def _apart(a: torch.Tensor, a_columns: int, b: torch.Tensor, b_columns: int) -> bool:
-    """Whether the first columns of ``a``'s rows and of ``b``'s, which are as many and of one type, have no byte in common."""
-    rows, size = a.shape[0], a.element_size()
-    at_a, at_b, step_a, step_b = a.data_ptr(), b.data_ptr(), a.stride(0) * size, b.stride(0) * size
-    if at_b >= at_a + (rows - 1) * step_a + a_columns * size or at_a >= at_b + (rows - 1) * step_b + b_columns * size:
+def _apart(rows: int, size: int, at_a: int, step_a: int, a: int, at_b: int, step_b: int, b: int) -> bool:
+    """Whether ``rows`` rows of ``a`` numbers of ``size`` bytes from address ``at_a`` on, ``step_a`` numbers apart, have no byte in common with as
+    many rows of ``b`` from ``at_b`` on."""
+    if at_b >= at_a + ((rows - 1) * step_a + a) * size or at_a >= at_b + ((rows - 1) * step_b + b) * size:
         return True
-    between = (at_b - at_a) % step_a if step_a else 0      # (rows of one buffer beside each other)
-    return rows > 1 and step_a == step_b and between >= a_columns * size and between + b_columns * size <= step_a
+    between = (at_b - at_a) % (step_a * size) if step_a else 0      # (rows of one buffer beside each other)
+    return rows > 1 and step_a == step_b and between >= a * size and between + b * size <= step_a * size
 
 
 # The arguments of the entry points as the structures of csrc/cache8_maps.hip, cache8_store.hip and cache8_attn.h, put together at once.
@@ -192,11 +191,12 @@ def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, vie
     stride, q_stride = qkv.stride(0), q_out.stride(0)
     if tokens > 1 and (stride < columns or q_stride < nq * d):
         _refuse(what, "rows that overlap")
+    qkv_at, q_at = qkv.data_ptr(), q_out.data_ptr()
     if tokens and parts is None:
-        if qkv.data_ptr() == q_out.data_ptr() and (tokens == 1 or stride == q_stride):
+        if qkv_at == q_at and (tokens == 1 or stride == q_stride):
             if v_head0 < nq:
                 _refuse(what, f"values from head {v_head0} on lie among the {nq} heads of q that q_out takes the place of")
-        elif not _apart(qkv, columns, q_out, nq * d):
+        elif not _apart(tokens, qkv.element_size(), qkv_at, stride, columns, q_at, q_stride, nq * d):
             _refuse(what, "q_out overlaps rows of qkv (it may be their front, or lie apart)")
     _ints(what, "positions", positions, tokens)
     places = _block_list(what, blocks)
@@ -233,7 +233,7 @@ def store(qkv: torch.Tensor, q_out: torch.Tensor, nq: int, nkv: int, d: int, vie
     if tokens == 0:       # (whose tensors have no addresses)
         return
     call("pulse_store8", _STORE.pack(
-        qkv.data_ptr(), stride, q_out.data_ptr(), q_stride, _at(q_weight), _at(k_weight), _at(cos), _at(sin), view.keys.data_ptr(),
+        qkv_at, stride, q_at, q_stride, _at(q_weight), _at(k_weight), _at(cos), _at(sin), view.keys.data_ptr(),
         view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(), blocks.data_ptr(), _tag(qkv, what), w_tag, rotated, pairing,
         pages, page, places, tokens, nq, nkv, d, plain_norm, v_head0, every, eps, coef, _at(parts), part_stride, part_row, shares), _stream())
 
@@ -300,7 +300,7 @@ class AttentionPlan:
         # (one that no position of 32 bits reaches beyond hides nothing)
         self.window, self.chunk = (0 if v >= 2 ** 31 else int(v) for v in (window, chunk))
         self.workspace = workspace
-        self.tag = _TAG[dtype]
+        self.tag, self.size = _TAG[dtype], dtype.itemsize
         self.rows, self.entries = 0, len(entries)
         for e in entries:
             if e.first_row != self.rows or e.count < 0 or e.start < 0:
@@ -371,15 +371,14 @@ class AttentionPlan:
         add("pulse_attn8_many", MANY, many, nkv, self.MANY_NARROW_SLOTS if d in (32, 64) else self.MANY_SLOTS, self.MANY_LEAST,
             self.MANY_ROUNDS if d < 256 else (1, 1))
 
-    def on(self, stream: Any) -> Any:
-        """``stream``, the current one, which reads the lists from now on: they may have been made on another, and the plan be dropped
-        before it has come to them."""
+    def on(self, stream: Any) -> None:
+        """``stream``, the current one, reads the lists from now on: they may have been made on another, and the plan be dropped before it
+        has come to them."""
         if stream.value not in self.streams:
             self.streams.add(stream.value)
             for work in self.works:
                 for t in (work[0], work[-1]):
                     t.record_stream(torch.cuda.current_stream())
-        return stream
 
     def _tiles(self, start: int, count: int) -> int:
         """Tiles that hold keys of ``count`` tokens from position ``start`` on."""
@@ -393,7 +392,8 @@ class AttentionPlan:
         if self.device.index is not None and positions.device != self.device:
             _refuse("plan", f"it was made for {self.device}, the positions lie on {positions.device}")
         self.ready = True
-        stream = self.on(_stream())
+        stream = _stream()
+        self.on(stream)
         for items, n, slots, least, room, groups, even, shrink, cut in self.works:
             call("pulse_attn8_cut", _ptr(items), _i32(n), _ptr(positions), _i32(self.window), _i32(self.chunk), _i32(slots), _i32(least),
                  _i32(room), _i32(groups), _i32(even), _i32(shrink), _ptr(cut), stream)
@@ -440,13 +440,14 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     q_stride, o_stride = (q.stride(0), out.stride(0)) if tokens > 1 else (nq * d, nq * d)
     if q_stride < nq * d or o_stride < nq * d:
         _refuse(what, "rows that overlap")
-    if tokens and not (q.data_ptr() == out.data_ptr() and q_stride == o_stride) and not _apart(q, nq * d, out, nq * d):
+    q_at, out_at = q.data_ptr(), out.data_ptr()
+    if tokens and not (q_at == out_at and q_stride == o_stride) and not _apart(tokens, plan.size, q_at, q_stride, nq * d, out_at, o_stride, nq * d):
         _refuse(what, "out overlaps rows of q (it may be the same, or lie apart)")
     if plan.rows > tokens:
         _refuse(what, f"the plan has {plan.rows} rows, q {tokens}")
     if not plan.ready:
         _refuse(what, "the plan has not been cut for any positions")
-    if not 0.0 < scale < math.inf or not 0.0 <= softcap < math.inf:
+    if not 0.0 < scale < INF or not 0.0 <= softcap < INF:
         _refuse(what, "the scale must be positive and the cap not negative, and both finite")
     _ints(what, "positions", positions, tokens)
     _ints(what, "token_entry", token_entry, tokens)
@@ -466,7 +467,9 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
     if tokens == 0:
         return
     workspace = workspace if workspace is not None else plan.workspace
-    q_at, out_at, stream = q.data_ptr(), out.data_ptr(), plan.on(_stream())
+    stream = _stream()
+    if stream.value not in plan.streams:
+        plan.on(stream)
     calls = plan.calls if softcap <= MATRIX_CAP else PLAIN_CALLS
     if calls is not PLAIN_CALLS and (q_at % 16 or q_stride % 8 or out_at % 8 or o_stride % 4):
         _refuse(what, "rows must be aligned to 16 bytes")
@@ -476,7 +479,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
             if workspace is not None:
                 o = workspace.buffer("attention8.part_o", rows, d, torch.float32)
                 ml = workspace.buffer("attention8.part_ml", rows, 2, torch.float32)
-                place = o.data_ptr(), ml.data_ptr(), stream.value
+                part_o, part_ml = o.data_ptr(), ml.data_ptr()
+                place = part_o, part_ml, stream.value
                 if place not in plan.rooms:
                     plan.rooms[place] = o, ml
                     for t in (o, ml):          # (made on another stream, perhaps)
@@ -484,7 +488,7 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
             else:
                 o = torch.empty((rows, d), dtype=torch.float32, device=q.device)
                 ml = torch.empty((rows, 2), dtype=torch.float32, device=q.device)
-            part_o, part_ml = o.data_ptr(), ml.data_ptr()
+                part_o, part_ml = o.data_ptr(), ml.data_ptr()
         call(name, _ATTN.pack(
             q_at, q_stride, out_at, o_stride, view.keys.data_ptr(), view.values.data_ptr(), view.scales.data_ptr(), positions.data_ptr(),
             token_entry.data_ptr(), table.data_ptr(), _at(gate), gate_stride, _at(sink), items, cut, part_o, part_ml, plan.tag, plan.rows,

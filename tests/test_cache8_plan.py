@@ -32,7 +32,7 @@ def test_rows_that_lie_apart(seed):
     b = buffer.as_strided((rows, b_columns), (b_step, 1), r.randint(0, 300))
     a.fill_(1.0)
     share = bool((b == 1.0).any())
-    got = cache8._apart(a, a_columns, b, b_columns)
+    got = cache8._apart(rows, 2, a.data_ptr(), a_step, a_columns, b.data_ptr(), b_step, b_columns)
     if rows == 1 or a_step == b_step:
         assert got == (not share)
     else:                        # (rows of two steps that interleave are taken to overlap)
