@@ -7,10 +7,11 @@
 // A lane takes a key's score (its row of bytes in pieces of 16) and then channels of the sum, for which the weights come as scalars.
 // A row that sees no key is zeros; a row of no entry (token_entry outside the table) is left as it is.  Keys and values that a row does
 // not see are not multiplied, so that what is not finite stays with those who see it.
-// Bound by trips to memory (keys, then values, a wavefront's 64 keys at a time) and, with many rows, by its own arithmetic: nothing is shared
-// between rows (280 rows of up to 90 keys, 6 heads of 32, float32, 8.0 us; 24 tokens behind up to 2,000, pages of 8, 42).
+// Bound by trips to memory (keys, then values, a wavefront's 64 keys at a time: 24 tokens behind 2,000 to 600, 32 heads on 8 of 128, pages of 8, 53 us,
+// of which its wavefronts wait for data 47 %) and, with many rows, by its own arithmetic, for nothing is shared between rows or heads (float32 prompts
+// of 512 / 1,024 tokens 110 / 357 us, the vector units busy 83 %; 280 rows of up to 90 keys, 6 heads of 32, float32, 8.0).
 // It serves what the matrix-core kernels do not: float32 rows, heads that are no multiple of 16 channels from 32 on (of 32 above 128), pages that are
-// no multiple of 16 tokens.
+// no multiple of 16 tokens, caps above 256.
 #include "cache8_attn.h"
 
 namespace {
@@ -193,9 +194,11 @@ extern "C" int pulse_attn8_plain(const PulseAttn8* a, hipStream_t stream) {
     PULSE_REQUIRE(a->nq <= 65535, "attn8_plain: too many heads");
     if (a->tokens == 0) return 0;
     const int block = cache8::block_tokens(a->page_size);
-    // Few rows: as many wavefronts as a workgroup can have share a row's keys, so that each walks a quarter (a token behind 2,000, 32 heads on 8
-    // of 128, us: pages of 8 40.5 -> 20, float32 rows 25.4 -> 15.4; the same for more rows than fill the GPU, 18.5 for 10.5 at 1,700).
-    const bool few = static_cast<int64_t>(a->tokens) * a->nq <= 512;
+    // A workgroup a compute unit at the most: as many wavefronts as it can have share a row's keys, so that each walks a quarter.  Tokens of 32
+    // heads on 8 of 128 behind 2,000 (200), us, 4 / 16 wavefronts: 8 tokens, 256 workgroups, pages of 8 31.5 / 21.9 (6.3 / 6.7), float32 rows
+    // 26.1 / 17.8 (5.6 / 6.0); 14 tokens 49.7 / 51.0 (9.7 / 13.0), 43.3 / 44.2 (8.9 / 11.6); 16 tokens 47.9 / 47.4 (8.9 / 12.0), 40.7 / 38.9 (7.8 / 10.6); 18
+    // tokens 65 / 71 (11.5 / 17.6), 55 / 62 (10.3 / 15.6).
+    const bool few = static_cast<int64_t>(a->tokens) * a->nq <= 256;
     auto go = [&](auto t, auto ch, auto wide, auto vq) {
         const dim3 grid(a->tokens, a->nq);
         if (few) attn8_plain_kernel<decltype(t), decltype(ch)::value, decltype(wide)::value, decltype(vq)::value, 16><<<grid, 16 * PULSE_WAVE, 0, stream>>>(*a);
