@@ -137,10 +137,9 @@ __global__ __launch_bounds__(THREADS) void step_maps_kernel(MapArgs a) {
             const int b = find(block0, i);
             const int s = max(a.start[b], 0), c = max(a.count[b], 0);
             const int number = a.block.over(s) + i - block0[b];
-            const int from = max(number * a.block.b, s), to = min((number + 1) * a.block.b, s + c);
+            const int from = max(number * a.block.b, s), at = from - number * a.block.b;      // (the block may end behind the last position)
             const int p = page_at(b, number / a.blocks_per_page);
-            out = make_int4(row0[b] + from - s, to - from, of_pool(p) ? p * a.blocks_per_page + number % a.blocks_per_page : -1,
-                            from - number * a.block.b);
+            out = make_int4(row0[b] + from - s, min(a.block.b - at, s + c - from), of_pool(p) ? p * a.blocks_per_page + number % a.blocks_per_page : -1, at);
         }
         a.blocks[i] = out;
     }

@@ -113,7 +113,8 @@ def step_maps(start: torch.Tensor, count: torch.Tensor, *, page_size: int, num_p
     beyond the width are left out) and ``blocks`` [n, 4]: the blocks of ``block`` tokens that the step writes to, request by request
     (first row, rows, the block's number page * (page_size / block) + block in the page or -1, place in the block of the first row);
     places that are left over say "no rows".  Without ``pages``, ``table`` is read instead of written.  Rows behind the last request's are
-    left as they were; what does not fit is left out.  T < 2^31, num_pages * page_size < 2^31, B <= 4096."""
+    left as they were; what does not fit is left out.  T < 2^31, start + count < 2^31,
+    num_pages * page_size < 2^31, B <= 4096."""
     what = "step_maps"
     _here(what, (start, count, pages, table, first_row, positions, token_entry, slots, blocks))
     n = start.numel()

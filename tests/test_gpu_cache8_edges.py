@@ -410,3 +410,22 @@ def test_a_recording_outlives_the_workspace_it_was_recorded_with():
             run()
             torch.cuda.synchronize()
             assert torch.equal(out, want), i
+
+
+# ---------------------------------------------------------------------------------------------------- the last positions' maps
+@pytest.mark.parametrize("start,count", [(2 ** 31 - 40, 39), (2 ** 31 - 16, 15), (2 ** 31 - 2, 1), (2 ** 31 - 17, 1)])
+def test_maps_of_the_last_positions(start, count):
+    """Rows up to the last position that a length of 32 bits leaves, in pages of 2^20 tokens."""
+    require_gpu()
+    from pulse_infer_amd.ops import cache8
+
+    page, pool = 1 << 20, 2047
+    pages = [(7 * i) % pool for i in range(2048)]
+    want = plain.maps([(start, count), (0, 3)], pages + [5], page, pool, 2048)
+    n = count + 3
+    got = dict(positions=ints([-9] * n), token_entry=ints([-9] * n), slots=ints([-9] * n), first_row=ints([-9] * 3),
+               blocks=torch.full((len(want["blocks"]), 4), -9, dtype=torch.int32, device=DEV), table=torch.full((2, 2048), -9, dtype=torch.int32, device=DEV))
+    assert cache8.blocks_touched(metas([(start, count), (0, 3)]), page) == len(want["blocks"])
+    cache8.step_maps(ints([start, 0]), ints([count, 3]), page_size=page, num_pages=pool, pages=ints(pages + [5]), **got)
+    for name, t in got.items():
+        assert t.tolist() == want[name], name
