@@ -354,6 +354,8 @@ class AttentionPlan:
                         low = middle + 1
                 items = [it for _, it in sorted(zip(tiles, items), key=lambda x: -(-x[0] // -(-x[0] // low)), reverse=True)]
             on_gpu = to_device([v for _, row, rows, entry in items for v in (row, rows, entry, 0)])
+            _need(on_gpu.dtype == torch.int32 and on_gpu.device == self.device and on_gpu.is_contiguous() and on_gpu.numel() >= 4 * n,
+                  f"plan: to_device must give {4 * n} contiguous int32 numbers on {self.device}")
             here = int(columns == FEW or slots <= self.MANY_HERE * n)
             counters = n * groups if here else 0
             cut = torch.empty(PIECE_INTS * room + 2 * n + counters, dtype=torch.int32, device=self.device)

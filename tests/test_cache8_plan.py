@@ -7,7 +7,7 @@ import torch
 from test_cache8_host import metas
 
 from pulse_infer_amd.cache import CacheManager, Paged8KVSpec, PagedKVSpec
-from pulse_infer_amd.ops import cache8
+from pulse_infer_amd.ops import KernelError, cache8
 
 
 def test_a_plan_is_one_devices(monkeypatch):
@@ -79,3 +79,10 @@ def test_portions_of_uneven_walks_are_cut_where_they_fill_the_gpu(monkeypatch):
     assert room([(8000, 300), (0, 2000)]) == room([(6000, 600), (0, 2000)]) == 3      # (the items and twice as many)
     assert room([(0, 2048)]) == room([(0, 2600)]) == room([(0, 1044), (0, 1668)]) == room([(8000, 2048)]) == 1
     assert room([(8000, 300), (0, 2000)], d=256) == 2
+
+
+@pytest.mark.parametrize("send", [lambda v: torch.tensor(v), lambda v: torch.tensor(v, dtype=torch.int32)[:-1], lambda v: torch.tensor(v + v, dtype=torch.int32)[::2],
+                                  lambda v: torch.tensor(v, dtype=torch.int32, device="meta")])
+def test_lists_that_are_not_what_the_kernels_read_are_refused(send):
+    with pytest.raises(KernelError, match="to_device"):
+        cache8.AttentionPlan(metas([(40, 1), (0, 3)]), 4, 2, 32, page_size=16, dtype=torch.bfloat16, device="cpu", to_device=send)
