@@ -485,6 +485,8 @@ def attention(q: torch.Tensor, out: torch.Tensor, plan: AttentionPlan, view: Pag
                 part_o, part_ml = o.data_ptr(), ml.data_ptr()
                 place = part_o, part_ml, stream.value
                 if place not in plan.rooms:
+                    if o.get_device() != q.get_device():
+                        _refuse(what, f"the workspace is on {o.device}, q on {q.device}")
                     plan.rooms[place] = o, ml
                     for t in (o, ml):          # (made on another stream, perhaps)
                         t.record_stream(torch.cuda.current_stream())

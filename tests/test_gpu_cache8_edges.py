@@ -429,3 +429,20 @@ def test_maps_of_the_last_positions(start, count):
     cache8.step_maps(ints([start, 0]), ints([count, 3]), page_size=page, num_pages=pool, pages=ints(pages + [5]), **got)
     for name, t in got.items():
         assert t.tolist() == want[name], name
+
+
+def test_a_workspace_of_another_device_is_refused():
+    """Room for joined pieces that the GPU's kernels cannot write to."""
+    require_gpu()
+    from pulse_infer_amd.ops import KernelError, cache8
+    from pulse_infer_amd.parts.base import Workspace
+
+    view, positions = view_of(plain.Cache(80, 2, 16, 32)), ints([1200])
+    q = torch.zeros((1, 128), dtype=torch.bfloat16, device=DEV)
+    table = ints([list(range(76))])
+    for ws, call in ((Workspace(torch.device("cpu")), None), (None, Workspace(torch.device("cpu")))):
+        made = cache8.plan(metas([(1200, 1)]), 4, 2, 32, positions, page_size=16, dtype=torch.bfloat16, workspace=ws)
+        assert made.calls[0][5] > 0
+        for _ in range(2):
+            with pytest.raises(KernelError, match="workspace"):
+                cache8.attention(q, q.clone(), made, view, positions, ints([0]), table, 1.0, workspace=call)
