@@ -405,11 +405,12 @@ class AttentionPlan:
 
 def plan(entries: Sequence[Any], nq: int, nkv: int, d: int, positions: torch.Tensor, *, page_size: int, dtype: torch.dtype,
          window: int = 0, chunk: int = 0, workspace: Any = None, to_device: Optional[Callable] = None) -> AttentionPlan:
-    """The attention of a step of ``entries`` (``EntryMeta``: start, count, first_row; one's rows behind the other's from row 0 on, at
-    positions that follow each other) whose rows stand at ``positions``, for layers of these heads.  It is made outside a recording; a step of the same shape takes the same plan, cut anew (``AttentionPlan.cut``, which may be
-    recorded).  A plan, its counters among it, serves calls that follow each other, on whichever stream.  ``workspace`` (a ``Workspace``):
-    where the room for joined pieces comes from, for calls and replays that follow each other; without one every call takes it from
-    torch's pool.  A recording needs its plan (the lists, and the room that it was recorded with) for as long as it is replayed."""
+    """The attention of a step of ``entries`` (``EntryMeta``: start, count, first_row; one's rows behind the other's from row 0 on, at positions
+    that follow each other) whose rows stand at ``positions``, for layers of these heads.  It is made outside a recording; a step of the same
+    shape takes the same plan, cut anew (``AttentionPlan.cut``, which may be recorded).  A plan, its counters among it, serves calls that follow
+    each other, on whichever stream.  ``workspace`` (a ``Workspace``): where the room for joined pieces comes from, for calls and replays that
+    follow each other; without one every call takes it from torch's pool.  A recording needs its plan (the lists, and the room that it was
+    recorded with) for as long as it is replayed."""
     return AttentionPlan(entries, nq, nkv, d, page_size=page_size, dtype=dtype, window=window, chunk=chunk, device=positions.device,
                          workspace=workspace, to_device=to_device).cut(positions)
 
