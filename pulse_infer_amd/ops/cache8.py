@@ -389,11 +389,13 @@ class AttentionPlan:
         return (start + count - 1) // TILE + 1 - low // TILE
 
     def cut(self, positions: torch.Tensor) -> "AttentionPlan":
-        """Shares the keys out for the rows' ``positions``: for every step, before its first ``attention``."""
+        """Shares the keys out for the rows' ``positions``: for every step, before its first ``attention``; the first time outside a recording."""
         _here("plan", (positions,))
         _ints("plan", "positions", positions, self.rows)
         if self.device.index is not None and positions.device != self.device:
             _refuse("plan", f"it was made for {self.device}, the positions lie on {positions.device}")
+        if not self.ready and self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            _refuse("plan", "its first cut cannot be a recorded one, behind which nothing has been shared out yet")
         self.ready = True
         stream = _stream()
         self.on(stream)

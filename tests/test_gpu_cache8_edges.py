@@ -446,3 +446,34 @@ def test_a_workspace_of_another_device_is_refused():
         for _ in range(2):
             with pytest.raises(KernelError, match="workspace"):
                 cache8.attention(q, q.clone(), made, view, positions, ints([0]), table, 1.0, workspace=call)
+
+
+def test_the_first_cut_is_no_recorded_one():
+    """Behind a recording that has not been replayed nothing is shared out: a call outside it would follow a list that nobody has written."""
+    require_gpu()
+    from pulse_infer_amd.ops import KernelError, cache8
+
+    view, positions, table = view_of(plain.Cache(80, 2, 16, 32)), ints([1200]), ints([list(range(76))])
+    q = torch.zeros((1, 128), dtype=torch.bfloat16, device=DEV)
+    out, other = q.clone(), q.clone()
+    made = cache8.AttentionPlan(metas([(1200, 1)]), 4, 2, 32, page_size=16, dtype=torch.bfloat16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other.add_(1.0)
+        with pytest.raises(KernelError, match="first cut"):
+            made.cut(positions)
+    with pytest.raises(KernelError, match="not been cut"):
+        cache8.attention(q, out, made, view, positions, ints([0]), table, 1.0)
+    made.cut(positions)
+    cache8.attention(q, out, made, view, positions, ints([0]), table, 1.0)
+    again = torch.cuda.CUDAGraph()
+    zero = ints([0])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(again):
+        made.cut(positions)
+        cache8.attention(q, out, made, view, positions, zero, table, 1.0)
+    for _ in range(3):
+        graph.replay()
+        again.replay()
+        torch.cuda.synchronize()
+    assert (other == 3.0).all() and torch.isfinite(out).all()
